@@ -27,6 +27,13 @@ PRECISION_F16 = 2
 DECODE_RANDOM = 0
 DECODE_N_TO_C = 1
 DECODE_INPUT = 2
+F32 = 0
+F16 = 1
+BF16 = 2
+F64 = 3
+VOCAB_MAX = 262144
+VOCAB_ROWS_MAX = 134217728
+LISTING_MAX = 1024
 
 # Every symbol include/hkb_mpnn.h declares.
 EXPORTED = ["hkb_mpnn_create", "hkb_mpnn_destroy", "hkb_mpnn_design",
@@ -36,7 +43,8 @@ EXPORTED = ["hkb_mpnn_create", "hkb_mpnn_destroy", "hkb_mpnn_design",
             "hkb_mpnn_abi_version",
             "hkb_structure_load_file", "hkb_structure_load_text", "hkb_structure_residue_count",
             "hkb_structure_copy", "hkb_structure_destroy", "hkb_backbone_noise",
-            "hkb_write_design_fasta", "hkb_write_logprobs_npz"]
+            "hkb_write_design_fasta", "hkb_write_logprobs_npz",
+            "hkb_sample_tokens", "hkb_top_logits", "hkb_distill"]
 
 
 class StructureOptions(ctypes.Structure):
@@ -70,6 +78,36 @@ class ScoreBatch(ctypes.Structure):
 
 class ScoreOut(ctypes.Structure):
     _fields_ = [("log_probs", c_void_p), ("orders", c_void_p), ("scores", c_void_p)]
+
+
+class VocabRows(ctypes.Structure):
+    _fields_ = [("rows", c_int64), ("vocab", c_int32), ("dtype", c_int32), ("logits", c_void_p),
+                ("row_stride", c_int64)]
+
+
+class SampleSettings(ctypes.Structure):
+    _fields_ = [("temperatures", c_void_p), ("top_ks", c_void_p), ("top_ps", c_void_p),
+                ("min_ps", c_void_p), ("temperature", c_float), ("top_k", c_int32),
+                ("top_p", c_float), ("min_p", c_float), ("uniforms", c_void_p),
+                ("uniforms_dtype", c_int32)]
+
+
+class SampleOut(ctypes.Structure):
+    _fields_ = [("tokens", c_void_p), ("log_probs", c_void_p), ("kept", c_void_p)]
+
+
+class TopOut(ctypes.Structure):
+    _fields_ = [("values", c_void_p), ("tokens", c_void_p), ("log_norm", c_void_p)]
+
+
+class DistillTeacher(ctypes.Structure):
+    _fields_ = [("k", c_int32), ("dtype", c_int32), ("values", c_void_p), ("tokens", c_void_p),
+                ("log_norm", c_void_p), ("temperature", c_float)]
+
+
+class DistillOut(ctypes.Structure):
+    _fields_ = [("loss", c_void_p), ("grad", c_void_p), ("grad_row_stride", c_int64),
+                ("row_weights", c_void_p), ("row_weight_stride", c_int64)]
 
 
 class HkbError(RuntimeError):
@@ -139,6 +177,15 @@ def load() -> ctypes.CDLL:
                                            c_void_p, c_float, c_int32]
     lib.hkb_write_logprobs_npz.restype = Status
     lib.hkb_write_logprobs_npz.argtypes = [c_char_p, c_int32, c_int32, c_void_p]
+    lib.hkb_sample_tokens.restype = Status
+    lib.hkb_sample_tokens.argtypes = [c_int, POINTER(VocabRows), POINTER(SampleSettings),
+                                      POINTER(SampleOut), c_void_p]
+    lib.hkb_top_logits.restype = Status
+    lib.hkb_top_logits.argtypes = [c_int, POINTER(VocabRows), c_int32, c_float, POINTER(TopOut),
+                                   c_void_p]
+    lib.hkb_distill.restype = Status
+    lib.hkb_distill.argtypes = [c_int, POINTER(VocabRows), POINTER(DistillTeacher),
+                                POINTER(DistillOut), c_void_p]
     _lib = lib
     return lib
 
@@ -149,4 +196,5 @@ def check(st: Status) -> None:
 
 
 __all__ = ["load", "check", "Status", "DesignBatch", "DesignOut", "ScoreBatch", "ScoreOut",
-           "StructureOptions", "HkbError", "EXPORTED", "c_uint8"]
+           "StructureOptions", "VocabRows", "SampleSettings", "SampleOut", "TopOut",
+           "DistillTeacher", "DistillOut", "HkbError", "EXPORTED", "c_uint8"]

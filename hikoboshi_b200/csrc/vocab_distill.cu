@@ -1,0 +1,268 @@
+// Divergence of student rows from a teacher's listed logits, and its gradient.
+//
+// With M the row's largest logit, S = sum exp((x_i - M) / tau) and the
+// teacher's masses q_k (in 64 bits, K of them), the loss needs S, the K listed
+// logits and, where the unlisted tokens form a class, their own sum.  That sum
+// is taken over the row with the listed entries replaced by -inf, not as a
+// difference of sums: a student that puts almost everything on the list would
+// lose it to cancellation.  The gradient is e_i G for every unlisted token,
+// with e_i recomputed from the row in shared memory and one factor G per row,
+// and is set entry by entry on the list.
+#include "hkb_mpnn.h"
+#include "kernels.hpp"
+#include "vocab.hpp"
+#include "vocab_rows.cuh"
+
+namespace hkb {
+namespace vocab {
+namespace {
+
+constexpr double kLog2e = 1.4426950408889634074;
+
+template <int kBytes>
+struct BitsOf;
+template <>
+struct BitsOf<4> {
+  using type = uint32_t;
+};
+template <>
+struct BitsOf<2> {
+  using type = uint16_t;
+};
+
+__device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i) {
+  if (dtype == HKB_F32) return static_cast<const float*>(p)[i];
+  if (dtype == HKB_F16) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+struct DistillSmem {
+  ReduceScratch cluster;
+  ReduceScratch block;
+};
+
+// Listing of a row in shared memory, behind the slice's buffer.
+struct Listing {
+  double* q;   // teacher's mass
+  float* x;    // student's logit, where this CTA owns the entry
+  int* token;  // -1: no entry
+  int* own;    // 1: this CTA's slice has the token and this entry stands for it
+};
+
+// Writes one value over the row's slice of the gradient.
+template <typename T, bool kClustered>
+__device__ void fill_slice(const RowSlice<T, kClustered>& row, T* grad, float value) {
+  for (int i = threadIdx.x; i < row.n; i += blockDim.x) grad[row.start + i] = narrow<T>(value);
+}
+
+template <typename T, bool kClustered>
+__global__ void __launch_bounds__(kMaxThreads) distill_rows_kernel(
+    const T* logits, int64_t row_stride, int vocab, int chunk, int slice_bytes, DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ DistillSmem sm;
+  using Bits = typename BitsOf<sizeof(T)>::type;
+  constexpr int kE = Vec<T>::kN;
+  const int cluster = kClustered ? (int)cg::this_cluster().num_blocks() : 1;
+  const int64_t r = blockIdx.x / cluster;
+  RowSlice<T, kClustered> row;
+  const T* g = logits + r * row_stride;
+  row.init(reinterpret_cast<T*>(smem_raw), g, vocab, chunk);
+  row.load(g);
+  Listing ls;
+  ls.q = reinterpret_cast<double*>(smem_raw + slice_bytes);
+  ls.x = reinterpret_cast<float*>(ls.q + a.k);
+  ls.token = reinterpret_cast<int*>(ls.x + a.k);
+  ls.own = ls.token + a.k;
+
+  // the teacher's masses, while the row is on its way
+  const bool tail = a.log_norm != nullptr;
+  const double inv_tau = 1.0 / (double)a.temperature;
+  Reducer<false> block(&sm.block);
+  float amax = -CUDART_INF_F;
+  bool any = false, bad = false;
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+    int token = a.tokens[r * a.k + k];
+    if (token < 0 || v == -CUDART_INF_F) token = -1;
+    bad |= token >= vocab;
+    any |= token >= 0;
+    if (token >= 0) amax = fmaxf(amax, v);
+    ls.token[k] = token;
+    ls.x[k] = v;
+  }
+  const bool row_bad = __syncthreads_or(bad), row_any = __syncthreads_or(any);
+  cp_async_wait_all();
+  if (kClustered) cg::this_cluster().sync();
+  else __syncthreads();
+  T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
+  const bool writer = threadIdx.x == 0 && row.rank == 0;
+  if (row_bad || !row_any) {
+    const float v = row_bad ? CUDART_NAN_F : 0.0f;
+    const bool zero_weight =
+        a.row_weights != nullptr && a.row_weights[r * a.row_weight_stride] == 0.0f;
+    if (writer && a.loss) a.loss[r] = v;
+    if (grad) fill_slice(row, grad, zero_weight ? 0.0f : v);
+    return;
+  }
+  // log q_k = a_k / tau - norm, in natural logarithms
+  double norm;
+  if (tail) {
+    norm = (double)a.log_norm[r];
+  } else {
+    amax = block.max(amax);
+    double e = 0.0;
+    for (int k = threadIdx.x; k < a.k; k += blockDim.x)
+      if (ls.token[k] >= 0) e += exp(((double)ls.x[k] - (double)amax) * inv_tau);
+    norm = (double)amax * inv_tau + log(block.sum(e));
+  }
+  double q_sum = 0.0, dot = 0.0;  // sum q, sum over owned entries q (log q - z)
+  float listed_max = -CUDART_INF_F;
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    const int token = ls.token[k];
+    double q = 0.0;
+    int own = 0;
+    if (token >= 0) {
+      const double log_q = (double)ls.x[k] * inv_tau - norm;
+      q = exp(log_q);
+      q_sum += q;
+      const int at = token - row.start;
+      if (at >= 0 && at < row.n) {
+        const float x = widen(row.s[row.ph + at]);
+        ls.x[k] = x;
+        listed_max = fmaxf(listed_max, x);
+        // a mass that underflows counts nothing, also on a masked token
+        if (q != 0.0) dot += q * (log_q - (double)x * inv_tau);
+        own = 1;
+      }
+    }
+    ls.q[k] = q;
+    ls.own[k] = own;
+  }
+  q_sum = block.sum(q_sum);
+  // One entry stands for a token that is listed more than once: each writes
+  // its number in the token's place, the one that is found there stays.  Then
+  // the place gets -inf (unlisted class) or its logit back.
+  __syncthreads();
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x)
+    if (ls.own[k])
+      reinterpret_cast<Bits*>(row.s)[row.ph + ls.token[k] - row.start] = (Bits)k;
+  __syncthreads();
+  bool twice = false;
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x)
+    if (ls.own[k] && reinterpret_cast<Bits*>(row.s)[row.ph + ls.token[k] - row.start] != (Bits)k) {
+      ls.own[k] = 0;
+      twice = true;
+    }
+  const bool row_twice = __syncthreads_or(twice);
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x)
+    if (ls.own[k])
+      row.s[row.ph + ls.token[k] - row.start] = narrow<T>(tail ? -CUDART_INF_F : ls.x[k]);
+  __syncthreads();
+
+  Reducer<kClustered> red(&sm.cluster);
+  float bmax = -CUDART_INF_F;
+  row.for_each([&](int, const Vec<T>& x) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) bmax = fmaxf(bmax, widen(x.v[e]));
+  });
+  bmax = red.max(bmax);           // of the body: all tokens, or the unlisted ones
+  listed_max = red.max(listed_max);
+  const float xmax = fmaxf(bmax, listed_max);
+  const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
+  const float c = (float)(kLog2e * inv_tau);
+  float s = 0.0f;
+  row.for_each([&](int, const Vec<T>& x) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) s += exp2_fast((widen(x.v[e]) - base) * c);
+  });
+  double listed = 0.0;  // sum over listed tokens exp((x - xmax) / tau)
+  if (tail)
+    for (int k = threadIdx.x; k < a.k; k += blockDim.x)
+      if (ls.own[k]) listed += exp(((double)ls.x[k] - (double)xmax) * inv_tau);
+  const double body = red.sum((double)s);
+  if (tail) listed = red.sum(listed);
+  dot = red.sum(dot);
+  const double lift = bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
+  const double total = body * lift + listed;  // relative to xmax
+  const double log_total = (double)xmax * inv_tau + log(total);
+  double rest_q = 0.0;
+  if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
+  const double mass = tail ? q_sum + rest_q : 1.0;
+  if (writer && a.loss) {
+    double l = dot + (tail ? q_sum : 1.0) * log_total;
+    if (rest_q > 0.0)
+      l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
+    const double tau = (double)a.temperature;
+    a.loss[r] = (float)(tau * tau * l);
+  }
+  if (grad == nullptr) return;
+  const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+  if (weight == 0.0f) {
+    fill_slice(row, grad, 0.0f);
+    return;
+  }
+  const double wt = (double)weight * (double)a.temperature;
+  double factor = mass * lift / total;
+  if (rest_q > 0.0) factor -= rest_q / body;
+  const float G = (float)(wt * factor);
+  T* gs = grad + row.start - row.ph;  // element e0 of the slice's vectors goes to gs[e0]
+  const bool same_phase = (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
+  row.for_each([&](int i0, const Vec<T>& x) {
+    Vec<T> y;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) y.v[e] = narrow<T>(exp2_fast((widen(x.v[e]) - base) * c) * G);
+    const int e0 = i0 - row.start + row.ph;
+    if (same_phase && e0 >= row.ph && e0 + kE <= row.ph + row.n) {
+      *reinterpret_cast<Vec<T>*>(gs + e0) = y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        if (e0 + e >= row.ph && e0 + e < row.ph + row.n) gs[e0 + e] = y.v[e];
+    }
+  });
+  __syncthreads();
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    if (!ls.own[k]) continue;
+    double q = ls.q[k];
+    if (row_twice) {
+      q = 0.0;
+      for (int j = 0; j < a.k; ++j)
+        if (ls.token[j] == ls.token[k]) q += ls.q[j];
+    }
+    const double p = exp(((double)ls.x[k] - (double)xmax) * inv_tau) / total;
+    grad[ls.token[k]] = narrow<T>((float)(wt * (mass * p - q)));
+  }
+}
+
+template <typename T>
+cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(v.rows * s.cluster));
+  cfg.blockDim = dim3((unsigned)s.threads);
+  cfg.dynamicSmemBytes = s.smem + (size_t)a.k * 20;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)s.cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  auto kernel = s.cluster > 1 ? distill_rows_kernel<T, true> : distill_rows_kernel<T, false>;
+  ensure_dynamic_smem((const void*)kernel, 131072 + 16 + HKB_LISTING_MAX * 20);
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(v.logits), v.row_stride, v.vocab,
+                            s.chunk, (int)s.smem, a);
+}
+
+}  // namespace
+}  // namespace vocab
+
+cudaError_t launch_distill(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  switch (v.dtype) {
+    case HKB_F32: return vocab::launch<float>(st, v, a);
+    case HKB_F16: return vocab::launch<__half>(st, v, a);
+    default: return vocab::launch<__nv_bfloat16>(st, v, a);
+  }
+}
+
+}  // namespace hkb

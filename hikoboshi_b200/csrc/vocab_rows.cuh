@@ -1,0 +1,216 @@
+// Shared device code of the operators on vocabulary rows (vocab_sample.cu,
+// vocab_top.cu, vocab_distill.cu).
+//
+// A row is V logits of one position, f32, fp16 or bf16.  A cluster of C CTAs
+// (C = 1, 2, 4 or 8) holds one row in its shared memory, CTA c the slice
+// [c * chunk, min(V, (c + 1) * chunk)), so every pass after the first reads
+// shared memory and the row crosses HBM once.  C grows with V (a slice has to
+// fit) and when there are few rows (a row is then read by more SMs).
+//
+// Slices are kept in the 16-byte phase of their global addresses: element i of
+// the slice sits at index ph + i, so whole 16-byte vectors are copied by
+// cp.async whatever the row's alignment, and every pass reads 16-byte vectors.
+// The ph elements in front and those behind the slice up to the vector's end
+// hold -inf, which no operator selects and whose weight is zero.
+#pragma once
+
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math_constants.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace hkb {
+namespace vocab {
+
+namespace cg = cooperative_groups;
+
+constexpr int kMaxThreads = 512;
+constexpr int kMaxWarps = kMaxThreads / 32;
+constexpr int kMaxCluster = 8;
+
+__device__ __forceinline__ float widen(float x) { return x; }
+__device__ __forceinline__ float widen(__half x) { return __half2float(x); }
+__device__ __forceinline__ float widen(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T narrow(float x);
+template <>
+__device__ __forceinline__ float narrow<float>(float x) {
+  return x;
+}
+template <>
+__device__ __forceinline__ __half narrow<__half>(float x) {
+  return __float2half_rn(x);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) {
+  return __float2bfloat16_rn(x);
+}
+
+// 16 bytes of a row.
+template <typename T>
+struct alignas(16) Vec {
+  static constexpr int kN = 16 / (int)sizeof(T);
+  T v[kN];
+};
+
+// Order-preserving key of a value: a < b <=> key(a) < key(b); -0 and +0 share
+// one key.  NaN never reaches it (rows are cleaned on load).
+__device__ __forceinline__ uint32_t order_key(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+constexpr uint32_t kKeyNegInf = 0x007fffffu;  // order_key(-inf)
+
+// 2^t for t <= 0 in 64 bits: t = n + f with |f| <= 1/2, 2^f = e^(f ln 2) by its
+// Taylor series to the 12th power (remainder 0.347^13 / 13! = 1.7e-16), then
+// the exponent.  0 below 2^-1020.  The choice of a token compares sums of such
+// weights with each other; in 64 bits a sum over 2^18 tokens keeps 1e-13, so
+// the token is the formula's unless the uniform lies that close to a border.
+__device__ __forceinline__ double exp2_neg(double t) {
+  const double shift = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer
+  const double tn = __dadd_rn(t, shift);
+  const int n = __double2loint(tn);
+  const double y = __dmul_rn(__dsub_rn(t, __dsub_rn(tn, shift)), 0.693147180559945309417);
+  double p = 1.0 / 479001600.0;
+  p = fma(p, y, 1.0 / 39916800.0);
+  p = fma(p, y, 1.0 / 3628800.0);
+  p = fma(p, y, 1.0 / 362880.0);
+  p = fma(p, y, 1.0 / 40320.0);
+  p = fma(p, y, 1.0 / 5040.0);
+  p = fma(p, y, 1.0 / 720.0);
+  p = fma(p, y, 1.0 / 120.0);
+  p = fma(p, y, 1.0 / 24.0);
+  p = fma(p, y, 1.0 / 6.0);
+  p = fma(p, y, 0.5);
+  p = fma(p, y, 1.0);
+  p = fma(p, y, 1.0);
+  const double r = __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p));
+  return t > -1020.0 ? r : 0.0;
+}
+
+// 2^x on the special-function unit (2 ulp over the range used here).
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// The slice of a row that one CTA holds, and the cluster it belongs to.
+template <typename T, bool kClustered>
+struct RowSlice {
+  static constexpr int kE = Vec<T>::kN;
+  T* s;          // shared memory, 16-byte aligned
+  int ph;        // first element of the slice is s[ph]
+  int n;         // elements of the slice
+  int nvec;      // 16-byte vectors that hold them
+  int start;     // index in the row of the slice's first element
+  int rank;      // CTA of the cluster
+  int size;      // CTAs of the cluster
+  int per_warp;  // vectors of a warp: warp w owns [w * per_warp, (w + 1) * per_warp)
+
+  __device__ __forceinline__ void init(T* smem, const T* row, int vocab, int chunk) {
+    if (kClustered) {
+      rank = (int)cg::this_cluster().block_rank();
+      size = (int)cg::this_cluster().num_blocks();
+    } else {
+      rank = 0;
+      size = 1;
+    }
+    s = smem;
+    start = min(vocab, rank * chunk);
+    n = min(vocab - start, chunk);
+    ph = (int)((reinterpret_cast<uintptr_t>(row + start) & 15) / sizeof(T));
+    nvec = n > 0 ? (ph + n + kE - 1) / kE : 0;
+    const int warps = (int)blockDim.x >> 5;
+    per_warp = (nvec + warps - 1) / warps;
+  }
+
+  // Copies the slice (asynchronously where whole vectors lie inside it); the
+  // caller waits with cp_async_wait_all and a barrier.
+  __device__ __forceinline__ void load(const T* row) {
+    const T* g = row + start - ph;  // 16-byte aligned; read only at [ph, ph + n)
+    const T lowest = narrow<T>(-CUDART_INF_F);
+    for (int v = threadIdx.x; v < nvec; v += blockDim.x) {
+      const int e0 = v * kE;
+      if (e0 >= ph && e0 + kE <= ph + n) {
+        cp_async16(s + e0, g + e0, true);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+          s[e0 + e] = (e0 + e >= ph && e0 + e < ph + n) ? g[e0 + e] : lowest;
+      }
+    }
+    cp_async_commit();
+  }
+
+  // f(first element index of the vector in the row, vector) over this warp's
+  // vectors, in the order of their indices over the lanes.
+  template <typename F>
+  __device__ __forceinline__ void for_each(F f) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int end = min(nvec, (warp + 1) * per_warp);
+    for (int v = warp * per_warp + lane; v < end; v += 32)
+      f(v * kE - ph + start, reinterpret_cast<Vec<T>*>(s)[v]);
+  }
+};
+
+// Reductions over the CTA and its cluster; every thread gets the result, the
+// same bits in every CTA.  The partial results are added in a fixed order.
+struct ReduceScratch {
+  alignas(8) unsigned char warp[2][kMaxWarps * 8];
+  alignas(8) unsigned char cta[2][kMaxCluster * 8];
+};
+
+template <bool kClustered>
+struct Reducer {
+  ReduceScratch* sc;
+  int buf;
+
+  __device__ __forceinline__ explicit Reducer(ReduceScratch* s) : sc(s), buf(0) {}
+
+  template <typename V, typename Op>
+  __device__ __forceinline__ V all(V v, Op op) {
+    static_assert(sizeof(V) <= 8, "one slot is 8 bytes");
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+    V* part = reinterpret_cast<V*>(sc->warp[buf]);
+    if (lane == 0) part[warp] = v;
+    __syncthreads();
+    V r = part[0];
+    for (int w = 1; w < warps; ++w) r = op(r, part[w]);
+    if (kClustered) {
+      // each CTA writes its value into every CTA's slots; two buffers, so a
+      // slot is written again only after the next reduction's barrier
+      auto cl = cg::this_cluster();
+      const int size = (int)cl.num_blocks();
+      V* slots = reinterpret_cast<V*>(sc->cta[buf]);
+      if ((int)threadIdx.x < size) cl.map_shared_rank(slots, threadIdx.x)[cl.block_rank()] = r;
+      cl.sync();
+      r = slots[0];
+      for (int c = 1; c < size; ++c) r = op(r, slots[c]);
+    }
+    buf ^= 1;
+    return r;
+  }
+
+  template <typename V>
+  __device__ __forceinline__ V sum(V v) {
+    return all(v, [](V a, V b) { return a + b; });
+  }
+  template <typename V>
+  __device__ __forceinline__ V max(V v) {
+    return all(v, [](V a, V b) { return a > b ? a : b; });
+  }
+};
+
+}  // namespace vocab
+}  // namespace hkb

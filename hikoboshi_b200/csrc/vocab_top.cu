@@ -1,0 +1,164 @@
+// The k largest logits of each vocabulary row in the order (logit down, index
+// up), with the row's log-sum-exp.
+#include "hkb_mpnn.h"
+#include "kernels.hpp"
+#include "vocab.hpp"
+#include "vocab_rows.cuh"
+
+namespace hkb {
+namespace vocab {
+namespace {
+
+constexpr float kLog2ef = 1.44269504f;
+
+struct TopSmem {
+  ReduceScratch red;
+  unsigned count;
+  unsigned long long list[HKB_LISTING_MAX];  // key << 32 | ~index
+};
+
+template <typename T, bool kClustered>
+__global__ void __launch_bounds__(kMaxThreads) top_rows_kernel(const T* __restrict__ logits,
+                                                               int64_t row_stride, int vocab,
+                                                               int chunk, TopArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ TopSmem sm;
+  constexpr int kE = Vec<T>::kN;
+  const int cluster = kClustered ? (int)cg::this_cluster().num_blocks() : 1;
+  const int64_t r = blockIdx.x / cluster;
+  RowSlice<T, kClustered> row;
+  const T* g = logits + r * row_stride;
+  row.init(reinterpret_cast<T*>(smem_raw), g, vocab, chunk);
+  row.load(g);
+  if (threadIdx.x == 0) sm.count = 0;
+  cp_async_wait_all();
+  if (kClustered) cg::this_cluster().sync();
+  else __syncthreads();
+  Reducer<kClustered> red(&sm.red);
+
+  uint32_t kmax = 0;
+  row.for_each([&](int, Vec<T>& x) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const float v = widen(x.v[e]);
+      if (v != v) x.v[e] = narrow<T>(-CUDART_INF_F);
+      else kmax = ::max(kmax, order_key(v));
+    }
+  });
+  kmax = red.max(kmax);
+  const float xmax = key_value(kmax);
+  if (a.log_norm) {
+    const float c = kLog2ef / a.temperature;
+    float s = 0.0f;
+    row.for_each([&](int, const Vec<T>& x) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float v = widen(x.v[e]);
+        s += exp2_fast((v == xmax ? 0.0f : v - xmax) * c);
+      }
+    });
+    const double total = red.sum((double)s);
+    if (threadIdx.x == 0 && row.rank == 0)
+      a.log_norm[r] = kmax <= kKeyNegInf ? -CUDART_INF_F
+                                         : (float)((double)xmax / (double)a.temperature + log(total));
+  }
+  // k-th largest key, and of the tokens that share it the last index taken
+  uint32_t t = kKeyNegInf + 1;
+  int icut = 0x7fffffff;
+  auto count = [&](uint32_t lo, int last) {
+    int c = 0;
+    row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const uint32_t k = order_key(widen(x.v[e]));
+        c += k > lo || (k == lo && i0 + e <= last);
+      }
+    });
+    return red.sum(c);
+  };
+  int n = count(t, icut);
+  if (n > a.k) {
+    uint32_t lo = t, hi = kmax;
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      if (count(mid, 0x7fffffff) >= a.k) lo = mid;
+      else hi = mid - 1;
+    }
+    t = lo;
+    int i_lo = 0, i_hi = vocab - 1;
+    while (i_lo < i_hi) {
+      const int mid = (i_lo + i_hi) / 2;
+      if (count(t, mid) >= a.k) i_hi = mid;
+      else i_lo = mid + 1;
+    }
+    icut = i_lo;
+    n = a.k;
+  }
+  unsigned* counter = &sm.count;
+  unsigned long long* list = sm.list;
+  if (kClustered) {
+    counter = cg::this_cluster().map_shared_rank(counter, 0);
+    list = cg::this_cluster().map_shared_rank(list, 0);
+  }
+  row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const uint32_t k = order_key(widen(x.v[e]));
+      if (k > t || (k == t && i0 + e <= icut)) {
+        const unsigned at = atomicAdd(counter, 1u);
+        list[at] = ((unsigned long long)k << 32) | (uint32_t)~(i0 + e);
+      }
+    }
+  });
+  if (kClustered) cg::this_cluster().sync();
+  else __syncthreads();
+  if (row.rank != 0) return;
+  T* values = static_cast<T*>(a.values) + r * a.k;
+  int32_t* tokens = a.tokens + r * a.k;
+  for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
+    if (i >= n) {
+      values[i] = narrow<T>(-CUDART_INF_F);
+      tokens[i] = -1;
+      continue;
+    }
+    const unsigned long long me = sm.list[i];
+    int place = 0;
+    for (int j = 0; j < n; ++j) place += sm.list[j] > me;
+    const int index = (int)~(uint32_t)me;
+    values[place] = g[index];
+    tokens[place] = index;
+  }
+}
+
+template <typename T>
+cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
+  const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(v.rows * s.cluster));
+  cfg.blockDim = dim3((unsigned)s.threads);
+  cfg.dynamicSmemBytes = s.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = (unsigned)s.cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  auto kernel = s.cluster > 1 ? top_rows_kernel<T, true> : top_rows_kernel<T, false>;
+  ensure_dynamic_smem((const void*)kernel, 131072 + 16);
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(v.logits), v.row_stride, v.vocab,
+                            s.chunk, a);
+}
+
+}  // namespace
+}  // namespace vocab
+
+cudaError_t launch_top_logits(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
+  switch (v.dtype) {
+    case HKB_F32: return vocab::launch<float>(st, v, a);
+    case HKB_F16: return vocab::launch<__half>(st, v, a);
+    default: return vocab::launch<__nv_bfloat16>(st, v, a);
+  }
+}
+
+}  // namespace hkb

@@ -266,6 +266,132 @@ hkb_status hkb_write_design_fasta(const char* path, int32_t num_seqs, int32_t re
 hkb_status hkb_write_logprobs_npz(const char* path, int32_t num_seqs, int32_t residue_count,
                                   const float* log_probs);
 
+/* ---- operators on vocabulary rows --------------------------------------- */
+
+/* A vocabulary row is one position's logits over `vocab` tokens: the rows of
+ * hkb_mpnn_score / hkb_mpnn_design (21 letters) or of any other model.  These
+ * calls have no counterpart in the reference: they draw from such rows with
+ * filters, keep a teacher's answer, and train a student on it.
+ *
+ * They need no engine and no workspace and keep nothing between calls.  All
+ * pointers are device memory of `device`; the work is enqueued on `stream` (a
+ * cudaStream_t of that device, NULL = its default stream) and the call returns
+ * after enqueueing.  Calls on any number of streams and threads may overlap,
+ * and every call can be captured into a CUDA graph.  The calling thread's
+ * current device is left as it was.  Zero rows are a valid call that does
+ * nothing.
+ *
+ * logits[r * row_stride + i] is row r's logit of token i; row_stride counts
+ * elements and may be anything >= 0 (0: all rows are the same).  A logit of
+ * -inf is a token that is masked out.  vocab is 1 to HKB_VOCAB_MAX. */
+#define HKB_VOCAB_MAX 262144
+#define HKB_VOCAB_ROWS_MAX 134217728
+#define HKB_LISTING_MAX 1024
+
+typedef enum { HKB_F32 = 0, HKB_F16 = 1, HKB_BF16 = 2, HKB_F64 = 3 } hkb_dtype;
+
+typedef struct {
+  int64_t rows;
+  int32_t vocab;
+  int32_t dtype;      /* hkb_dtype of the logits: F32, F16 or BF16 */
+  const void* logits;
+  int64_t row_stride;
+} hkb_vocab_rows;
+
+typedef struct {
+  /* per-row settings, or NULL: the number below for every row */
+  const float* temperatures; /* [N] */
+  const int32_t* top_ks;     /* [N] */
+  const float* top_ps;       /* [N] */
+  const float* min_ps;       /* [N] */
+  float temperature;         /* finite, >= 0; 0 = greedy */
+  int32_t top_k;             /* >= 0; 0 = off */
+  float top_p;               /* 0..1; 1 = off */
+  float min_p;               /* 0..1; 0 = off */
+  const void* uniforms;      /* [N] in [0, 1], F32 or F64 */
+  int32_t uniforms_dtype;
+} hkb_sample_settings;
+
+typedef struct {
+  int32_t* tokens;  /* [N] required */
+  float* log_probs; /* [N] required */
+  int32_t* kept;    /* [N] required */
+} hkb_sample_out;
+
+/* Draws one token of each row.  With w_i = exp((x_i - max x) / T), the row's
+ * tokens in the order (logit down, index up) are cut to the shortest of three
+ * heads: the first top_k; the shortest head whose mass reaches top_p of the
+ * top-k mass (at least one token); the tokens with w_i >= min_p.  The token is
+ * the first in index order whose running kept mass exceeds u times the kept
+ * mass, log_probs its log-probability among the kept, kept their number.  The
+ * sampler of hkb_mpnn_design (sampler_scalar.cpp:49-131) draws by the same
+ * rule without filters.  Masses are 64-bit sums in a fixed order.
+ *
+ * T = 0 takes the largest logit, the lowest index of equals (log_prob 0, kept
+ * 1).  A NaN logit counts as -inf; +inf ones share the whole mass.  A row with
+ * no logit above -inf gives token -1, log_prob -inf, kept 0.  Numbers out of
+ * range are InvalidArgument; in the per-row arrays, which the host does not
+ * read, they give that row token -1, log_prob NaN, kept 0. */
+hkb_status hkb_sample_tokens(int device, const hkb_vocab_rows* rows,
+                             const hkb_sample_settings* settings, const hkb_sample_out* out,
+                             void* stream);
+
+typedef struct {
+  void* values;    /* [N,k] in the logits' type, required */
+  int32_t* tokens; /* [N,k] required */
+  float* log_norm; /* [N] optional: log sum_i exp(x_i / temperature) */
+} hkb_top_out;
+
+/* The k largest logits of each row with their tokens, in the order (logit
+ * down, index up): what a teacher stores of its answer.  k is 1 to
+ * HKB_LISTING_MAX; places past the row's logits above -inf hold (-inf, -1).  A
+ * NaN logit counts as -inf.  temperature (finite, > 0) only scales log_norm,
+ * which is -inf for a row with no logit above -inf. */
+hkb_status hkb_top_logits(int device, const hkb_vocab_rows* rows, int32_t k, float temperature,
+                          const hkb_top_out* out, void* stream);
+
+typedef struct {
+  int32_t k;             /* entries a row, 1..HKB_LISTING_MAX */
+  int32_t dtype;         /* hkb_dtype of the values: F32, F16 or BF16 */
+  const void* values;    /* [N,k] teacher logits */
+  const int32_t* tokens; /* [N,k]; negative = no entry, as is a value of -inf */
+  const float* log_norm; /* [N] teacher's log sum exp(a / temperature) over its
+                            whole row, or NULL */
+  float temperature;     /* finite, > 0 */
+} hkb_distill_teacher;
+
+typedef struct {
+  float* loss;               /* [N], or NULL */
+  void* grad;                /* [N, vocab] in the logits' type, or NULL */
+  int64_t grad_row_stride;   /* elements, >= vocab */
+  const float* row_weights;  /* d(objective) / d(loss of row r) is
+                                row_weights[r * row_weight_stride]; NULL = 1 */
+  int64_t row_weight_stride; /* 0 (one number for all rows) or more */
+} hkb_distill_out;
+
+/* Divergence of student rows from a teacher's listed logits a_k at tokens t_k,
+ * its gradient with respect to the student's logits, or both in one pass over
+ * the rows.  With p = softmax(x / temperature):
+ *   log_norm NULL:  q = softmax(a / temperature) over the listed entries,
+ *     loss = temperature^2 sum_k q_k (log q_k - log p[t_k]);
+ *   log_norm given: q_k = exp(a_k / temperature - log_norm); the tokens that
+ *     are not listed form one class of mass q_T = max(0, 1 - sum_k q_k)
+ *     against the student's p_T, and q_T (log q_T - log p_T) joins the sum.  A
+ *     student with no mass outside the list (p_T = 0) has no such term.
+ * The gradient is temperature (Q p_i - q_i) with Q the teacher's mass, where
+ * an unlisted token's q_i is its share q_T p_i / p_T of the class.  An entry
+ * listed twice counts with both masses.
+ *
+ * A row without entries has loss 0 and gradient 0 whatever its logits are, and
+ * a row of weight 0 has gradient 0.  A token >= vocab makes its row's loss and
+ * gradient NaN; so do a NaN or +inf logit and a row with no logit above -inf.
+ * A listed token whose student logit is -inf makes the loss +inf.
+ *
+ * grad may be the logits' own buffer (the same address, row stride and type);
+ * any other overlap is not allowed, and rows must not overlap then. */
+hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill_teacher* teacher,
+                       const hkb_distill_out* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
