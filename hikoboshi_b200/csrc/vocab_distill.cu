@@ -234,8 +234,141 @@ __global__ void __launch_bounds__(kMaxThreads) distill_rows_kernel(
   }
 }
 
+// Short rows, one thread each.  The masses of a row's tokens are added up in
+// shared memory, so a token listed twice needs no special case; the gradient
+// replaces the row's copy and leaves coalesced.
+template <typename T>
+__global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logits,
+                                                                   int64_t row_stride,
+                                                                   int64_t n_rows, int vocab,
+                                                                   DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  double* qs = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
+  float* xs = reinterpret_cast<float*>(smem_raw + sizeof(double) * kShortRows * vocab);
+  const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
+  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
+  load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, false);
+  __syncthreads();
+  if ((int)threadIdx.x < rows) {
+    const int64_t r = r0 + threadIdx.x;
+    float* x = xs + threadIdx.x;  // [i * kShortPitch]
+    const bool tail = a.log_norm != nullptr;
+    const double inv_tau = 1.0 / (double)a.temperature;
+    unsigned listed = 0;
+    bool bad = false;
+    float amax = -CUDART_INF_F;
+    for (int i = 0; i < vocab; ++i) qs[i * kShortRows] = 0.0;
+    for (int k = 0; k < a.k; ++k) {
+      const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+      const int token = a.tokens[r * a.k + k];
+      if (token < 0 || v == -CUDART_INF_F) continue;
+      if (token >= vocab) {
+        bad = true;
+        continue;
+      }
+      listed |= 1u << token;
+      amax = fmaxf(amax, v);
+    }
+    const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+    if (bad || listed == 0) {
+      const float v = bad ? CUDART_NAN_F : 0.0f;
+      if (a.loss) a.loss[r] = v;
+      if (a.grad)
+        for (int i = 0; i < vocab; ++i) x[i * kShortPitch] = weight == 0.0f ? 0.0f : v;
+    } else {
+      double norm;
+      if (tail) {
+        norm = (double)a.log_norm[r];
+      } else {
+        double e = 0.0;
+        for (int k = 0; k < a.k; ++k) {
+          const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+          if (a.tokens[r * a.k + k] >= 0 && v != -CUDART_INF_F)
+            e += exp(((double)v - (double)amax) * inv_tau);
+        }
+        norm = (double)amax * inv_tau + log(e);
+      }
+      double q_sum = 0.0, dot = 0.0;
+      for (int k = 0; k < a.k; ++k) {
+        const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+        const int token = a.tokens[r * a.k + k];
+        if (token < 0 || v == -CUDART_INF_F) continue;
+        const double log_q = (double)v * inv_tau - norm;
+        const double q = exp(log_q);
+        q_sum += q;
+        if (q != 0.0) dot += q * (log_q - (double)x[token * kShortPitch] * inv_tau);
+        qs[token * kShortRows] += q;
+      }
+      // the body is the whole row, or its unlisted tokens; the rest of the
+      // row is added in 64 bits relative to the same largest logit
+      const unsigned body_mask = tail ? ~listed : ~0u;
+      float bmax = -CUDART_INF_F, lmax = -CUDART_INF_F;
+      for (int i = 0; i < vocab; ++i) {
+        const float v = x[i * kShortPitch];
+        if (body_mask >> i & 1u) bmax = fmaxf(bmax, v);
+        else lmax = fmaxf(lmax, v);
+      }
+      const float xmax = fmaxf(bmax, lmax);
+      const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
+      const float c = (float)(kLog2e * inv_tau);
+      float s = 0.0f;
+      double rest = 0.0;
+      for (int i = 0; i < vocab; ++i) {
+        const float v = x[i * kShortPitch];
+        if (body_mask >> i & 1u) s += exp2_fast((v - base) * c);
+        else rest += exp(((double)v - (double)xmax) * inv_tau);
+      }
+      const double body = (double)s;
+      const double lift =
+          bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
+      const double total = body * lift + rest;
+      const double log_total = (double)xmax * inv_tau + log(total);
+      double rest_q = 0.0;
+      if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
+      const double mass = tail ? q_sum + rest_q : 1.0;
+      if (a.loss) {
+        double l = dot + (tail ? q_sum : 1.0) * log_total;
+        if (rest_q > 0.0)
+          l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
+        a.loss[r] = (float)((double)a.temperature * (double)a.temperature * l);
+      }
+      if (a.grad) {
+        const double wt = (double)weight * (double)a.temperature;
+        double factor = mass * lift / total;
+        if (rest_q > 0.0) factor -= rest_q / body;
+        const float G = (float)(wt * factor);
+        const double P = wt * mass / total;
+        for (int i = 0; i < vocab; ++i) {
+          const float v = x[i * kShortPitch];
+          float g;
+          if (weight == 0.0f) g = 0.0f;
+          else if (listed >> i & 1u)
+            g = (float)(P * exp(((double)v - (double)xmax) * inv_tau) - wt * qs[i * kShortRows]);
+          else g = exp2_fast((v - base) * c) * G;
+          x[i * kShortPitch] = g;
+        }
+      }
+    }
+  }
+  if (a.grad == nullptr) return;
+  __syncthreads();
+  T* grad = static_cast<T*>(a.grad) + r0 * a.grad_row_stride;
+  for_each_short(rows, vocab, [&](int row, int col, int) {
+    grad[row * a.grad_row_stride + col] = narrow<T>(xs[col * kShortPitch + row]);
+  });
+}
+
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  if (v.vocab <= kShortVocab) {
+    const int smem = v.vocab * (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch);
+    ensure_dynamic_smem((const void*)distill_short_kernel<T>, kShortVocab *
+                        (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch));
+    const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
+    distill_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
+        static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    return cudaGetLastError();
+  }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(v.rows * s.cluster));

@@ -212,5 +212,42 @@ struct Reducer {
   }
 };
 
+// Short rows (at most kShortVocab tokens): a thread owns a row, a CTA kShortRows
+// of them.  The rows are staged through shared memory token by token, element
+// (row, i) at [i * kShortPitch + row], so that global accesses are coalesced
+// and a thread walking its row meets no bank conflict.
+constexpr int kShortVocab = 32;
+constexpr int kShortRows = 128;
+constexpr int kShortPitch = kShortRows + 1;
+
+// f(row in the CTA, token, element index in the dense block of rows) over the
+// CTA's `rows` rows of `width` numbers, consecutive threads on consecutive
+// elements.
+template <typename F>
+__device__ __forceinline__ void for_each_short(int rows, int width, F f) {
+  const int step_row = kShortRows / width, step_col = kShortRows % width;
+  int row = (int)threadIdx.x / width, col = (int)threadIdx.x % width;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * width; i += kShortRows) {
+    f(row, col, i);
+    row += step_row;
+    col += step_col;
+    if (col >= width) {
+      col -= width;
+      ++row;
+    }
+  }
+}
+
+// Stages the CTA's rows; with `clean` a NaN becomes -inf.
+template <typename T>
+__device__ __forceinline__ void load_short(float* x, const T* g, int64_t row_stride, int rows,
+                                           int vocab, bool clean) {
+  for_each_short(rows, vocab, [&](int row, int col, int) {
+    const float v = widen(g[row * row_stride + col]);
+    x[col * kShortPitch + row] = clean && v != v ? -CUDART_INF_F : v;
+  });
+}
+
 }  // namespace vocab
 }  // namespace hkb

@@ -46,6 +46,12 @@ namespace {
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 
+__device__ __forceinline__ bool settings_valid(float T, int top_k, float top_p, float min_p,
+                                               double u) {
+  return T >= 0.0f && T < CUDART_INF_F && top_k >= 0 && top_p >= 0.0f && top_p <= 1.0f &&
+         min_p >= 0.0f && min_p <= 1.0f && u >= 0.0 && u <= 1.0;
+}
+
 struct SampleSmem {
   ReduceScratch red;
   double seg[kMaxWarps];
@@ -172,8 +178,7 @@ __global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
   const float min_p = a.min_ps ? a.min_ps[r] : a.min_p;
   const double u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
                                   : (double)static_cast<const float*>(a.uniforms)[r];
-  const bool valid = Tf >= 0.0f && Tf < CUDART_INF_F && topk >= 0 && top_p >= 0.0f &&
-                     top_p <= 1.0f && min_p >= 0.0f && min_p <= 1.0f && u >= 0.0 && u <= 1.0;
+  const bool valid = settings_valid(Tf, topk, top_p, min_p, u);
   const bool writer = threadIdx.x == 0 && row.rank == 0;
   cp_async_wait_all();
   if (kClustered) cg::this_cluster().sync();  // every CTA of the row runs from here on
@@ -313,8 +318,125 @@ __global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
   }
 }
 
+// Short rows, one thread each: 64-bit weights in shared memory; the head is
+// found by taking the largest remaining token until a filter stops it, which
+// ends early on the peaked rows that filters are for.
+template <typename T>
+__global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __restrict__ logits,
+                                                                  int64_t row_stride, int64_t n_rows,
+                                                                  int vocab, SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  double* w = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
+  float* xs = reinterpret_cast<float*>(smem_raw + sizeof(double) * kShortRows * vocab);
+  const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
+  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
+  load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, true);
+  __syncthreads();
+  if ((int)threadIdx.x >= rows) return;
+  const int64_t r = r0 + threadIdx.x;
+  const float* x = xs + threadIdx.x;  // [i * kShortPitch]
+  const float Tf = a.temperatures ? a.temperatures[r] : a.temperature;
+  const int topk = a.top_ks ? a.top_ks[r] : a.top_k;
+  const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  const float min_p = a.min_ps ? a.min_ps[r] : a.min_p;
+  const double u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
+                                  : (double)static_cast<const float*>(a.uniforms)[r];
+  if (!settings_valid(Tf, topk, top_p, min_p, u)) {
+    a.tokens[r] = -1;
+    a.log_probs[r] = CUDART_NAN_F;
+    a.kept[r] = 0;
+    return;
+  }
+  float xmax = -CUDART_INF_F;
+  int best = -1, live = 0;
+  for (int i = 0; i < vocab; ++i) {
+    const float v = x[i * kShortPitch];
+    if (v > xmax) {
+      xmax = v;
+      best = i;
+    }
+    live += v > -CUDART_INF_F;
+  }
+  if (best < 0 || Tf == 0.0f) {
+    a.tokens[r] = best;
+    a.log_probs[r] = best < 0 ? -CUDART_INF_F : 0.0f;
+    a.kept[r] = best < 0 ? 0 : 1;
+    return;
+  }
+  const double c2 = kLog2e / (double)Tf;
+  double sum = 0.0;
+  for (int i = 0; i < vocab; ++i) {
+    const float v = x[i * kShortPitch];
+    const double wi = exp2_neg(v == xmax ? 0.0 : ((double)v - (double)xmax) * c2);
+    w[i * kShortRows] = wi;
+    sum += wi;
+  }
+  unsigned keep = 0;  // the kept tokens
+  const bool cut_k = topk > 0 && topk < live;
+  if (cut_k || top_p < 1.0f) {
+    // takes tokens in the head's order while `more` says so; their mass goes to `sum`
+    auto head = [&](auto more) {
+      unsigned taken = 0;
+      int n = 0;
+      double mass = 0.0;
+      while (n < live && more(n, mass)) {
+        float top = -CUDART_INF_F;
+        int at = 0;
+        for (int i = 0; i < vocab; ++i) {
+          const float v = x[i * kShortPitch];
+          if (v > top && !(taken >> i & 1u)) {
+            top = v;
+            at = i;
+          }
+        }
+        taken |= 1u << at;
+        mass += w[at * kShortRows];
+        ++n;
+      }
+      sum = mass;
+      return taken;
+    };
+    if (cut_k) keep = head([&](int n, double) { return n < topk; });
+    if (top_p < 1.0f) {
+      const double need = (double)top_p * sum;
+      keep = head([&](int n, double mass) {
+        return n == 0 || (mass < need && !(cut_k && n >= topk));
+      });
+    }
+  } else {
+    for (int i = 0; i < vocab; ++i)
+      if (x[i * kShortPitch] > -CUDART_INF_F) keep |= 1u << i;
+  }
+  double total = 0.0;
+  for (int i = 0; i < vocab; ++i) {
+    const double wi = w[i * kShortRows];
+    if (wi < (double)min_p) keep &= ~(1u << i);
+    if (keep >> i & 1u) total += wi;
+  }
+  const double target = u * total;
+  double run = 0.0;
+  int token = best;
+  for (int i = 0; i < vocab && !(run > target); ++i) {
+    const double wi = keep >> i & 1u ? w[i * kShortRows] : 0.0;
+    run += wi;
+    if (wi > 0.0) token = i;
+  }
+  a.tokens[r] = token;
+  a.log_probs[r] = (float)log(w[token * kShortRows] / total);
+  a.kept[r] = __popc(keep);
+}
+
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const SampleArgs& a) {
+  if (v.vocab <= kShortVocab) {
+    const int smem = v.vocab * (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch);
+    ensure_dynamic_smem((const void*)sample_short_kernel<T>, kShortVocab *
+                        (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch));
+    const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
+    sample_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
+        static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    return cudaGetLastError();
+  }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(v.rows * s.cluster));
