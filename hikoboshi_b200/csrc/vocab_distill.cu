@@ -56,7 +56,7 @@ __device__ void fill_slice(const RowSlice<T, kClustered>& row, T* grad, float va
 }
 
 template <typename T, bool kClustered>
-__global__ void __launch_bounds__(kMaxThreads) distill_rows_kernel(
+__global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     const T* logits, int64_t row_stride, int vocab, int chunk, int slice_bytes, DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ DistillSmem sm;

@@ -202,6 +202,25 @@ struct Reducer {
     return r;
   }
 
+  // Every CTA's value (uniform within it), in rank order; valid until the next
+  // call.
+  template <typename V>
+  __device__ __forceinline__ const V* spread(V v) {
+    static_assert(sizeof(V) <= 8, "one slot is 8 bytes");
+    V* slots = reinterpret_cast<V*>(sc->cta[buf]);
+    if (kClustered) {
+      auto cl = cg::this_cluster();
+      if (threadIdx.x < cl.num_blocks())
+        cl.map_shared_rank(slots, threadIdx.x)[cl.block_rank()] = v;
+      cl.sync();
+    } else {
+      if (threadIdx.x == 0) slots[0] = v;
+      __syncthreads();
+    }
+    buf ^= 1;
+    return slots;
+  }
+
   template <typename V>
   __device__ __forceinline__ V sum(V v) {
     return all(v, [](V a, V b) { return a + b; });
@@ -211,6 +230,110 @@ struct Reducer {
     return all(v, [](V a, V b) { return a > b ? a : b; });
   }
 };
+
+// Tokens of a row picked out for the CTA of rank 0 to put in order: key << 32 |
+// ~index, so that the larger item is the earlier one of the row's order (value
+// down, index up).
+constexpr int kListCap = 2048;
+struct TokenList {
+  unsigned count;  // of this CTA's own items
+  unsigned long long item[kListCap];
+};
+__device__ __forceinline__ unsigned long long list_item(uint32_t key, int index) {
+  return ((unsigned long long)key << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ uint32_t item_key(unsigned long long it) { return (uint32_t)(it >> 32); }
+__device__ __forceinline__ int item_index(unsigned long long it) { return (int)~(uint32_t)it; }
+
+// Collects the row's elements for which pick(index, value) holds.  Returns
+// their number; if it is at most kListCap, rank 0's list holds them all, in no
+// particular order, else the lists are of no use.
+template <typename T, bool kClustered, typename F>
+__device__ int collect(const RowSlice<T, kClustered>& row, Reducer<kClustered>& red,
+                       TokenList& list, F pick) {
+  constexpr int kE = Vec<T>::kN;
+  if (threadIdx.x == 0) list.count = 0;
+  __syncthreads();
+  row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const float v = widen(x.v[e]);
+      if (pick(i0 + e, v)) {
+        const unsigned at = atomicAdd(&list.count, 1u);
+        if (at < kListCap) list.item[at] = list_item(order_key(v), i0 + e);
+      }
+    }
+  });
+  __syncthreads();
+  if (!kClustered) return (int)list.count;
+  const int mine = (int)list.count;
+  const int* counts = red.spread(mine);
+  int total = 0, offset = 0;
+  for (int c = 0; c < row.size; ++c) {
+    if (c < row.rank) offset += counts[c];
+    total += counts[c];
+  }
+  if (total > kListCap) return total;
+  // rank 0's own items are in place, the other CTAs' go behind them
+  if (row.rank != 0) {
+    unsigned long long* out = cg::this_cluster().map_shared_rank(list.item, 0) + offset;
+    for (int i = threadIdx.x; i < mine; i += blockDim.x) out[i] = list.item[i];
+  }
+  cg::this_cluster().sync();
+  return total;
+}
+
+// Sorts n <= kListCap items downwards (bitonic; the CTA's threads).
+__device__ __forceinline__ void sort_down(unsigned long long* item, int n) {
+  int size = 1;
+  while (size < n) size <<= 1;
+  for (int i = n + (int)threadIdx.x; i < size; i += blockDim.x) item[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      for (int p = threadIdx.x; p < size / 2; p += blockDim.x) {
+        const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1)), l = i | j;
+        const unsigned long long a = item[i], b = item[l];
+        if ((a < b) == ((i & k) == 0)) {
+          item[i] = b;
+          item[l] = a;
+        }
+      }
+      __syncthreads();
+    }
+  }
+}
+
+// Of the threads' largest keys: a key, in its upper 16 bits, that at least
+// `want` threads of this CTA reach; 0 if fewer threads have one.
+__device__ __forceinline__ uint32_t reached_by(uint32_t key, int want) {
+  uint32_t lo = 0;
+  for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1)
+    if (__syncthreads_count(key >= (lo | bit)) >= want) lo |= bit;
+  return lo;
+}
+
+// Inclusive prefix sums over the CTA: thread t's value becomes the sum of those
+// of threads 0..t.  `scratch` holds a number per warp.
+template <typename V>
+__device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const V y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  __syncthreads();  // the scratch may still be read
+  if (lane == 31) scratch[warp] = v;
+  __syncthreads();
+  V base = V(0), all = V(0);
+  for (int w = 0; w < warps; ++w) {
+    if (w == warp) base = all;
+    all += scratch[w];
+  }
+  *total = all;
+  return base + v;
+}
 
 // Short rows (at most kShortVocab tokens): a thread owns a row, a CTA kShortRows
 // of them.  The rows are staged through shared memory token by token, element

@@ -36,7 +36,10 @@ RowShape row_shape(int64_t rows, int vocab, int elem_bytes) {
   s.chunk = (chunk + per16 - 1) / per16 * per16;
   const int vecs = s.chunk / per16 + 1;
   s.smem = (size_t)vecs * 16;
-  s.threads = std::min(vocab::kMaxThreads, std::max(32, (vecs / 2 + 31) / 32 * 32));
+  // a power of two (the bins of the sampler are dealt out evenly), about two
+  // vectors a thread
+  s.threads = 32;
+  while (s.threads < vocab::kMaxThreads && s.threads * 2 < vecs) s.threads *= 2;
   return s;
 }
 
@@ -52,29 +55,40 @@ __device__ __forceinline__ bool settings_valid(float T, int top_k, float top_p, 
          min_p >= 0.0f && min_p <= 1.0f && u >= 0.0 && u <= 1.0;
 }
 
+constexpr int kBins = 1024;
+
 struct SampleSmem {
   ReduceScratch red;
+  ReduceScratch block;
   double seg[kMaxWarps];
   int found;
+  int bin[2];
+  TokenList list;
+  unsigned hist[kBins];
 };
 
-// First token, in index order, whose running sum of f exceeds `target`, over
-// the whole row; every thread of the cluster gets it.  f(index, value) >= 0.
-// Rounding may leave the sum at the end no larger than the target: then the
-// last token with f > 0 is it.  -1 if there is none.
+// First token, in index order, whose running sum of f exceeds `share` times the
+// sum over the row (`absolute`: exceeds `share`); every thread of the cluster
+// gets it.  f(index, value) is a weight, or negative for a token that is not
+// kept; *total_out is the sum, *kept_out the number of kept tokens.  Rounding
+// may leave no sum larger than the target: then the last token with f > 0 is
+// it.  -1 if there is none.
 template <typename T, bool kClustered, typename F>
 __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& red, SampleSmem& sm,
-                      double share, bool absolute, double* total_out, F f) {
+                      double share, bool absolute, double* total_out, int* kept_out, F f) {
   constexpr int kE = Vec<T>::kN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
   double mine = 0.0;
-  int last = -1;
+  int last = -1, n = 0;
   row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       const double w = f(i0 + e, widen(x.v[e]));
-      mine += w;
-      if (w > 0.0) last = i0 + e;
+      if (w >= 0.0) {
+        mine += w;
+        ++n;
+        if (w > 0.0) last = i0 + e;
+      }
     }
   });
 #pragma unroll
@@ -82,19 +96,15 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
   __syncthreads();
   if (lane == 0) sm.seg[warp] = mine;
   if (threadIdx.x == 0) sm.found = -1;
-  __syncthreads();
+  *kept_out = red.sum(n);
   // mass of this CTA, of the row, and of the CTAs before this one
   double cta = 0.0;
   for (int w = 0; w < warps; ++w) cta += sm.seg[w];
-  double before = 0.0, total = cta;
-  if (kClustered) {
-    // one reduction per CTA's value: the sums below run in rank order
-    total = 0.0;
-    for (int c = 0; c < row.size; ++c) {
-      const double v = red.max(c == row.rank ? cta : 0.0);
-      if (c < row.rank) before += v;
-      total += v;
-    }
+  const double* of_cta = red.spread(cta);
+  double before = 0.0, total = 0.0;
+  for (int c = 0; c < row.size; ++c) {
+    if (c == row.rank) before = total;
+    total += of_cta[c];
   }
   *total_out = total;
   const double target = absolute ? share : share * total;
@@ -119,6 +129,7 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
         w[e] = v < end ? f(i0 + e, widen(reinterpret_cast<const Vec<T>*>(row.s)[v].v[e])) : 0.0;
+        w[e] = w[e] > 0.0 ? w[e] : 0.0;
         sum += w[e];
       }
       double incl = sum;
@@ -153,14 +164,95 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
     if (lane == 0) sm.found = token;
   }
   __syncthreads();
-  // at most one CTA found it; the largest also serves the fallback
   const int found = red.max(sm.found);
   if (found >= 0) return found;
   return red.max(last);
 }
 
+// Settings of one row.
+struct RowSettings {
+  float temperature;
+  int top_k;
+  float top_p, min_p;
+  double u;
+};
+
+// Weights of a row: exponents relative to the largest logit.
+struct Weights {
+  float xmax;
+  double c2;  // log2(e) / T
+  __device__ __forceinline__ float below(float x) const { return x == xmax ? 0.0f : xmax - x; }
+  __device__ __forceinline__ double exponent(float x) const {
+    return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2;
+  }
+  __device__ __forceinline__ double weight(float x) const { return exp2_neg(exponent(x)); }
+};
+
+// Finishes a row whose kept tokens are all among the n items of this CTA's
+// list: puts them in order, cuts them to the shortest head and draws.  `need`
+// is the mass that ends the top-p head, or negative: top_p of the mass of the
+// first top_k items.
+__device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
+                            double need, int64_t r, const SampleArgs& a) {
+  unsigned long long* item = sm.list.item;
+  Reducer<false> red(&sm.block);
+  sort_down(item, n);
+  const int nk = s.top_k > 0 ? ::min(n, s.top_k) : n;
+  const int per = (nk + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int i0 = ::min(nk, (int)threadIdx.x * per), i1 = ::min(nk, i0 + per);
+  auto weight = [&](int i) { return wt.weight(key_value(item_key(item[i]))); };
+  int n_kept = nk;
+  if (s.top_p < 1.0f || s.min_p > 0.0f) {
+    double mine = 0.0, total;
+    for (int i = i0; i < i1; ++i) mine += weight(i);
+    double run = block_scan(mine, sm.seg, &total) - mine;
+    if (need < 0.0) need = (double)s.top_p * total;
+    int under = 0, heavy = 0;
+    for (int i = i0; i < i1; ++i) {
+      const double w = weight(i);
+      run += w;
+      under += run < need;
+      heavy += w >= (double)s.min_p;
+    }
+    under = red.sum(under);
+    heavy = red.sum(heavy);
+    if (s.top_p < 1.0f) n_kept = ::min(n_kept, under + 1);
+    n_kept = ::max(1, ::min(n_kept, heavy));
+  }
+  // the kept items in index order: (~index, key) downwards
+  __syncthreads();
+  for (int i = threadIdx.x; i < n_kept; i += blockDim.x) item[i] = item[i] << 32 | item[i] >> 32;
+  __syncthreads();
+  sort_down(item, n_kept);
+  const int per2 = (n_kept + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int j0 = ::min(n_kept, (int)threadIdx.x * per2), j1 = ::min(n_kept, j0 + per2);
+  auto weight2 = [&](int i) { return wt.weight(key_value((uint32_t)item[i])); };
+  double mine = 0.0, total;
+  for (int i = j0; i < j1; ++i) mine += weight2(i);
+  double run = block_scan(mine, sm.seg, &total) - mine;
+  const double target = s.u * total;
+  int hit = 0x7fffffff, last = -1;
+  for (int i = j0; i < j1; ++i) {
+    const double w = weight2(i);
+    run += w;
+    if (w > 0.0) {
+      last = i;
+      if (run > target && hit == 0x7fffffff) hit = i;
+    }
+  }
+  hit = -red.max(-hit);
+  last = red.max(last);
+  if (threadIdx.x == 0) {
+    const unsigned long long it = item[hit != 0x7fffffff ? hit : last];
+    const float x = key_value((uint32_t)it);
+    a.tokens[r] = (int)~(uint32_t)(it >> 32);
+    a.log_probs[r] = (float)(wt.exponent(x) * kLn2 - log(total));
+    a.kept[r] = n_kept;
+  }
+}
+
 template <typename T, bool kClustered>
-__global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
+__global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ SampleSmem sm;
@@ -172,14 +264,16 @@ __global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
   row.init(reinterpret_cast<T*>(smem_raw), g, vocab, chunk);
   row.load(g);
 
-  const float Tf = a.temperatures ? a.temperatures[r] : a.temperature;
-  const int topk = a.top_ks ? a.top_ks[r] : a.top_k;
-  const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  const float min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-  const double u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
-                                  : (double)static_cast<const float*>(a.uniforms)[r];
-  const bool valid = settings_valid(Tf, topk, top_p, min_p, u);
+  RowSettings s;
+  s.temperature = a.temperatures ? a.temperatures[r] : a.temperature;
+  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  s.min_p = a.min_ps ? a.min_ps[r] : a.min_p;
+  s.u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
+                       : (double)static_cast<const float*>(a.uniforms)[r];
+  const bool valid = settings_valid(s.temperature, s.top_k, s.top_p, s.min_p, s.u);
   const bool writer = threadIdx.x == 0 && row.rank == 0;
+  for (int b = threadIdx.x; b < kBins; b += blockDim.x) sm.hist[b] = 0;
   cp_async_wait_all();
   if (kClustered) cg::this_cluster().sync();  // every CTA of the row runs from here on
   else __syncthreads();
@@ -194,48 +288,56 @@ __global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
   Reducer<kClustered> red(&sm.red);
 
   // largest logit and its first place; NaN becomes -inf
-  uint32_t kbest = 0;
+  float tmax = -CUDART_INF_F;
   int ibest = 0x7fffffff;
   row.for_each([&](int i0, Vec<T>& x) {
-    bool nan = false;
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       const float v = widen(x.v[e]);
-      if (v != v) {
-        x.v[e] = narrow<T>(-CUDART_INF_F);
-        nan = true;
-        continue;
-      }
-      const uint32_t k = order_key(v);
-      if (k > kbest) {
-        kbest = k;
+      if (v != v) x.v[e] = narrow<T>(-CUDART_INF_F);
+      if (v > tmax) {
+        tmax = v;
         ibest = i0 + e;
       }
     }
-    (void)nan;
   });
-  const unsigned long long best = red.max(((unsigned long long)kbest << 32) | (uint32_t)~ibest);
-  const uint32_t kmax = (uint32_t)(best >> 32);
-  if (kmax <= kKeyNegInf || Tf == 0.0f) {
+  const uint32_t tkey = order_key(tmax);
+  const unsigned long long best = red.max(list_item(tkey, ibest));
+  const uint32_t kmax = item_key(best);
+  if (kmax <= kKeyNegInf || s.temperature == 0.0f) {
     if (writer) {
       const bool none = kmax <= kKeyNegInf;
-      a.tokens[r] = none ? -1 : (int)~(uint32_t)best;
+      a.tokens[r] = none ? -1 : item_index(best);
       a.log_probs[r] = none ? -CUDART_INF_F : 0.0f;
       a.kept[r] = none ? 0 : 1;
     }
     return;
   }
-  const float xmax = key_value(kmax);
-  const double c2 = kLog2e / (double)Tf;
-  auto exponent = [&](float x) { return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2; };
+  const Weights wt{key_value(kmax), kLog2e / (double)s.temperature};
+  if (s.top_k >= vocab) s.top_k = 0;
 
-  // The kept head is { (key, index) : key > t, or key == t and index <= icut }.
+  // Top-k of a number that fits the list: the k-th largest of the row is no
+  // less than the k/C-th largest of the threads' own largest logits in the CTA
+  // where that is least, and few more than k tokens reach it.
+  if (s.top_k > 0 && s.top_k <= kListCap / 2) {
+    const uint32_t mine = reached_by(tkey, (s.top_k + row.size - 1) / row.size);
+    const uint32_t bound = ~red.max(~mine);
+    const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
+    const int n = collect(row, red, sm.list, [&](int, float x) { return x >= from; });
+    if (n <= kListCap) {
+      if (row.rank == 0) finish_list(sm, n, wt, s, -1.0, r, a);
+      return;
+    }
+  }
+
+  // The kept head is { (key, index) : key > t, or key == t and index <= icut },
+  // further cut by min-p and by `reach`, the largest distance from the largest
+  // logit that a kept token can have.
   uint32_t t = kKeyNegInf + 1;
   int icut = 0x7fffffff;
   auto in_head = [&](int i, uint32_t k) { return k > t || (k == t && i <= icut); };
-
-  if (topk > 0 && topk < vocab) {
-    // largest key with at least k tokens at or above it
+  if (s.top_k > 0) {
+    // largest key with at least k tokens at or above it, by bisection
     auto count = [&](uint32_t lo) {
       int c = 0;
       row.for_each([&](int, const Vec<T>& x) {
@@ -244,76 +346,196 @@ __global__ void __launch_bounds__(kMaxThreads) sample_rows_kernel(
       });
       return red.sum(c);
     };
-    if (count(kKeyNegInf + 1) > topk) {
+    if (count(kKeyNegInf + 1) > s.top_k) {
       uint32_t lo = kKeyNegInf + 1, hi = kmax;
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (count(mid) >= topk) lo = mid;
+        if (count(mid) >= s.top_k) lo = mid;
         else hi = mid - 1;
       }
       t = lo;
       const int above = t == 0xffffffffu ? 0 : count(t + 1);
       double ties;
-      icut = locate(row, red, sm, (double)(topk - above) - 0.5, true, &ties,
-                    [&](int, float x) { return order_key(x) == t ? 1.0 : 0.0; });
+      int n;
+      icut = locate(row, red, sm, (double)(s.top_k - above) - 0.5, true, &ties, &n,
+                    [&](int, float x) { return order_key(x) == t ? 1.0 : -1.0; });
     }
   }
-  if (top_p < 1.0f) {
-    auto mass = [&](uint32_t lo) {
-      double m = 0.0;
-      row.for_each([&](int i0, const Vec<T>& x) {
+  const double zmin = s.min_p > 0.0f ? log2((double)s.min_p) - 1e-3 : -CUDART_INF;
+  float reach = CUDART_INF_F;
+  if (zmin > -CUDART_INF) reach = (float)(-zmin / wt.c2) * 1.000001f;
+
+  if (s.top_p < 1.0f) {
+    double m = 0.0;
+    row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const float v = widen(x.v[e]);
-          const uint32_t k = order_key(v);
-          if (k >= lo && in_head(i0 + e, k)) m += exp2_neg(exponent(v));
-        }
-      });
-      return red.sum(m);
-    };
-    const double need = (double)top_p * mass(t);
-    uint32_t lo = t, hi = kmax;
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (mass(mid) >= need) lo = mid;
-      else hi = mid - 1;
-    }
-    // `lo` is the border's key: of its tokens the first m are kept
-    const double above = lo == kmax ? 0.0 : mass(lo + 1);
-    const double w = exp2_neg(exponent(key_value(lo)));
-    double m = w > 0.0 ? ceil((need - above) / w) : 1.0;
-    if (m < 1.0) m = 1.0;
-    const uint32_t old_t = t;
-    const int old_cut = icut;
-    t = lo;
-    icut = 0x7fffffff;
-    double ties;
-    icut = locate(row, red, sm, m - 0.5, true, &ties, [&](int i, float x) {
-      const uint32_t k = order_key(x);
-      return k == lo && (k > old_t || i <= old_cut) ? 1.0 : 0.0;
+      for (int e = 0; e < kE; ++e) {
+        const float v = widen(x.v[e]);
+        if (in_head(i0 + e, order_key(v))) m += wt.weight(v);
+      }
     });
+    const double mass = red.sum(m);
+    const double need = (double)s.top_p * mass;
+    // Tokens lighter than (1 - p) * mass / V have less than (1 - p) * mass
+    // together, so the border lies above them.
+    const double z0 =
+        fmax(zmin, log2((1.0 - (double)s.top_p) * mass / (double)vocab) - 1e-3);
+    reach = (float)(-z0 / wt.c2) * 1.000001f;
+    // Count the tokens within reach in bins of equal width: a bin's weights lie
+    // between those of its ends, so the counts bound the running mass from both
+    // sides (1e-4 covers the 32-bit arithmetic), and the border lies in the
+    // few bins that the two bounds leave.
+    const float scale = (float)kBins / reach;
+    auto bin_of = [&](float x) { return ::min(kBins - 1, (int)(wt.below(x) * scale)); };
+    row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float v = widen(x.v[e]);
+        if (wt.below(v) <= reach && in_head(i0 + e, order_key(v))) atomicAdd(&sm.hist[bin_of(v)], 1u);
+      }
+    });
+    if (kClustered) cg::this_cluster().sync();
+    else __syncthreads();
+    // every CTA adds up the whole row's bins and finds the same border
+    const int per = kBins / (int)blockDim.x, b0 = (int)threadIdx.x * per;
+    const float width2 = (float)(wt.c2 / (double)scale);  // of a bin, in powers of two
+    float low = 0.0f, high = 0.0f, all;
+    int number = 0;
+    auto bin_count = [&](int b) {
+      if (!kClustered) return (int)sm.hist[b];
+      int c = 0;
+      for (int k = 0; k < row.size; ++k)
+        c += (int)cg::this_cluster().map_shared_rank(sm.hist, k)[b];
+      return c;
+    };
+    for (int b = b0; b < b0 + per; ++b) {
+      const float c = (float)bin_count(b);
+      low += c * exp2f(-(float)(b + 1) * width2) * 0.9999f;
+      high += c * exp2f(-(float)b * width2) * 1.0001f;
+      number += (int)c;
+    }
+    float* fscratch = reinterpret_cast<float*>(sm.seg);
+    int* iscratch = reinterpret_cast<int*>(sm.seg);
+    int number_all;
+    float run_low = block_scan(low, fscratch, &all) - low;
+    float run_high = block_scan(high, fscratch, &all) - high;
+    int run_number = block_scan(number, iscratch, &number_all) - number;
+    // last bin that is certainly kept, first bin that certainly ends the head
+    int certain = -1, ends = kBins;
+    for (int b = b0; b < b0 + per; ++b) {
+      const float c = (float)bin_count(b);
+      run_low += c * exp2f(-(float)(b + 1) * width2) * 0.9999f;
+      run_high += c * exp2f(-(float)b * width2) * 1.0001f;
+      if (run_high < (float)need * 0.9999f) certain = b;
+      if (run_low >= (float)need * 1.0001f) ends = ::min(ends, b);
+    }
+    Reducer<false> block(&sm.block);
+    certain = block.max(certain);
+    ends = ::min(kBins - 1, -block.max(-ends));
+    int upto_certain = 0, upto_ends = 0;
+    for (int b = b0; b < b0 + per; ++b) {
+      run_number += bin_count(b);
+      if (b == certain) upto_certain = run_number;
+      if (b == ends) upto_ends = run_number;
+    }
+    upto_certain = block.sum(upto_certain);
+    upto_ends = block.sum(upto_ends);
+    // (the others may still read this CTA's bins: until their next reduction)
+
+    // temperatures at the ends of the type's range leave no finite bin width
+    const bool binned = scale > 0.0f && scale < CUDART_INF_F;
+    const int list_from = upto_ends <= kListCap ? -1 : certain;
+    if (binned && upto_ends - (list_from < 0 ? 0 : upto_certain) <= kListCap) {
+      double above = 0.0;
+      if (list_from >= 0) {
+        row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            const float v = widen(x.v[e]);
+            if (wt.below(v) <= reach && in_head(i0 + e, order_key(v)) && bin_of(v) <= list_from)
+              above += wt.weight(v);
+          }
+        });
+        above = red.sum(above);
+      }
+      const int n = collect(row, red, sm.list, [&](int i, float x) {
+        if (!(wt.below(x) <= reach) || !in_head(i, order_key(x))) return false;
+        const int b = bin_of(x);
+        return b > list_from && b <= ends;
+      });
+      if (list_from < 0) {
+        if (row.rank == 0) finish_list(sm, n, wt, s, need, r, a);
+        return;
+      }
+      // the head ends inside the list, or (cut by min-p) nowhere
+      unsigned long long border = 0;
+      if (row.rank == 0) {
+        sort_down(sm.list.item, n);
+        const int per_t = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+        const int i0 = ::min(n, (int)threadIdx.x * per_t), i1 = ::min(n, i0 + per_t);
+        double mine = 0.0, total;
+        for (int i = i0; i < i1; ++i) mine += wt.weight(key_value(item_key(sm.list.item[i])));
+        double run = above + (block_scan(mine, sm.seg, &total) - mine);
+        int under = 0;
+        for (int i = i0; i < i1; ++i) {
+          run += wt.weight(key_value(item_key(sm.list.item[i])));
+          under += run < need;
+        }
+        under = block.sum(under);
+        if (under < n) border = sm.list.item[under];
+      }
+      border = red.spread(border)[0];
+      if (border != 0) {
+        t = item_key(border);
+        icut = item_index(border);
+      }
+    } else {
+      // equal logits crowd a bin: bisect between its ends
+      auto mass_from = [&](uint32_t lo) {
+        double m = 0.0;
+        row.for_each([&](int i0, const Vec<T>& x) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) {
+            const float v = widen(x.v[e]);
+            const uint32_t k = order_key(v);
+            if (k >= lo && in_head(i0 + e, k)) m += wt.weight(v);
+          }
+        });
+        return red.sum(m);
+      };
+      uint32_t lo = t, hi = kmax;
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        if (mass_from(mid) >= need) lo = mid;
+        else hi = mid - 1;
+      }
+      // `lo` is the border's key: of its tokens the first `ties` are kept
+      const double above = lo == kmax ? 0.0 : mass_from(lo + 1);
+      const double w = wt.weight(key_value(lo));
+      double ties = w > 0.0 ? ceil((need - above) / w) : 1.0;
+      if (ties < 1.0) ties = 1.0;
+      const uint32_t old_t = t;
+      const int old_cut = icut;
+      t = lo;
+      icut = 0x7fffffff;
+      double all_ties;
+      int n;
+      icut = locate(row, red, sm, ties - 0.5, true, &all_ties, &n, [&](int i, float x) {
+        const uint32_t k = order_key(x);
+        return k == lo && (k > old_t || i <= old_cut) ? 1.0 : -1.0;
+      });
+    }
   }
   double total;
-  int n = 0;
-  const int token = locate(row, red, sm, u, false, &total, [&](int i, float x) {
-    const uint32_t k = order_key(x);
-    if (!in_head(i, k)) return 0.0;
-    const double w = exp2_neg(exponent(x));
-    return w >= (double)min_p ? w : 0.0;
+  int n;
+  const int token = locate(row, red, sm, s.u, false, &total, &n, [&](int i, float x) {
+    if (!(wt.below(x) <= reach) || !in_head(i, order_key(x))) return -1.0;
+    const double w = wt.weight(x);
+    return w >= (double)s.min_p ? w : -1.0;
   });
-  row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const float v = widen(x.v[e]);
-      n += in_head(i0 + e, order_key(v)) &&
-           (min_p == 0.0f || exp2_neg(exponent(v)) >= (double)min_p);
-    }
-  });
-  n = red.sum(n);
   if (writer) {
-    const float x = widen(g[token]);
     a.tokens[r] = token;
-    a.log_probs[r] = (float)(exponent(x) * kLn2 - log(total));
+    a.log_probs[r] = (float)(wt.exponent(widen(g[token])) * kLn2 - log(total));
     a.kept[r] = n;
   }
 }

@@ -13,12 +13,11 @@ constexpr float kLog2ef = 1.44269504f;
 
 struct TopSmem {
   ReduceScratch red;
-  unsigned count;
-  unsigned long long list[HKB_LISTING_MAX];  // key << 32 | ~index
+  TokenList list;
 };
 
 template <typename T, bool kClustered>
-__global__ void __launch_bounds__(kMaxThreads) top_rows_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __restrict__ logits,
                                                                int64_t row_stride, int vocab,
                                                                int chunk, TopArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -30,23 +29,21 @@ __global__ void __launch_bounds__(kMaxThreads) top_rows_kernel(const T* __restri
   const T* g = logits + r * row_stride;
   row.init(reinterpret_cast<T*>(smem_raw), g, vocab, chunk);
   row.load(g);
-  if (threadIdx.x == 0) sm.count = 0;
   cp_async_wait_all();
-  if (kClustered) cg::this_cluster().sync();
+  if (kClustered) cg::this_cluster().sync();  // every CTA of the row runs from here on
   else __syncthreads();
   Reducer<kClustered> red(&sm.red);
 
-  uint32_t kmax = 0;
+  float tmax = -CUDART_INF_F;
   row.for_each([&](int, Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       const float v = widen(x.v[e]);
       if (v != v) x.v[e] = narrow<T>(-CUDART_INF_F);
-      else kmax = ::max(kmax, order_key(v));
+      tmax = fmaxf(tmax, v);
     }
   });
-  kmax = red.max(kmax);
-  const float xmax = key_value(kmax);
+  const float xmax = red.max(tmax);
   if (a.log_norm) {
     const float c = kLog2ef / a.temperature;
     float s = 0.0f;
@@ -59,26 +56,34 @@ __global__ void __launch_bounds__(kMaxThreads) top_rows_kernel(const T* __restri
     });
     const double total = red.sum((double)s);
     if (threadIdx.x == 0 && row.rank == 0)
-      a.log_norm[r] = kmax <= kKeyNegInf ? -CUDART_INF_F
-                                         : (float)((double)xmax / (double)a.temperature + log(total));
+      a.log_norm[r] = xmax == -CUDART_INF_F
+                          ? xmax
+                          : (float)((double)xmax / (double)a.temperature + log(total));
   }
-  // k-th largest key, and of the tokens that share it the last index taken
-  uint32_t t = kKeyNegInf + 1;
-  int icut = 0x7fffffff;
-  auto count = [&](uint32_t lo, int last) {
-    int c = 0;
-    row.for_each([&](int i0, const Vec<T>& x) {
+  // The k-th largest of the row is no less than the k/C-th largest of the
+  // threads' own largest logits in the CTA where that is least; few more than
+  // k tokens reach it.
+  const uint32_t mine = reached_by(order_key(tmax), (a.k + row.size - 1) / row.size);
+  const uint32_t bound = ~red.max(~mine);
+  const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
+  int n = collect(row, red, sm.list, [&](int, float x) { return x >= from; });
+  if (n > kListCap) {
+    // many equal logits, or a row whose large logits lie side by side: the
+    // k-th largest key by bisection, and the last index taken of its tokens
+    uint32_t t = kKeyNegInf + 1;
+    int icut = 0x7fffffff;
+    auto count = [&](uint32_t lo, int last) {
+      int c = 0;
+      row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const uint32_t k = order_key(widen(x.v[e]));
-        c += k > lo || (k == lo && i0 + e <= last);
-      }
-    });
-    return red.sum(c);
-  };
-  int n = count(t, icut);
-  if (n > a.k) {
-    uint32_t lo = t, hi = kmax;
+        for (int e = 0; e < kE; ++e) {
+          const uint32_t k = order_key(widen(x.v[e]));
+          c += k > lo || (k == lo && i0 + e <= last);
+        }
+      });
+      return red.sum(c);
+    };
+    uint32_t lo = t, hi = order_key(xmax);
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
       if (count(mid, 0x7fffffff) >= a.k) lo = mid;
@@ -92,41 +97,20 @@ __global__ void __launch_bounds__(kMaxThreads) top_rows_kernel(const T* __restri
       else i_lo = mid + 1;
     }
     icut = i_lo;
-    n = a.k;
+    n = collect(row, red, sm.list, [&](int i, float x) {
+      const uint32_t k = order_key(x);
+      return k > t || (k == t && i <= icut);
+    });
   }
-  unsigned* counter = &sm.count;
-  unsigned long long* list = sm.list;
-  if (kClustered) {
-    counter = cg::this_cluster().map_shared_rank(counter, 0);
-    list = cg::this_cluster().map_shared_rank(list, 0);
-  }
-  row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const uint32_t k = order_key(widen(x.v[e]));
-      if (k > t || (k == t && i0 + e <= icut)) {
-        const unsigned at = atomicAdd(counter, 1u);
-        list[at] = ((unsigned long long)k << 32) | (uint32_t)~(i0 + e);
-      }
-    }
-  });
-  if (kClustered) cg::this_cluster().sync();
-  else __syncthreads();
   if (row.rank != 0) return;
+  sort_down(sm.list.item, n);
   T* values = static_cast<T*>(a.values) + r * a.k;
   int32_t* tokens = a.tokens + r * a.k;
   for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
-    if (i >= n) {
-      values[i] = narrow<T>(-CUDART_INF_F);
-      tokens[i] = -1;
-      continue;
-    }
-    const unsigned long long me = sm.list[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += sm.list[j] > me;
-    const int index = (int)~(uint32_t)me;
-    values[place] = g[index];
-    tokens[place] = index;
+    const bool there = i < n;
+    const int index = there ? item_index(sm.list.item[i]) : -1;
+    values[i] = there ? g[index] : narrow<T>(-CUDART_INF_F);
+    tokens[i] = index;
   }
 }
 
