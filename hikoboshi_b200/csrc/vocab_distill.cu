@@ -36,9 +36,54 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+
+// What a row's loss and gradient need beside the row, from one thread.
+struct RowFactors {
+  float base;    // of the body's exponents
+  float G;       // gradient of an unlisted token: exp2((x - base) c) * G
+  double shift;  // largest logit, of which p is formed on the list
+  double P;      // gradient on the list: P exp((x - shift) / tau) - Q q
+  double Q;
+};
+
+// The body's largest logit and sum (relative to it), the listed tokens' largest
+// logit and, where the unlisted tokens are a class of their own, their sum
+// relative to the row's largest; q_sum the listed masses' sum (1 without the
+// class) and dot = sum q (log q - z).
+__device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double body, float lmax,
+                                                  double listed, double q_sum, double dot,
+                                                  double inv_tau, float temperature, float weight,
+                                                  float* loss) {
+  RowFactors f;
+  const float xmax = fmaxf(bmax, lmax);
+  const double lift =
+      bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
+  const double total = body * lift + listed;  // relative to xmax
+  double rest_q = 0.0;
+  if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
+  const double mass = tail ? q_sum + rest_q : 1.0;
+  if (loss) {
+    const double log_total = (double)xmax * inv_tau + log(total);
+    double l = dot + (tail ? q_sum : 1.0) * log_total;
+    if (rest_q > 0.0)
+      l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
+    *loss = (float)((double)temperature * (double)temperature * l);
+  }
+  const double wt = (double)weight * (double)temperature;
+  double factor = mass * lift / total;
+  if (rest_q > 0.0) factor -= rest_q / body;
+  f.base = bmax == -CUDART_INF_F ? 0.0f : bmax;
+  f.G = (float)(wt * factor);
+  f.shift = (double)xmax;
+  f.P = wt * mass / total;
+  f.Q = wt;
+  return f;
+}
+
 struct DistillSmem {
   ReduceScratch cluster;
   ReduceScratch block;
+  RowFactors f;
 };
 
 // Listing of a row in shared memory, behind the slice's buffer.
@@ -182,35 +227,23 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   const double body = red.sum((double)s);
   if (tail) listed = red.sum(listed);
   dot = red.sum(dot);
-  const double lift = bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
-  const double total = body * lift + listed;  // relative to xmax
-  const double log_total = (double)xmax * inv_tau + log(total);
-  double rest_q = 0.0;
-  if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
-  const double mass = tail ? q_sum + rest_q : 1.0;
-  if (writer && a.loss) {
-    double l = dot + (tail ? q_sum : 1.0) * log_total;
-    if (rest_q > 0.0)
-      l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
-    const double tau = (double)a.temperature;
-    a.loss[r] = (float)(tau * tau * l);
-  }
-  if (grad == nullptr) return;
   const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+  if (threadIdx.x == 0)
+    sm.f = row_factors(tail, bmax, body, listed_max, listed, tail ? q_sum : 1.0, dot, inv_tau,
+                       a.temperature, weight, writer && a.loss ? a.loss + r : nullptr);
+  if (grad == nullptr) return;
   if (weight == 0.0f) {
     fill_slice(row, grad, 0.0f);
     return;
   }
-  const double wt = (double)weight * (double)a.temperature;
-  double factor = mass * lift / total;
-  if (rest_q > 0.0) factor -= rest_q / body;
-  const float G = (float)(wt * factor);
+  __syncthreads();
+  const RowFactors f = sm.f;
   T* gs = grad + row.start - row.ph;  // element e0 of the slice's vectors goes to gs[e0]
   const bool same_phase = (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
   row.for_each([&](int i0, const Vec<T>& x) {
     Vec<T> y;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) y.v[e] = narrow<T>(exp2_fast((widen(x.v[e]) - base) * c) * G);
+    for (int e = 0; e < kE; ++e) y.v[e] = narrow<T>(exp2_fast((widen(x.v[e]) - base) * c) * f.G);
     const int e0 = i0 - row.start + row.ph;
     if (same_phase && e0 >= row.ph && e0 + kE <= row.ph + row.n) {
       *reinterpret_cast<Vec<T>*>(gs + e0) = y;
@@ -229,8 +262,197 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
       for (int j = 0; j < a.k; ++j)
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
-    const double p = exp(((double)ls.x[k] - (double)xmax) * inv_tau) / total;
-    grad[ls.token[k]] = narrow<T>((float)(wt * (mass * p - q)));
+    const double e = exp(((double)ls.x[k] - f.shift) * inv_tau);
+    grad[ls.token[k]] = narrow<T>((float)(f.P * e - f.Q * q));
+  }
+}
+
+struct StreamSmem {
+  ReduceScratch red;
+  RowFactors f;
+};
+
+// Many rows: a CTA streams a row for its sum, then again for the gradient.  The
+// listed tokens are marked in a bit map in the phase of the row's vectors, a
+// vector's marks in one byte or half a byte, so that the first pass leaves them
+// out where the unlisted ones form a class; the entry that sets a mark stands
+// for its token.
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T* logits,
+                                                                        int64_t row_stride,
+                                                                        int vocab, DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ StreamSmem sm;
+  constexpr int kE = Vec<T>::kN, kU = 4;
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const T* g = logits + r * row_stride;
+  const RowStream<T> row(g, vocab);
+  Listing ls;  // q holds masses up to the factor q_scale
+  ls.q = reinterpret_cast<double*>(smem_raw);
+  ls.x = reinterpret_cast<float*>(ls.q + a.k);
+  ls.token = reinterpret_cast<int*>(ls.x + a.k);
+  ls.own = ls.token + a.k;
+  uint32_t* marks = reinterpret_cast<uint32_t*>(ls.own + a.k);
+  Reducer<false> red(&sm.red);
+
+  const bool tail = a.log_norm != nullptr;
+  const double inv_tau = 1.0 / (double)a.temperature;
+  for (int w = tid; w < (row.end + 31) / 32; w += threads) marks[w] = 0;
+  unsigned flags = 0;  // 1: an entry, 2: a token outside the vocabulary
+  float amax = -CUDART_INF_F;
+  for (int k = tid; k < a.k; k += threads) {
+    const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+    int token = a.tokens[r * a.k + k];
+    if (token < 0 || v == -CUDART_INF_F) token = -1;
+    if (token >= 0) {
+      flags |= token < vocab ? 1u : 2u;
+      amax = fmaxf(amax, v);
+    }
+    ls.token[k] = token;
+    ls.x[k] = v;
+  }
+  const unsigned long long head =
+      red.all(((unsigned long long)order_key(amax) << 32) | flags,
+              [](unsigned long long p, unsigned long long q) {
+                return (p > q ? p : q) | (p & 3) | (q & 3);
+              });
+  T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
+  const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+  const bool row_bad = head & 2, row_any = head & 1;
+  if (row_bad || !row_any) {
+    const float v = row_bad ? CUDART_NAN_F : 0.0f;
+    if (tid == 0 && a.loss) a.loss[r] = v;
+    if (grad)
+      for (int i = tid; i < vocab; i += threads) grad[i] = narrow<T>(weight == 0.0f ? 0.0f : v);
+    return;
+  }
+  amax = key_value((uint32_t)(head >> 32));
+  // masses: exp(a / tau - norm), or relative to the largest until their sum is known
+  const double norm = tail ? (double)a.log_norm[r] : (double)amax * inv_tau;
+  double q_sum = 0.0, dot = 0.0;
+  float lmax = -CUDART_INF_F;
+  bool twice = false;
+  for (int k = tid; k < a.k; k += threads) {
+    const int token = ls.token[k];
+    double q = 0.0;
+    int own = 0;
+    if (token >= 0) {
+      const double log_q = tail ? (double)ls.x[k] * inv_tau - norm
+                                : ((double)ls.x[k] - (double)amax) * inv_tau;
+      q = exp(log_q);
+      const float x = widen(g[token]);
+      ls.x[k] = x;
+      lmax = fmaxf(lmax, x);
+      q_sum += q;
+      // a mass that underflows counts nothing, also on a masked token
+      if (q != 0.0) dot += q * (log_q - (double)x * inv_tau);
+      const int bit = token + row.ph;
+      own = !(atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u);
+      twice |= !own;
+    }
+    ls.q[k] = q;
+    ls.own[k] = own;
+  }
+  q_sum = red.sum(q_sum);
+  dot = red.sum(dot);
+  const bool row_twice = __syncthreads_or(twice);
+  double q_scale = 1.0;
+  if (!tail) {
+    q_scale = 1.0 / q_sum;
+    dot = dot * q_scale - log(q_sum);
+    q_sum = 1.0;
+    lmax = -CUDART_INF_F;
+  }
+
+  const float c = (float)(kLog2e * inv_tau);
+  SoftSum soft;
+  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
+    Vec<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = v0 + u * threads;
+      if (v < row.nvec) x[u] = row.load(v);
+      else
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
+    }
+    if (tail) {
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int v = v0 + u * threads;
+        if (v >= row.nvec) continue;
+        const uint32_t m = marks[v * kE >> 5] >> (v * kE & 31) & ((1u << kE) - 1u);
+        if (m)
+#pragma unroll
+          for (int e = 0; e < kE; ++e)
+            if (m >> e & 1u) x[u].v[e] = narrow<T>(-CUDART_INF_F);
+      }
+    }
+    soft.add(x, c);
+  }
+  soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
+    return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
+  }));
+  double listed = 0.0;
+  if (tail) {
+    lmax = red.max(lmax);
+    const float xmax = fmaxf(soft.m, lmax);
+    for (int k = tid; k < a.k; k += threads)
+      if (ls.own[k]) listed += exp(((double)ls.x[k] - (double)xmax) * inv_tau);
+    listed = red.sum(listed);
+  }
+  if (tid == 0)
+    sm.f = row_factors(tail, soft.m, (double)soft.s, lmax, listed, q_sum, dot, inv_tau,
+                       a.temperature, weight, a.loss ? a.loss + r : nullptr);
+  if (grad == nullptr) return;
+  if (weight == 0.0f) {
+    for (int i = tid; i < vocab; i += threads) grad[i] = narrow<T>(0.0f);
+    return;
+  }
+  __syncthreads();
+  const RowFactors f = sm.f;
+  T* gv = grad - row.ph;  // vector v of the row goes to gv[v * kE ..]
+  const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
+  const float2 minus = make_float2(-f.base, -f.base), scale = make_float2(c, c),
+               G = make_float2(f.G, f.G);
+  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
+    Vec<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = v0 + u * threads;
+      if (v < row.nvec) x[u] = row.load(v);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = v0 + u * threads;
+      if (v >= row.nvec) continue;
+      Vec<T> y;
+#pragma unroll
+      for (int i = 0; i < kE / 2; ++i) {
+        const float2 t = __fmul2_rn(__fadd2_rn(pair_of(x[u], i), minus), scale);
+        set_pair(y, i, __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), G));
+      }
+      if (same_phase && row.whole(v)) {
+        __stcs(reinterpret_cast<uint4*>(gv + v * kE), *reinterpret_cast<const uint4*>(&y));
+      } else {
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+          if (v * kE + e >= row.ph && v * kE + e < row.end) gv[v * kE + e] = y.v[e];
+      }
+    }
+  }
+  __syncthreads();
+  for (int k = tid; k < a.k; k += threads) {
+    if (!ls.own[k]) continue;
+    double q = ls.q[k];
+    if (row_twice) {
+      q = 0.0;
+      for (int j = 0; j < a.k; ++j)
+        if (ls.token[j] == ls.token[k]) q += ls.q[j];
+    }
+    const double e = exp(((double)ls.x[k] - f.shift) * inv_tau);
+    grad[ls.token[k]] = narrow<T>((float)(f.P * e - f.Q * (q * q_scale)));
   }
 }
 
@@ -367,6 +589,17 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
     distill_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
         static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    return cudaGetLastError();
+  }
+  if (v.rows >= kStreamRows) {
+    // bits of a row in its vectors' phase, in whole words
+    const int words = (v.vocab + 16 / (int)sizeof(T) - 1 + 31) / 32;
+    const int smem = a.k * 20 + words * 4;
+    ensure_dynamic_smem((const void*)distill_stream_kernel<T>,
+                        HKB_LISTING_MAX * 20 + HKB_VOCAB_MAX / 8 + 8);
+    distill_stream_kernel<T>
+        <<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), smem, st>>>(
+            static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
     return cudaGetLastError();
   }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));

@@ -18,6 +18,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <math_constants.h>
 #include <stdint.h>
 
@@ -333,6 +334,144 @@ __device__ __forceinline__ V block_scan(V v, V* scratch, V* total) {
   }
   *total = all;
   return base + v;
+}
+
+// ---- rows that are streamed -------------------------------------------------
+//
+// With many rows a CTA walks a whole row once for its sums and once more for
+// what depends on them; the second walk finds the row in L2 (the CTAs of all
+// SMs hold some 100 MB of rows at most, usually far less).  That needs no
+// cluster and no shared memory for the row, so several CTAs a SM cover each
+// other's barriers.
+
+template <typename T>
+struct RowStream {
+  static constexpr int kE = Vec<T>::kN;
+  const T* g;   // 16-byte aligned: vector v is g[v * kE ..]; row element i is g[ph + i]
+  int ph, end;  // the row's elements are [ph, end)
+  int nvec;
+
+  __device__ __forceinline__ RowStream(const T* row, int vocab) {
+    ph = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    g = row - ph;
+    end = ph + vocab;
+    nvec = (end + kE - 1) / kE;
+  }
+  __device__ __forceinline__ bool whole(int v) const {
+    return (v > 0 || ph == 0) && (v + 1) * kE <= end;
+  }
+  // Vector v, -inf outside the row.
+  __device__ __forceinline__ Vec<T> load(int v) const {
+    if (whole(v)) return *reinterpret_cast<const Vec<T>*>(g + v * kE);
+    Vec<T> x;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const int i = v * kE + e;
+      x.v[e] = i >= ph && i < end ? g[i] : narrow<T>(-CUDART_INF_F);
+    }
+    return x;
+  }
+};
+
+// The i-th pair of a vector's elements.
+__device__ __forceinline__ float2 pair_of(const Vec<float>& x, int i) {
+  return make_float2(x.v[2 * i], x.v[2 * i + 1]);
+}
+__device__ __forceinline__ float2 pair_of(const Vec<__half>& x, int i) {
+  return __half22float2(__halves2half2(x.v[2 * i], x.v[2 * i + 1]));
+}
+__device__ __forceinline__ float2 pair_of(const Vec<__nv_bfloat16>& x, int i) {
+  return __bfloat1622float2(__halves2bfloat162(x.v[2 * i], x.v[2 * i + 1]));
+}
+__device__ __forceinline__ void set_pair(Vec<float>& x, int i, float2 y) {
+  x.v[2 * i] = y.x;
+  x.v[2 * i + 1] = y.y;
+}
+__device__ __forceinline__ void set_pair(Vec<__half>& x, int i, float2 y) {
+  const __half2 h = __float22half2_rn(y);
+  x.v[2 * i] = __low2half(h);
+  x.v[2 * i + 1] = __high2half(h);
+}
+__device__ __forceinline__ void set_pair(Vec<__nv_bfloat16>& x, int i, float2 y) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(y);
+  x.v[2 * i] = __low2bfloat16(h);
+  x.v[2 * i + 1] = __high2bfloat16(h);
+}
+
+// Largest element of a vector; a NaN counts as less than any number.
+__device__ __forceinline__ float vec_max(const Vec<float>& x) {
+  return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
+}
+__device__ __forceinline__ float vec_max(const Vec<__half>& x) {
+  const __half2* h = reinterpret_cast<const __half2*>(x.v);
+  const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
+__device__ __forceinline__ float vec_max(const Vec<__nv_bfloat16>& x) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(x.v);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
+
+// Running largest logit m and sum of 2^((x - m) c), 32 bits.  -inf and 0 when
+// nothing above -inf was added; NaN once a NaN or +inf was.
+struct SoftSum {
+  float m, s;
+
+  __device__ __forceinline__ SoftSum() : m(-INFINITY), s(0.0f) {}
+
+  // Adds the vectors x[0..kU): one test for a new maximum, then pairs on the
+  // packed 32-bit pipe.
+  template <typename T, int kU>
+  __device__ __forceinline__ void add(const Vec<T> (&x)[kU], float c) {
+    float vm = vec_max(x[0]);
+#pragma unroll
+    for (int u = 1; u < kU; ++u) vm = fmaxf(vm, vec_max(x[u]));
+    if (vm > m) {
+      s *= exp2_fast((m - vm) * c);
+      m = vm;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+    const float2 minus = make_float2(-ref, -ref), scale = make_float2(c, c);
+    float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int i = 0; i < Vec<T>::kN / 2; ++i) {
+        const float2 t = __fmul2_rn(__fadd2_rn(pair_of(x[u], i), minus), scale);
+        sum = __fadd2_rn(sum, make_float2(exp2_fast(t.x), exp2_fast(t.y)));
+      }
+    s += sum.x + sum.y;
+  }
+  __device__ __forceinline__ unsigned long long pack() const {
+    return ((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s);
+  }
+  __device__ __forceinline__ static SoftSum unpack(unsigned long long v) {
+    SoftSum r;
+    r.m = __uint_as_float((uint32_t)(v >> 32));
+    r.s = __uint_as_float((uint32_t)v);
+    return r;
+  }
+  __device__ __forceinline__ static SoftSum join(SoftSum a, SoftSum b, float c) {
+    SoftSum r;
+    r.m = fmaxf(a.m, b.m);
+    const float fa = a.m == r.m ? 1.0f : exp2_fast((a.m - r.m) * c);
+    const float fb = b.m == r.m ? 1.0f : exp2_fast((b.m - r.m) * c);
+    r.s = __fadd_rn(__fmul_rn(a.s, fa), __fmul_rn(b.s, fb));
+    return r;
+  }
+};
+
+// Rows from which on streaming is used: one a SM.
+constexpr int kStreamRows = 148;
+
+// Threads for a CTA that streams rows of `nvec` vectors: a power of two, at
+// least four vectors a thread where the row has them.
+inline int stream_threads(int vocab, int elem_bytes) {
+  const int nvec = vocab * elem_bytes / 16 + 1;
+  int t = 32;
+  while (t < kMaxThreads && t * 4 < nvec) t *= 2;
+  return t;
 }
 
 // Short rows (at most kShortVocab tokens): a thread owns a row, a CTA kShortRows

@@ -114,6 +114,182 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   }
 }
 
+// Many rows: a CTA streams a row for its maxima and sum, then again to collect
+// what reaches the bound.
+struct TopStreamSmem {
+  ReduceScratch red;
+  TokenList list;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __restrict__ logits,
+                                                                    int64_t row_stride, int vocab,
+                                                                    TopArgs a) {
+  __shared__ TopStreamSmem sm;
+  constexpr int kE = Vec<T>::kN, kU = 4;
+  const int64_t r = blockIdx.x;
+  const T* g = logits + r * row_stride;
+  const RowStream<T> row(g, vocab);
+  Reducer<false> red(&sm.red);
+  const int tid = threadIdx.x, threads = blockDim.x;
+  if (tid == 0) sm.list.count = 0;
+
+  const float c = kLog2ef / a.temperature;
+  SoftSum soft;
+  float part[kU];  // largest logit of every kU-th of the thread's vectors
+#pragma unroll
+  for (int u = 0; u < kU; ++u) part[u] = -CUDART_INF_F;
+  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
+    Vec<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = v0 + u * threads;
+      if (v < row.nvec) x[u] = row.load(v);
+      else
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) part[u] = fmaxf(part[u], vec_max(x[u]));
+    if (a.log_norm) soft.add(x, c);
+  }
+  const float tmax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  if (a.log_norm) {
+    if (soft.s != soft.s) {
+      // a NaN or +inf among the thread's logits: again, one at a time, without
+      // the NaN (with a +inf the sum is not used)
+      soft = SoftSum();
+      soft.m = tmax;
+      for (int v = tid; v < row.nvec; v += threads) {
+        const Vec<T> x = row.load(v);
+        for (int e = 0; e < kE; ++e) {
+          const float y = widen(x.v[e]);
+          if (y == y && tmax > -CUDART_INF_F) soft.s += exp2_fast((y == tmax ? 0.0f : y - tmax) * c);
+        }
+      }
+    }
+    soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
+      return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
+    }));
+    if (tid == 0) {
+      const bool inf = soft.m == -CUDART_INF_F || soft.m == CUDART_INF_F;
+      a.log_norm[r] =
+          inf ? soft.m : (float)((double)soft.m / (double)a.temperature + log((double)soft.s));
+    }
+  }
+  // a lower bound of the k-th largest logit: one that k of the threads' own
+  // maxima reach, or k of the maxima of quarters of their logits
+  uint32_t bound = 0;
+  if (a.k <= threads / 2) {
+    bound = reached_by(order_key(tmax), a.k);
+  } else {
+    for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+      int n = 0;
+#pragma unroll
+      for (int u = 0; u < kU; ++u) n += __syncthreads_count(order_key(part[u]) >= (bound | bit));
+      if (n >= a.k) bound |= bit;
+    }
+  }
+  const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
+  __syncthreads();
+  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
+    Vec<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int v = v0 + u * threads;
+      if (v < row.nvec) x[u] = row.load(v);
+      else
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (!(vec_max(x[u]) >= from)) continue;
+      const int i0 = (v0 + u * threads) * kE - row.ph;
+      for (int e = 0; e < kE; ++e) {
+        const float y = widen(x[u].v[e]);
+        if (y >= from) {
+          const unsigned at = atomicAdd(&sm.list.count, 1u);
+          if (at < kListCap) sm.list.item[at] = list_item(order_key(y), i0 + e);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int n = (int)sm.list.count;
+  if (n > kListCap) {
+    // many equal logits or a large k: the k-th largest key by bisection, and
+    // the last index taken of its tokens
+    auto count = [&](uint32_t lo, int last) {
+      int m = 0;
+      for (int v = tid; v < row.nvec; v += threads) {
+        const Vec<T> x = row.load(v);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const float y = widen(x.v[e]);
+          const uint32_t k = y == y ? order_key(y) : 0u;
+          m += k > lo || (k == lo && v * kE - row.ph + e <= last);
+        }
+      }
+      return red.sum(m);
+    };
+    uint32_t lo = bound > kKeyNegInf ? bound : kKeyNegInf + 1, hi = 0xffffffffu;
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo) / 2 + 1;
+      if (count(mid, 0x7fffffff) >= a.k) lo = mid;
+      else hi = mid - 1;
+    }
+    int i_lo = 0, i_hi = vocab - 1;
+    while (i_lo < i_hi) {
+      const int mid = (i_lo + i_hi) / 2;
+      if (count(lo, mid) >= a.k) i_hi = mid;
+      else i_lo = mid + 1;
+    }
+    if (tid == 0) sm.list.count = 0;
+    __syncthreads();
+    for (int v = tid; v < row.nvec; v += threads) {
+      const Vec<T> x = row.load(v);
+      for (int e = 0; e < kE; ++e) {
+        const float y = widen(x.v[e]);
+        const uint32_t k = y == y ? order_key(y) : 0u;
+        const int i = v * kE - row.ph + e;
+        if (k > lo || (k == lo && i <= i_lo))
+          sm.list.item[atomicAdd(&sm.list.count, 1u)] = list_item(k, i);
+      }
+    }
+    __syncthreads();
+    n = a.k;
+  }
+  T* values = static_cast<T*>(a.values) + r * a.k;
+  int32_t* tokens = a.tokens + r * a.k;
+  if (n <= 2 * threads) {
+    // an item's place is the number of larger ones
+    for (int i = tid; i < n; i += threads) {
+      const unsigned long long me = sm.list.item[i];
+      int place = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) place += sm.list.item[j] > me;
+      if (place < a.k) {
+        const int index = item_index(me);
+        values[place] = g[index];
+        tokens[place] = index;
+      }
+    }
+    for (int i = n + tid; i < a.k; i += threads) {
+      values[i] = narrow<T>(-CUDART_INF_F);
+      tokens[i] = -1;
+    }
+    return;
+  }
+  sort_down(sm.list.item, n);
+  for (int i = tid; i < a.k; i += threads) {
+    const bool there = i < n;
+    const int index = there ? item_index(sm.list.item[i]) : -1;
+    values[i] = there ? g[index] : narrow<T>(-CUDART_INF_F);
+    tokens[i] = index;
+  }
+}
+
 // Short rows, one thread each: takes the largest remaining token k times.  The
 // row's listing replaces its logits' copy place by place and leaves coalesced.
 template <typename T>
@@ -175,6 +351,11 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
     top_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
         static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    return cudaGetLastError();
+  }
+  if (v.rows >= kStreamRows) {
+    top_stream_kernel<T><<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), 0, st>>>(
+        static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
     return cudaGetLastError();
   }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));
