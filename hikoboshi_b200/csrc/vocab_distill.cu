@@ -48,8 +48,9 @@ struct RowFactors {
 
 // The body's largest logit and sum (relative to it), the listed tokens' largest
 // logit and, where the unlisted tokens are a class of their own, their sum
-// relative to the row's largest; q_sum the listed masses' sum (1 without the
-// class) and dot = sum q (log q - z).
+// relative to the row's largest; q_sum the listed masses' sum (1, or NaN, without
+// the class) and dot = sum q (log q - (x - xmax) / tau).  Everything is relative
+// to the row's largest logit, so logits of any size leave the loss its digits.
 __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double body, float lmax,
                                                   double listed, double q_sum, double dot,
                                                   double inv_tau, float temperature, float weight,
@@ -61,12 +62,13 @@ __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double 
   const double total = body * lift + listed;  // relative to xmax
   double rest_q = 0.0;
   if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
-  const double mass = tail ? q_sum + rest_q : 1.0;
+  const double mass = q_sum + rest_q;
   if (loss) {
-    const double log_total = (double)xmax * inv_tau + log(total);
-    double l = dot + (tail ? q_sum : 1.0) * log_total;
+    const double log_total = log(total);
+    double l = dot + q_sum * log_total;
     if (rest_q > 0.0)
-      l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
+      l += rest_q * (log(rest_q) - log(body) + log_total -
+                     ((double)bmax - (double)xmax) * inv_tau);
     *loss = (float)((double)temperature * (double)temperature * l);
   }
   const double wt = (double)weight * (double)temperature;
@@ -91,7 +93,7 @@ struct Listing {
   double* q;   // teacher's mass
   float* x;    // student's logit, where this CTA owns the entry
   int* token;  // -1: no entry
-  int* own;    // 1: this CTA's slice has the token and this entry stands for it
+  int* own;    // 1: the token is this CTA's and the entry stands for it; -1: another does
 };
 
 // Writes one value over the row's slice of the gradient.
@@ -149,7 +151,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     if (grad) fill_slice(row, grad, zero_weight ? 0.0f : v);
     return;
   }
-  // log q_k = a_k / tau - norm, in natural logarithms
+  // log q_k = (a_k - from) / tau - norm
   double norm;
   if (tail) {
     norm = (double)a.log_norm[r];
@@ -158,16 +160,17 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     double e = 0.0;
     for (int k = threadIdx.x; k < a.k; k += blockDim.x)
       if (ls.token[k] >= 0) e += exp(((double)ls.x[k] - (double)amax) * inv_tau);
-    norm = (double)amax * inv_tau + log(block.sum(e));
+    norm = log(block.sum(e));
   }
-  double q_sum = 0.0, dot = 0.0;  // sum q, sum over owned entries q (log q - z)
+  const double from = tail ? 0.0 : (double)amax;
+  double q_sum = 0.0, dot = 0.0;  // sum q; over the entries in this slice sum q log q
   float listed_max = -CUDART_INF_F;
   for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
     const int token = ls.token[k];
     double q = 0.0;
     int own = 0;
     if (token >= 0) {
-      const double log_q = (double)ls.x[k] * inv_tau - norm;
+      const double log_q = ((double)ls.x[k] - from) * inv_tau - norm;
       q = exp(log_q);
       q_sum += q;
       const int at = token - row.start;
@@ -175,8 +178,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
         const float x = widen(row.s[row.ph + at]);
         ls.x[k] = x;
         listed_max = fmaxf(listed_max, x);
-        // a mass that underflows counts nothing, also on a masked token
-        if (q != 0.0) dot += q * (log_q - (double)x * inv_tau);
+        if (q != 0.0) dot += q * log_q;
         own = 1;
       }
     }
@@ -195,12 +197,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   bool twice = false;
   for (int k = threadIdx.x; k < a.k; k += blockDim.x)
     if (ls.own[k] && reinterpret_cast<Bits*>(row.s)[row.ph + ls.token[k] - row.start] != (Bits)k) {
-      ls.own[k] = 0;
+      ls.own[k] = -1;
       twice = true;
     }
   const bool row_twice = __syncthreads_or(twice);
   for (int k = threadIdx.x; k < a.k; k += blockDim.x)
-    if (ls.own[k])
+    if (ls.own[k] > 0)
       row.s[row.ph + ls.token[k] - row.start] = narrow<T>(tail ? -CUDART_INF_F : ls.x[k]);
   __syncthreads();
 
@@ -208,7 +210,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   float bmax = -CUDART_INF_F;
   row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) bmax = fmaxf(bmax, widen(x.v[e]));
+    for (int e = 0; e < kE; ++e) bmax = fmaxf(bmax, x.at(e));
   });
   bmax = red.max(bmax);           // of the body: all tokens, or the unlisted ones
   listed_max = red.max(listed_max);
@@ -218,18 +220,23 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   float s = 0.0f;
   row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) s += exp2_fast((widen(x.v[e]) - base) * c);
+    for (int e = 0; e < kE; ++e) s += exp2_fast((x.at(e) - base) * c);
   });
   double listed = 0.0;  // sum over listed tokens exp((x - xmax) / tau)
-  if (tail)
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x)
-      if (ls.own[k]) listed += exp(((double)ls.x[k] - (double)xmax) * inv_tau);
+  for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+    if (ls.own[k] == 0) continue;
+    const double z = ((double)ls.x[k] - (double)xmax) * inv_tau, q = ls.q[k];
+    // a mass that underflows counts nothing, also on a masked token
+    if (q != 0.0) dot -= q * z;
+    if (tail && ls.own[k] > 0) listed += exp(z);
+  }
   const double body = red.sum((double)s);
-  if (tail) listed = red.sum(listed);
-  dot = red.sum(dot);
+  const double2 sums = red.sum(make_double2(listed, dot));
+  listed = sums.x;
+  dot = sums.y;
   const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
   if (threadIdx.x == 0)
-    sm.f = row_factors(tail, bmax, body, listed_max, listed, tail ? q_sum : 1.0, dot, inv_tau,
+    sm.f = row_factors(tail, bmax, body, listed_max, listed, q_sum, dot, inv_tau,
                        a.temperature, weight, writer && a.loss ? a.loss + r : nullptr);
   if (grad == nullptr) return;
   if (weight == 0.0f) {
@@ -243,19 +250,22 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   row.for_each([&](int i0, const Vec<T>& x) {
     Vec<T> y;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) y.v[e] = narrow<T>(exp2_fast((widen(x.v[e]) - base) * c) * f.G);
+    for (int i = 0; i < kE / 2; ++i) {
+      const float2 p = x.pair(i);
+      y.set_pair(i, make_float2(exp2_fast((p.x - base) * c) * f.G, exp2_fast((p.y - base) * c) * f.G));
+    }
     const int e0 = i0 - row.start + row.ph;
     if (same_phase && e0 >= row.ph && e0 + kE <= row.ph + row.n) {
       *reinterpret_cast<Vec<T>*>(gs + e0) = y;
     } else {
 #pragma unroll
       for (int e = 0; e < kE; ++e)
-        if (e0 + e >= row.ph && e0 + e < row.ph + row.n) gs[e0 + e] = y.v[e];
+        if (e0 + e >= row.ph && e0 + e < row.ph + row.n) gs[e0 + e] = reinterpret_cast<const T*>(y.w)[e];
     }
   });
   __syncthreads();
   for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
-    if (!ls.own[k]) continue;
+    if (ls.own[k] <= 0) continue;
     double q = ls.q[k];
     if (row_twice) {
       q = 0.0;
@@ -345,8 +355,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
       ls.x[k] = x;
       lmax = fmaxf(lmax, x);
       q_sum += q;
-      // a mass that underflows counts nothing, also on a masked token
-      if (q != 0.0) dot += q * (log_q - (double)x * inv_tau);
+      if (q != 0.0) dot += q * log_q;
       const int bit = token + row.ph;
       own = !(atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u);
       twice |= !own;
@@ -354,54 +363,51 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
     ls.q[k] = q;
     ls.own[k] = own;
   }
-  q_sum = red.sum(q_sum);
-  dot = red.sum(dot);
+  const double2 masses = red.sum(make_double2(q_sum, dot));
+  q_sum = masses.x;
+  dot = masses.y;
   const bool row_twice = __syncthreads_or(twice);
   double q_scale = 1.0;
   if (!tail) {
     q_scale = 1.0 / q_sum;
     dot = dot * q_scale - log(q_sum);
-    q_sum = 1.0;
+    q_sum *= q_scale;
     lmax = -CUDART_INF_F;
   }
 
   const float c = (float)(kLog2e * inv_tau);
   SoftSum soft;
-  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
-    Vec<T> x[kU];
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int v = v0 + u * threads;
-      if (v < row.nvec) x[u] = row.load(v);
-      else
-#pragma unroll
-        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
-    }
+  row.template walk<kU>([&](auto& x, int v, int step, bool) {
     if (tail) {
+      constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int v = v0 + u * threads;
-        if (v >= row.nvec) continue;
-        const uint32_t m = marks[v * kE >> 5] >> (v * kE & 31) & ((1u << kE) - 1u);
+      for (int u = 0; u < n; ++u) {
+        const int e0 = (v + u * step) * kE;
+        const uint32_t m = marks[e0 >> 5] >> (e0 & 31) & ((1u << kE) - 1u);
         if (m)
 #pragma unroll
           for (int e = 0; e < kE; ++e)
-            if (m >> e & 1u) x[u].v[e] = narrow<T>(-CUDART_INF_F);
+            if (m >> e & 1u) x[u].clear(e);
       }
     }
     soft.add(x, c);
-  }
+  });
   soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
     return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
   }));
-  double listed = 0.0;
-  if (tail) {
-    lmax = red.max(lmax);
-    const float xmax = fmaxf(soft.m, lmax);
-    for (int k = tid; k < a.k; k += threads)
-      if (ls.own[k]) listed += exp(((double)ls.x[k] - (double)xmax) * inv_tau);
-    listed = red.sum(listed);
+  if (tail) lmax = red.max(lmax);
+  const float xmax = fmaxf(soft.m, lmax);
+  double listed = 0.0, cross = 0.0;
+  for (int k = tid; k < a.k; k += threads) {
+    if (ls.token[k] < 0) continue;
+    const double z = ((double)ls.x[k] - (double)xmax) * inv_tau, q = ls.q[k];
+    // a mass that underflows counts nothing, also on a masked token
+    if (q != 0.0) cross += q * z;
+    if (tail && ls.own[k]) listed += exp(z);
   }
+  const double2 sums = red.sum(make_double2(listed, cross));
+  listed = sums.x;
+  dot -= sums.y * q_scale;
   if (tid == 0)
     sm.f = row_factors(tail, soft.m, (double)soft.s, lmax, listed, q_sum, dot, inv_tau,
                        a.temperature, weight, a.loss ? a.loss + r : nullptr);
@@ -416,32 +422,26 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
   const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
   const float2 minus = make_float2(-f.base, -f.base), scale = make_float2(c, c),
                G = make_float2(f.G, f.G);
-  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
-    Vec<T> x[kU];
+  row.template walk<kU>([&](auto& x, int v, int step, bool whole) {
+    constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int v = v0 + u * threads;
-      if (v < row.nvec) x[u] = row.load(v);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int v = v0 + u * threads;
-      if (v >= row.nvec) continue;
+    for (int u = 0; u < n; ++u) {
+      const int e0 = (v + u * step) * kE;
       Vec<T> y;
 #pragma unroll
       for (int i = 0; i < kE / 2; ++i) {
-        const float2 t = __fmul2_rn(__fadd2_rn(pair_of(x[u], i), minus), scale);
-        set_pair(y, i, __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), G));
+        const float2 t = __fmul2_rn(__fadd2_rn(x[u].pair(i), minus), scale);
+        y.set_pair(i, __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), G));
       }
-      if (same_phase && row.whole(v)) {
-        __stcs(reinterpret_cast<uint4*>(gv + v * kE), *reinterpret_cast<const uint4*>(&y));
+      if (same_phase && whole) {
+        __stcs(reinterpret_cast<uint4*>(gv + e0), *reinterpret_cast<const uint4*>(&y));
       } else {
 #pragma unroll
         for (int e = 0; e < kE; ++e)
-          if (v * kE + e >= row.ph && v * kE + e < row.end) gv[v * kE + e] = y.v[e];
+          if (e0 + e >= row.ph && e0 + e < row.end) gv[e0 + e] = reinterpret_cast<const T*>(y.w)[e];
       }
     }
-  }
+  });
   __syncthreads();
   for (int k = tid; k < a.k; k += threads) {
     if (!ls.own[k]) continue;
@@ -508,17 +508,17 @@ __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logi
           if (a.tokens[r * a.k + k] >= 0 && v != -CUDART_INF_F)
             e += exp(((double)v - (double)amax) * inv_tau);
         }
-        norm = (double)amax * inv_tau + log(e);
+        norm = log(e);
       }
       double q_sum = 0.0, dot = 0.0;
       for (int k = 0; k < a.k; ++k) {
         const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
         const int token = a.tokens[r * a.k + k];
         if (token < 0 || v == -CUDART_INF_F) continue;
-        const double log_q = (double)v * inv_tau - norm;
+        const double log_q = ((double)v - (tail ? 0.0 : (double)amax)) * inv_tau - norm;
         const double q = exp(log_q);
         q_sum += q;
-        if (q != 0.0) dot += q * (log_q - (double)x[token * kShortPitch] * inv_tau);
+        if (q != 0.0) dot += q * log_q;
         qs[token * kShortRows] += q;
       }
       // the body is the whole row, or its unlisted tokens; the rest of the
@@ -537,36 +537,22 @@ __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logi
       double rest = 0.0;
       for (int i = 0; i < vocab; ++i) {
         const float v = x[i * kShortPitch];
+        const double q = qs[i * kShortRows];
+        // a mass that underflows counts nothing, also on a masked token
+        if (q != 0.0) dot -= q * (((double)v - (double)xmax) * inv_tau);
         if (body_mask >> i & 1u) s += exp2_fast((v - base) * c);
         else rest += exp(((double)v - (double)xmax) * inv_tau);
       }
-      const double body = (double)s;
-      const double lift =
-          bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
-      const double total = body * lift + rest;
-      const double log_total = (double)xmax * inv_tau + log(total);
-      double rest_q = 0.0;
-      if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
-      const double mass = tail ? q_sum + rest_q : 1.0;
-      if (a.loss) {
-        double l = dot + (tail ? q_sum : 1.0) * log_total;
-        if (rest_q > 0.0)
-          l += rest_q * (log(rest_q) - ((double)bmax * inv_tau + log(body) - log_total));
-        a.loss[r] = (float)((double)a.temperature * (double)a.temperature * l);
-      }
+      const RowFactors f = row_factors(tail, bmax, (double)s, lmax, rest, q_sum, dot, inv_tau,
+                                       a.temperature, weight, a.loss ? a.loss + r : nullptr);
       if (a.grad) {
-        const double wt = (double)weight * (double)a.temperature;
-        double factor = mass * lift / total;
-        if (rest_q > 0.0) factor -= rest_q / body;
-        const float G = (float)(wt * factor);
-        const double P = wt * mass / total;
         for (int i = 0; i < vocab; ++i) {
           const float v = x[i * kShortPitch];
           float g;
           if (weight == 0.0f) g = 0.0f;
           else if (listed >> i & 1u)
-            g = (float)(P * exp(((double)v - (double)xmax) * inv_tau) - wt * qs[i * kShortRows]);
-          else g = exp2_fast((v - base) * c) * G;
+            g = (float)(f.P * exp(((double)v - f.shift) * inv_tau) - f.Q * qs[i * kShortRows]);
+          else g = exp2_fast((v - base) * c) * f.G;
           x[i * kShortPitch] = g;
         }
       }

@@ -52,12 +52,86 @@ __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float x) {
   return __float2bfloat16_rn(x);
 }
 
-// 16 bytes of a row.
+// 16 bytes of a row, as 32-bit words: 16-bit elements stay packed in pairs.
 template <typename T>
 struct alignas(16) Vec {
   static constexpr int kN = 16 / (int)sizeof(T);
-  T v[kN];
+  uint32_t w[4];
+
+  __device__ __forceinline__ float at(int e) const;    // element e, widened
+  __device__ __forceinline__ void clear(int e);        // element e = -inf
+  __device__ __forceinline__ float2 pair(int i) const; // elements 2 i and 2 i + 1
+  __device__ __forceinline__ void set_pair(int i, float2 y);
+  __device__ __forceinline__ float largest() const;    // a NaN is less than any number
 };
+
+template <>
+__device__ __forceinline__ float Vec<float>::at(int e) const {
+  return __uint_as_float(w[e]);
+}
+template <>
+__device__ __forceinline__ float Vec<__half>::at(int e) const {
+  return __half2float(__ushort_as_half((unsigned short)(w[e >> 1] >> (16 * (e & 1)))));
+}
+template <>
+__device__ __forceinline__ float Vec<__nv_bfloat16>::at(int e) const {
+  return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+}
+template <>
+__device__ __forceinline__ void Vec<float>::clear(int e) {
+  w[e] = 0xff800000u;
+}
+template <>
+__device__ __forceinline__ void Vec<__half>::clear(int e) {
+  w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | 0xfc000000u : (w[e >> 1] & 0xffff0000u) | 0xfc00u;
+}
+template <>
+__device__ __forceinline__ void Vec<__nv_bfloat16>::clear(int e) {
+  w[e >> 1] = e & 1 ? (w[e >> 1] & 0xffffu) | 0xff800000u : (w[e >> 1] & 0xffff0000u) | 0xff80u;
+}
+template <>
+__device__ __forceinline__ float2 Vec<float>::pair(int i) const {
+  return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+}
+template <>
+__device__ __forceinline__ float2 Vec<__half>::pair(int i) const {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+}
+template <>
+__device__ __forceinline__ float2 Vec<__nv_bfloat16>::pair(int i) const {
+  return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ void Vec<float>::set_pair(int i, float2 y) {
+  w[2 * i] = __float_as_uint(y.x);
+  w[2 * i + 1] = __float_as_uint(y.y);
+}
+template <>
+__device__ __forceinline__ void Vec<__half>::set_pair(int i, float2 y) {
+  const __half2 h = __float22half2_rn(y);
+  w[i] = *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ void Vec<__nv_bfloat16>::set_pair(int i, float2 y) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(y);
+  w[i] = *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ float Vec<float>::largest() const {
+  return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
+}
+template <>
+__device__ __forceinline__ float Vec<__half>::largest() const {
+  const __half2* h = reinterpret_cast<const __half2*>(w);
+  const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
+template <>
+__device__ __forceinline__ float Vec<__nv_bfloat16>::largest() const {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(w);
+  const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+  return fmaxf(m.x, m.y);
+}
 
 // Order-preserving key of a value: a < b <=> key(a) < key(b); -0 and +0 share
 // one key.  NaN never reaches it (rows are cleaned on load).
@@ -166,9 +240,21 @@ struct RowSlice {
 // Reductions over the CTA and its cluster; every thread gets the result, the
 // same bits in every CTA.  The partial results are added in a fixed order.
 struct ReduceScratch {
-  alignas(8) unsigned char warp[2][kMaxWarps * 8];
-  alignas(8) unsigned char cta[2][kMaxCluster * 8];
+  alignas(16) unsigned char warp[2][kMaxWarps * 16];
+  alignas(16) unsigned char cta[2][kMaxCluster * 16];
 };
+
+__device__ __forceinline__ double2 operator+(double2 a, double2 b) {
+  return make_double2(a.x + b.x, a.y + b.y);
+}
+template <typename V>
+__device__ __forceinline__ V shfl_xor(V v, int o) {
+  return __shfl_xor_sync(0xffffffffu, v, o);
+}
+template <>
+__device__ __forceinline__ double2 shfl_xor(double2 v, int o) {
+  return make_double2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o));
+}
 
 template <bool kClustered>
 struct Reducer {
@@ -179,9 +265,9 @@ struct Reducer {
 
   template <typename V, typename Op>
   __device__ __forceinline__ V all(V v, Op op) {
-    static_assert(sizeof(V) <= 8, "one slot is 8 bytes");
+    static_assert(sizeof(V) <= 16, "one slot is 16 bytes");
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = op(v, shfl_xor(v, o));
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
     V* part = reinterpret_cast<V*>(sc->warp[buf]);
     if (lane == 0) part[warp] = v;
@@ -207,7 +293,7 @@ struct Reducer {
   // call.
   template <typename V>
   __device__ __forceinline__ const V* spread(V v) {
-    static_assert(sizeof(V) <= 8, "one slot is 8 bytes");
+    static_assert(sizeof(V) <= 16, "one slot is 16 bytes");
     V* slots = reinterpret_cast<V*>(sc->cta[buf]);
     if (kClustered) {
       auto cl = cg::this_cluster();
@@ -258,7 +344,7 @@ __device__ int collect(const RowSlice<T, kClustered>& row, Reducer<kClustered>& 
   row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const float v = widen(x.v[e]);
+      const float v = x.at(e);
       if (pick(i0 + e, v)) {
         const unsigned at = atomicAdd(&list.count, 1u);
         if (at < kListCap) list.item[at] = list_item(order_key(v), i0 + e);
@@ -349,69 +435,54 @@ struct RowStream {
   static constexpr int kE = Vec<T>::kN;
   const T* g;   // 16-byte aligned: vector v is g[v * kE ..]; row element i is g[ph + i]
   int ph, end;  // the row's elements are [ph, end)
-  int nvec;
+  int lo, hi;   // vectors that lie wholly in the row
 
   __device__ __forceinline__ RowStream(const T* row, int vocab) {
     ph = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
     g = row - ph;
     end = ph + vocab;
-    nvec = (end + kE - 1) / kE;
+    lo = ph > 0;
+    hi = end / kE;
   }
-  __device__ __forceinline__ bool whole(int v) const {
-    return (v > 0 || ph == 0) && (v + 1) * kE <= end;
-  }
-  // Vector v, -inf outside the row.
-  __device__ __forceinline__ Vec<T> load(int v) const {
-    if (whole(v)) return *reinterpret_cast<const Vec<T>*>(g + v * kE);
+  // A vector that lies partly in the row, -inf outside.
+  __device__ __forceinline__ Vec<T> partial(int v) const {
     Vec<T> x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.w[i] = 0;
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
       const int i = v * kE + e;
-      x.v[e] = i >= ph && i < end ? g[i] : narrow<T>(-CUDART_INF_F);
+      if (i >= ph && i < end) reinterpret_cast<T*>(x.w)[e] = g[i];
+      else x.clear(e);
     }
     return x;
   }
+  // f(x, v, step, whole) over the CTA's threads: x an array of vectors v, v +
+  // step, ...  kU loads are in flight at a time; the ends of the row that fill
+  // no vector come last, one vector each.
+  template <int kU, typename F>
+  __device__ __forceinline__ void walk(F f) const {
+    const int threads = blockDim.x;
+    const Vec<T>* vec = reinterpret_cast<const Vec<T>*>(g);
+    int v = lo + (int)threadIdx.x;
+    for (; v + (kU - 1) * threads < hi; v += kU * threads) {
+      Vec<T> x[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) x[u] = vec[v + u * threads];
+      f(x, v, threads, true);
+    }
+    for (; v < hi; v += threads) {
+      Vec<T> x[1] = {vec[v]};
+      f(x, v, threads, true);
+    }
+    if ((threadIdx.x == 0 && lo > 0) ||
+        ((int)threadIdx.x == threads - 1 && hi >= lo && hi * kE < end)) {
+      const int at = threadIdx.x == 0 && lo > 0 ? 0 : hi;
+      Vec<T> x[1] = {partial(at)};
+      f(x, at, threads, false);
+    }
+  }
 };
-
-// The i-th pair of a vector's elements.
-__device__ __forceinline__ float2 pair_of(const Vec<float>& x, int i) {
-  return make_float2(x.v[2 * i], x.v[2 * i + 1]);
-}
-__device__ __forceinline__ float2 pair_of(const Vec<__half>& x, int i) {
-  return __half22float2(__halves2half2(x.v[2 * i], x.v[2 * i + 1]));
-}
-__device__ __forceinline__ float2 pair_of(const Vec<__nv_bfloat16>& x, int i) {
-  return __bfloat1622float2(__halves2bfloat162(x.v[2 * i], x.v[2 * i + 1]));
-}
-__device__ __forceinline__ void set_pair(Vec<float>& x, int i, float2 y) {
-  x.v[2 * i] = y.x;
-  x.v[2 * i + 1] = y.y;
-}
-__device__ __forceinline__ void set_pair(Vec<__half>& x, int i, float2 y) {
-  const __half2 h = __float22half2_rn(y);
-  x.v[2 * i] = __low2half(h);
-  x.v[2 * i + 1] = __high2half(h);
-}
-__device__ __forceinline__ void set_pair(Vec<__nv_bfloat16>& x, int i, float2 y) {
-  const __nv_bfloat162 h = __float22bfloat162_rn(y);
-  x.v[2 * i] = __low2bfloat16(h);
-  x.v[2 * i + 1] = __high2bfloat16(h);
-}
-
-// Largest element of a vector; a NaN counts as less than any number.
-__device__ __forceinline__ float vec_max(const Vec<float>& x) {
-  return fmaxf(fmaxf(x.v[0], x.v[1]), fmaxf(x.v[2], x.v[3]));
-}
-__device__ __forceinline__ float vec_max(const Vec<__half>& x) {
-  const __half2* h = reinterpret_cast<const __half2*>(x.v);
-  const float2 m = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-  return fmaxf(m.x, m.y);
-}
-__device__ __forceinline__ float vec_max(const Vec<__nv_bfloat16>& x) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(x.v);
-  const float2 m = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
-  return fmaxf(m.x, m.y);
-}
 
 // Running largest logit m and sum of 2^((x - m) c), 32 bits.  -inf and 0 when
 // nothing above -inf was added; NaN once a NaN or +inf was.
@@ -423,10 +494,10 @@ struct SoftSum {
   // Adds the vectors x[0..kU): one test for a new maximum, then pairs on the
   // packed 32-bit pipe.
   template <typename T, int kU>
-  __device__ __forceinline__ void add(const Vec<T> (&x)[kU], float c) {
-    float vm = vec_max(x[0]);
+  __device__ __forceinline__ void add(Vec<T> (&x)[kU], float c) {
+    float vm = x[0].largest();
 #pragma unroll
-    for (int u = 1; u < kU; ++u) vm = fmaxf(vm, vec_max(x[u]));
+    for (int u = 1; u < kU; ++u) vm = fmaxf(vm, x[u].largest());
     if (vm > m) {
       s *= exp2_fast((m - vm) * c);
       m = vm;
@@ -438,7 +509,7 @@ struct SoftSum {
     for (int u = 0; u < kU; ++u)
 #pragma unroll
       for (int i = 0; i < Vec<T>::kN / 2; ++i) {
-        const float2 t = __fmul2_rn(__fadd2_rn(pair_of(x[u], i), minus), scale);
+        const float2 t = __fmul2_rn(__fadd2_rn(x[u].pair(i), minus), scale);
         sum = __fadd2_rn(sum, make_float2(exp2_fast(t.x), exp2_fast(t.y)));
       }
     s += sum.x + sum.y;

@@ -83,7 +83,7 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
   row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const double w = f(i0 + e, widen(x.v[e]));
+      const double w = f(i0 + e, x.at(e));
       if (w >= 0.0) {
         mine += w;
         ++n;
@@ -128,7 +128,7 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
       double w[kE], sum = 0.0;
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        w[e] = v < end ? f(i0 + e, widen(reinterpret_cast<const Vec<T>*>(row.s)[v].v[e])) : 0.0;
+        w[e] = v < end ? f(i0 + e, reinterpret_cast<const Vec<T>*>(row.s)[v].at(e)) : 0.0;
         w[e] = w[e] > 0.0 ? w[e] : 0.0;
         sum += w[e];
       }
@@ -293,8 +293,8 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
   row.for_each([&](int i0, Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const float v = widen(x.v[e]);
-      if (v != v) x.v[e] = narrow<T>(-CUDART_INF_F);
+      const float v = x.at(e);
+      if (v != v) x.clear(e);
       if (v > tmax) {
         tmax = v;
         ibest = i0 + e;
@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
       int c = 0;
       row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
-        for (int e = 0; e < kE; ++e) c += order_key(widen(x.v[e])) >= lo;
+        for (int e = 0; e < kE; ++e) c += order_key(x.at(e)) >= lo;
       });
       return red.sum(c);
     };
@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        const float v = widen(x.v[e]);
+        const float v = x.at(e);
         if (in_head(i0 + e, order_key(v))) m += wt.weight(v);
       }
     });
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        const float v = widen(x.v[e]);
+        const float v = x.at(e);
         if (wt.below(v) <= reach && in_head(i0 + e, order_key(v))) atomicAdd(&sm.hist[bin_of(v)], 1u);
       }
     });
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
         row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            const float v = widen(x.v[e]);
+            const float v = x.at(e);
             if (wt.below(v) <= reach && in_head(i0 + e, order_key(v)) && bin_of(v) <= list_from)
               above += wt.weight(v);
           }
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
         row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
           for (int e = 0; e < kE; ++e) {
-            const float v = widen(x.v[e]);
+            const float v = x.at(e);
             const uint32_t k = order_key(v);
             if (k >= lo && in_head(i0 + e, k)) m += wt.weight(v);
           }

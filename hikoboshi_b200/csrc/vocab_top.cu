@@ -38,8 +38,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   row.for_each([&](int, Vec<T>& x) {
 #pragma unroll
     for (int e = 0; e < kE; ++e) {
-      const float v = widen(x.v[e]);
-      if (v != v) x.v[e] = narrow<T>(-CUDART_INF_F);
+      const float v = x.at(e);
+      if (v != v) x.clear(e);
       tmax = fmaxf(tmax, v);
     }
   });
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
     row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
-        const float v = widen(x.v[e]);
+        const float v = x.at(e);
         s += exp2_fast((v == xmax ? 0.0f : v - xmax) * c);
       }
     });
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
       row.for_each([&](int i0, const Vec<T>& x) {
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          const uint32_t k = order_key(widen(x.v[e]));
+          const uint32_t k = order_key(x.at(e));
           c += k > lo || (k == lo && i0 + e <= last);
         }
       });
@@ -139,20 +139,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
   float part[kU];  // largest logit of every kU-th of the thread's vectors
 #pragma unroll
   for (int u = 0; u < kU; ++u) part[u] = -CUDART_INF_F;
-  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
-    Vec<T> x[kU];
+  row.template walk<kU>([&](auto& x, int, int, bool) {
+    constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int v = v0 + u * threads;
-      if (v < row.nvec) x[u] = row.load(v);
-      else
-#pragma unroll
-        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) part[u] = fmaxf(part[u], vec_max(x[u]));
+    for (int u = 0; u < n; ++u) part[u] = fmaxf(part[u], x[u].largest());
     if (a.log_norm) soft.add(x, c);
-  }
+  });
   const float tmax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
   if (a.log_norm) {
     if (soft.s != soft.s) {
@@ -160,13 +152,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
       // the NaN (with a +inf the sum is not used)
       soft = SoftSum();
       soft.m = tmax;
-      for (int v = tid; v < row.nvec; v += threads) {
-        const Vec<T> x = row.load(v);
+      row.template walk<1>([&](auto& x, int, int, bool) {
+#pragma unroll
         for (int e = 0; e < kE; ++e) {
-          const float y = widen(x.v[e]);
+          const float y = x[0].at(e);
           if (y == y && tmax > -CUDART_INF_F) soft.s += exp2_fast((y == tmax ? 0.0f : y - tmax) * c);
         }
-      }
+      });
     }
     soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
       return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
@@ -192,29 +184,22 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
   }
   const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
   __syncthreads();
-  for (int v0 = tid; v0 < row.nvec; v0 += threads * kU) {
-    Vec<T> x[kU];
+  row.template walk<kU>([&](auto& x, int v, int step, bool) {
+    constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int v = v0 + u * threads;
-      if (v < row.nvec) x[u] = row.load(v);
-      else
+    for (int u = 0; u < n; ++u) {
+      if (!(x[u].largest() >= from)) continue;
+      const int i0 = (v + u * step) * kE - row.ph;
 #pragma unroll
-        for (int e = 0; e < kE; ++e) x[u].v[e] = narrow<T>(-CUDART_INF_F);
-    }
-#pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (!(vec_max(x[u]) >= from)) continue;
-      const int i0 = (v0 + u * threads) * kE - row.ph;
       for (int e = 0; e < kE; ++e) {
-        const float y = widen(x[u].v[e]);
+        const float y = x[u].at(e);
         if (y >= from) {
           const unsigned at = atomicAdd(&sm.list.count, 1u);
           if (at < kListCap) sm.list.item[at] = list_item(order_key(y), i0 + e);
         }
       }
     }
-  }
+  });
   __syncthreads();
   int n = (int)sm.list.count;
   if (n > kListCap) {
@@ -222,15 +207,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
     // the last index taken of its tokens
     auto count = [&](uint32_t lo, int last) {
       int m = 0;
-      for (int v = tid; v < row.nvec; v += threads) {
-        const Vec<T> x = row.load(v);
+      row.template walk<1>([&](auto& x, int v, int, bool) {
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          const float y = widen(x.v[e]);
+          const float y = x[0].at(e);
           const uint32_t k = y == y ? order_key(y) : 0u;
           m += k > lo || (k == lo && v * kE - row.ph + e <= last);
         }
-      }
+      });
       return red.sum(m);
     };
     uint32_t lo = bound > kKeyNegInf ? bound : kKeyNegInf + 1, hi = 0xffffffffu;
@@ -247,16 +231,16 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
     }
     if (tid == 0) sm.list.count = 0;
     __syncthreads();
-    for (int v = tid; v < row.nvec; v += threads) {
-      const Vec<T> x = row.load(v);
+    row.template walk<1>([&](auto& x, int v, int, bool) {
+#pragma unroll
       for (int e = 0; e < kE; ++e) {
-        const float y = widen(x.v[e]);
+        const float y = x[0].at(e);
         const uint32_t k = y == y ? order_key(y) : 0u;
         const int i = v * kE - row.ph + e;
         if (k > lo || (k == lo && i <= i_lo))
           sm.list.item[atomicAdd(&sm.list.count, 1u)] = list_item(k, i);
       }
-    }
+    });
     __syncthreads();
     n = a.k;
   }

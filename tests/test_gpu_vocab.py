@@ -545,3 +545,111 @@ def test_gpu_refusals(vocab):
         with pytest.raises(HkbError) as e:
             call()
         assert e.value.code == 1 and "device" in e.value.detail
+
+
+# -- many rows: the kernels that stream rows instead of holding them ----------
+
+MANY = 160
+
+
+def pick(rows):
+    """Rows that are compared: from the first CTAs, the last ones, and between."""
+    return torch.tensor([0, 1, 2, 77, rows - 2, rows - 1], device="cuda")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [33, 40, 257, 1001, 4097, 33003])
+def test_many_rows_sizes(vocab, size, dtype):
+    at = pick(MANY)
+    x = logits(MANY, size, dtype, size)
+    u = torch.rand(MANY, generator=gen(1), device="cuda")
+    for f in FILTERS:
+        got = vocab.sample_tokens(x, u, **f)
+        check_sample([a[at] for a in got], x[at], u[at], **f)
+    for k in (1, 8, 200, 1024):
+        got = vocab.top_logits(x, k, temperature=0.7)
+        check_top([a[at] for a in got], x[at], k, 0.7)
+    for k in sorted({min(size, n) for n in (1, 40, 700)}):
+        for tail in (False, True):
+            v, t, norm = teacher(x, k, F32, k, 1.5, tail)
+            w = torch.rand(MANY, generator=gen(k), device="cuda") + 0.25
+            w[1] = 0.0
+            loss, grad = vocab.distill_loss_and_grad(x, v, t, row_weights=w, temperature=1.5,
+                                                     teacher_log_norm=norm)
+            n = norm[at] if tail else None
+            check_distill(loss[at], grad[at], x[at], v[at], t[at], n, 1.5, w[at])
+            only = vocab.distill_loss(x, v, t, temperature=1.5, teacher_log_norm=norm)
+            assert torch.equal(only, loss)
+            y = x.clone()
+            _, g2 = vocab.distill_loss_and_grad(y, v, t, row_weights=w, temperature=1.5,
+                                                teacher_log_norm=norm, grad_out=y)
+            assert torch.equal(g2, grad) and g2.data_ptr() == y.data_ptr()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [33, 100, 5000, 20001])
+def test_many_rows_edges(vocab, size, dtype):
+    x = edge_rows(size, dtype).repeat(11, 1)
+    n = len(x) // 11
+    for k in (1, 5, 300, 1024):
+        got = vocab.top_logits(x, k)
+        check_top([a[:n] for a in got], x[:n], k)
+        check_top([a[-n:] for a in got], x[-n:], k)
+    for f in FILTERS:
+        for v in (0.0, 0.3, 1.0):
+            u = torch.full((len(x),), v, device="cuda")
+            got = vocab.sample_tokens(x, u, **f)
+            check_sample([a[-n:] for a in got], x[-n:], u[-n:], **f)
+    # equal logits by the thousand: the list of candidates cannot hold them
+    flat = torch.zeros(MANY, size, dtype=dtype, device="cuda")
+    flat[:, size // 2] = 1.0
+    check_top([a[:2] for a in vocab.top_logits(flat, 20)], flat[:2], 20)
+
+
+@pytest.mark.parametrize("size", [50, 700, 9001])
+@pytest.mark.parametrize("tail", [False, True])
+def test_many_rows_listings(vocab, size, tail):
+    k = 12
+    x = logits(MANY, size, F32, 2)
+    v, t, norm = teacher(x, k, F32, 3, 1.0, True)
+    t[0] = -1
+    t[1, 3:] = -1
+    t[2, 4] = t[2, 9]
+    t[3, :] = t[3, 0]
+    v[4, 5:] = -INF
+    v[5] = -INF
+    t[6, 2] = size
+    x[0] = float("nan")
+    x[7, t[7, 1].long()] = -INF
+    x[8] = -INF
+    x[9, 5] = float("nan")
+    x[10, 7] = INF
+    x[11] = torch.finfo(F32).min
+    v[12, 3] = float("nan")
+    norm = norm if tail else None
+    loss, grad = vocab.distill_loss_and_grad(x, v, t, teacher_log_norm=norm)
+    assert loss[0] == 0 and (grad[0] == 0).all() and loss[5] == 0 and (grad[5] == 0).all()
+    assert loss[7] == INF
+    for r in (6, 8, 9, 10, 12):
+        assert loss[r].isnan() and grad[r].isnan().all(), r
+    x[0] = 0
+    at = torch.tensor([0, 1, 2, 3, 4, 5, 6, 7, 11, 13, MANY - 1], device="cuda")
+    check_distill(loss[at], grad[at], x[at], v[at], t[at], None if norm is None else norm[at], 1.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [35, 1001, 9000])
+def test_many_rows_at_any_offset_and_stride(vocab, size, dtype):
+    base = logits(1, MANY * (size + 13) + 16, dtype, 5)[0]
+    at = pick(MANY)
+    for offset in range(8):
+        x = base[offset:offset + MANY * (size + 13)].view(MANY, size + 13)[:, :size]
+        check_top([a[at] for a in vocab.top_logits(x, 9)], x[at], 9)
+        v, t, norm = teacher(x, 9, F32, 3, 1.0, True)
+        out = torch.full((MANY * (size + 5) + 16,), 7.0, dtype=dtype, device="cuda")
+        o = (3 * offset) % 8
+        g = out[o:o + MANY * (size + 5)].view(MANY, size + 5)[:, :size]
+        loss, grad = vocab.distill_loss_and_grad(x, v, t, teacher_log_norm=norm, grad_out=g)
+        check_distill(loss[at], grad[at], x[at], v[at], t[at], norm[at], 1.0)
+        g.fill_(7.0)
+        assert (out == 7.0).all()
