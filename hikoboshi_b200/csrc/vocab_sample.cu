@@ -61,8 +61,9 @@ struct SampleSmem {
   ReduceScratch red;
   ReduceScratch block;
   double seg[kMaxWarps];
+  double total;
   int found;
-  int bin[2];
+  Exp2Table table;
   TokenList list;
   unsigned hist[kBins];
 };
@@ -181,18 +182,16 @@ struct RowSettings {
 struct Weights {
   float xmax;
   double c2;  // log2(e) / T
+  const Exp2Table* table;
   __device__ __forceinline__ float below(float x) const { return x == xmax ? 0.0f : xmax - x; }
   __device__ __forceinline__ double exponent(float x) const {
     return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2;
   }
-  __device__ __forceinline__ double weight(float x) const { return exp2_neg(exponent(x)); }
+  __device__ __forceinline__ double weight(float x) const { return (*table)(exponent(x)); }
 };
 
-// Finishes a row whose kept tokens are all among the n items of this CTA's
-// list: puts them in order, cuts them to the shortest head and draws.  `need`
-// is the mass that ends the top-p head, or negative: top_p of the mass of the
-// first top_k items.
-__device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
+// finish_list for more items than threads: sorts them, twice.
+__device__ __noinline__ void finish_long_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
                             double need, int64_t r, const SampleArgs& a) {
   unsigned long long* item = sm.list.item;
   Reducer<false> red(&sm.block);
@@ -240,7 +239,7 @@ __device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowS
       if (run > target && hit == 0x7fffffff) hit = i;
     }
   }
-  hit = -red.max(-hit);
+  hit = red.min(hit);
   last = red.max(last);
   if (threadIdx.x == 0) {
     const unsigned long long it = item[hit != 0x7fffffff ? hit : last];
@@ -251,8 +250,72 @@ __device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowS
   }
 }
 
+// Finishes a row whose kept tokens are all among the n items of this CTA's
+// list: puts them in order, cuts them to the shortest head and draws.  `need`
+// is the mass that ends the top-p head, or negative: top_p of the mass of the
+// first top_k items.  No more items than threads: each item's place in the
+// order, and its running mass in index order, is counted over all items by a
+// group of threads, which takes few barriers.
+__device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
+                            double need, int64_t r, const SampleArgs& a) {
+  const int threads = blockDim.x, tid = threadIdx.x;
+  if (n > threads) {
+    finish_long_list(sm, n, wt, s, need, r, a);
+    return;
+  }
+  Reducer<false> red(&sm.block);
+  const unsigned long long* item = sm.list.item;
+  unsigned long long* sorted = sm.list.item + kMaxThreads;
+  double* weight = reinterpret_cast<double*>(sm.list.item + 2 * kMaxThreads);
+  int group = 32;  // threads an item, a power of two
+  while (group > 1 && n * group > threads) group >>= 1;
+  const int i = tid / group, part = tid % group;
+  const bool mine = i < n, lead = mine && part == 0;
+  int place = 0;
+  unsigned long long me = 0;
+  if (mine) {
+    me = item[i];
+    for (int j = part; j < n; j += group) place += item[j] > me;
+  }
+  for (int o = group >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+  if (lead) {
+    sorted[place] = me;
+    weight[place] = wt.weight(key_value(item_key(me)));
+  }
+  __syncthreads();
+  const int nk = s.top_k > 0 ? ::min(n, s.top_k) : n;
+  const double w = tid < nk ? weight[tid] : 0.0;
+  double total;
+  const double run = block_scan(w, sm.seg, &total);
+  if (need < 0.0) need = (double)s.top_p * total;
+  int kept = nk;
+  if (s.top_p < 1.0f) kept = ::min(kept, 1 + __syncthreads_count(tid < nk && run < need));
+  if (s.min_p > 0.0f) kept = ::min(kept, __syncthreads_count(tid < nk && w >= (double)s.min_p));
+  kept = ::max(kept, 1);
+  if (tid == kept - 1) sm.total = run;
+  __syncthreads();
+  const double mass = sm.total, target = s.u * mass;
+  double upto = 0.0, own = 0.0;
+  int index = -1;
+  if (mine && i < kept) {
+    me = sorted[i];
+    own = weight[i];
+    index = item_index(me);
+    for (int j = part; j < kept; j += group)
+      if (item_index(sorted[j]) <= index) upto += weight[j];
+  }
+  for (int o = group >> 1; o > 0; o >>= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
+  int token = red.min(own > 0.0 && upto > target ? index : 0x7fffffff);
+  if (token == 0x7fffffff) token = red.max(own > 0.0 ? index : -1);  // rounding, or u = 1
+  if (index == token && part == 0) {
+    a.tokens[r] = token;
+    a.log_probs[r] = (float)(wt.exponent(key_value(item_key(me))) * kLn2 - log(mass));
+    a.kept[r] = kept;
+  }
+}
+
 template <typename T, bool kClustered>
-__global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
+__global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ SampleSmem sm;
@@ -274,6 +337,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
   const bool valid = settings_valid(s.temperature, s.top_k, s.top_p, s.min_p, s.u);
   const bool writer = threadIdx.x == 0 && row.rank == 0;
   for (int b = threadIdx.x; b < kBins; b += blockDim.x) sm.hist[b] = 0;
+  sm.table.fill();
   cp_async_wait_all();
   if (kClustered) cg::this_cluster().sync();  // every CTA of the row runs from here on
   else __syncthreads();
@@ -302,7 +366,16 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     }
   });
   const uint32_t tkey = order_key(tmax);
-  const unsigned long long best = red.max(list_item(tkey, ibest));
+  // of a row with top-k: a key that ceil(k / C) threads of this CTA reach
+  if (s.top_k >= vocab) s.top_k = 0;
+  const bool list_k = s.top_k > 0 && s.top_k <= kListCap / 2 && s.temperature > 0.0f;
+  const uint32_t reached = list_k ? reached_by(tkey, (s.top_k + row.size - 1) / row.size) : 0;
+  const ulonglong2 joint = red.all(make_ulonglong2(list_item(tkey, ibest), reached),
+                                   [](ulonglong2 p, ulonglong2 q) {
+                                     return make_ulonglong2(p.x > q.x ? p.x : q.x,
+                                                            p.y < q.y ? p.y : q.y);
+                                   });
+  const unsigned long long best = joint.x;
   const uint32_t kmax = item_key(best);
   if (kmax <= kKeyNegInf || s.temperature == 0.0f) {
     if (writer) {
@@ -313,15 +386,13 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     }
     return;
   }
-  const Weights wt{key_value(kmax), kLog2e / (double)s.temperature};
-  if (s.top_k >= vocab) s.top_k = 0;
+  const Weights wt{key_value(kmax), kLog2e / (double)s.temperature, &sm.table};
 
   // Top-k of a number that fits the list: the k-th largest of the row is no
   // less than the k/C-th largest of the threads' own largest logits in the CTA
   // where that is least, and few more than k tokens reach it.
-  if (s.top_k > 0 && s.top_k <= kListCap / 2) {
-    const uint32_t mine = reached_by(tkey, (s.top_k + row.size - 1) / row.size);
-    const uint32_t bound = ~red.max(~mine);
+  if (list_k) {
+    const uint32_t bound = (uint32_t)joint.y;
     const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
     const int n = collect(row, red, sm.list, [&](int, float x) { return x >= from; });
     if (n <= kListCap) {
@@ -431,7 +502,7 @@ __global__ void __launch_bounds__(kMaxThreads, 1) sample_rows_kernel(
     }
     Reducer<false> block(&sm.block);
     certain = block.max(certain);
-    ends = ::min(kBins - 1, -block.max(-ends));
+    ends = ::min(kBins - 1, block.min(ends));
     int upto_certain = 0, upto_ends = 0;
     for (int b = b0; b < b0 + per; ++b) {
       run_number += bin_count(b);
@@ -548,10 +619,12 @@ __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __res
                                                                   int64_t row_stride, int64_t n_rows,
                                                                   int vocab, SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ Exp2Table table;
   double* w = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
   float* xs = reinterpret_cast<float*>(smem_raw + sizeof(double) * kShortRows * vocab);
   const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
   const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
+  table.fill();
   load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, true);
   __syncthreads();
   if ((int)threadIdx.x >= rows) return;
@@ -589,7 +662,7 @@ __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __res
   double sum = 0.0;
   for (int i = 0; i < vocab; ++i) {
     const float v = x[i * kShortPitch];
-    const double wi = exp2_neg(v == xmax ? 0.0 : ((double)v - (double)xmax) * c2);
+    const double wi = table(v == xmax ? 0.0 : ((double)v - (double)xmax) * c2);
     w[i * kShortRows] = wi;
     sum += wi;
   }
