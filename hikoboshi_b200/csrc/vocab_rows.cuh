@@ -174,7 +174,8 @@ struct Exp2Table {
     p = fma(p, r, 1.0) * v[n & 15];
     const double y =
         __hiloint2double(__double2hiint(p) + ((n >> 4) << 20), __double2loint(p));
-    return t > -1020.0 ? y : 0.0;
+    // t > -1020, by its upper word (t is not positive)
+    return (unsigned)__double2hiint(t) < 0xc08fe000u ? y : 0.0;
   }
 };
 
@@ -231,6 +232,17 @@ struct RowSlice {
       }
     }
     cp_async_commit();
+  }
+
+  // f(index in the row, value) over this warp's elements, leaving out vectors
+  // with no element of at least `skip`.
+  template <typename F>
+  __device__ __forceinline__ void for_each_from(float skip, F f) const {
+    for_each([&](int i0, const Vec<T>& x) {
+      if (!(x.largest() >= skip)) return;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) f(i0 + e, x.at(e));
+    });
   }
 
   // f(first element index of the vector in the row, vector) over this warp's
@@ -347,23 +359,19 @@ __device__ __forceinline__ unsigned long long list_item(uint32_t key, int index)
 __device__ __forceinline__ uint32_t item_key(unsigned long long it) { return (uint32_t)(it >> 32); }
 __device__ __forceinline__ int item_index(unsigned long long it) { return (int)~(uint32_t)it; }
 
-// Collects the row's elements for which pick(index, value) holds.  Returns
+// Collects the row's elements for which pick(index, value) holds, none of them
+// below `skip`.  Returns
 // their number; if it is at most kListCap, rank 0's list holds them all, in no
 // particular order, else the lists are of no use.
 template <typename T, bool kClustered, typename F>
 __device__ int collect(const RowSlice<T, kClustered>& row, Reducer<kClustered>& red,
-                       TokenList& list, F pick) {
-  constexpr int kE = Vec<T>::kN;
+                       TokenList& list, float skip, F pick) {
   if (threadIdx.x == 0) list.count = 0;
   __syncthreads();
-  row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const float v = x.at(e);
-      if (pick(i0 + e, v)) {
-        const unsigned at = atomicAdd(&list.count, 1u);
-        if (at < kListCap) list.item[at] = list_item(order_key(v), i0 + e);
-      }
+  row.for_each_from(skip, [&](int i, float x) {
+    if (pick(i, x)) {
+      const unsigned at = atomicAdd(&list.count, 1u);
+      if (at < kListCap) list.item[at] = list_item(order_key(x), i);
     }
   });
   __syncthreads();

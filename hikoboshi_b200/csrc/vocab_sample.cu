@@ -57,117 +57,153 @@ __device__ __forceinline__ bool settings_valid(float T, int top_k, float top_p, 
 
 constexpr int kBins = 1024;
 
+// Bounds of the running mass and the number of tokens up to a bin.
+struct alignas(16) Bounds {
+  float low, high;
+  int number, pad;
+};
+
 struct SampleSmem {
+  Bounds bounds[kMaxWarps];
   ReduceScratch red;
   ReduceScratch block;
   double seg[kMaxWarps];
+  int number[kMaxWarps];
+  double step[32];  // a warp owns at most 17 steps of 32 vectors
   double total;
-  int found;
   Exp2Table table;
   TokenList list;
   unsigned hist[kBins];
 };
 
 // First token, in index order, whose running sum of f exceeds `share` times the
-// sum over the row (`absolute`: exceeds `share`); every thread of the cluster
-// gets it.  f(index, value) is a weight, or negative for a token that is not
-// kept; *total_out is the sum, *kept_out the number of kept tokens.  Rounding
-// may leave no sum larger than the target: then the last token with f > 0 is
-// it.  -1 if there is none.
+// sum over the row (`absolute`: exceeds `share`).  f(index, value) is a weight,
+// or negative for a token that is not kept; *total_out is the sum, *kept_out
+// the number of kept tokens.  Rounding may leave no sum larger than the target:
+// then the last token with f > 0 is it.  The lanes of one warp of the cluster
+// get the token, all other threads -1.
 template <typename T, bool kClustered, typename F>
 __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& red, SampleSmem& sm,
-                      double share, bool absolute, double* total_out, int* kept_out, F f) {
+                      float skip, double share, bool absolute, double* total_out, int* kept_out,
+                      F f) {
   constexpr int kE = Vec<T>::kN;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
   double mine = 0.0;
-  int last = -1, n = 0;
-  row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const double w = f(i0 + e, x.at(e));
-      if (w >= 0.0) {
-        mine += w;
-        ++n;
-        if (w > 0.0) last = i0 + e;
-      }
+  int n = 0;
+  row.for_each_from(skip, [&](int i, float x) {
+    const double w = f(i, x);
+    if (w >= 0.0) {
+      mine += w;
+      ++n;
     }
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  n = __reduce_add_sync(0xffffffffu, n);
   __syncthreads();
-  if (lane == 0) sm.seg[warp] = mine;
-  if (threadIdx.x == 0) sm.found = -1;
-  *kept_out = red.sum(n);
-  // mass of this CTA, of the row, and of the CTAs before this one
-  double cta = 0.0;
-  for (int w = 0; w < warps; ++w) cta += sm.seg[w];
-  const double* of_cta = red.spread(cta);
-  double before = 0.0, total = 0.0;
+  if (lane == 0) {
+    sm.seg[warp] = mine;
+    sm.number[warp] = n;
+  }
+  __syncthreads();
+  // running masses of the CTA's warps, in every warp
+  const double seg = lane < warps ? sm.seg[lane] : 0.0;
+  n = __reduce_add_sync(0xffffffffu, lane < warps ? sm.number[lane] : 0);
+  double upto = seg;
+#pragma unroll
+  for (int o = 1; o < kMaxWarps; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  const double cta = __shfl_sync(0xffffffffu, upto, kMaxWarps - 1);
+  const double2* of_cta = red.spread(make_double2(cta, (double)n));
+  double total = 0.0, kept = 0.0;
   for (int c = 0; c < row.size; ++c) {
-    if (c == row.rank) before = total;
-    total += of_cta[c];
+    total += of_cta[c].x;
+    kept += of_cta[c].y;
   }
   *total_out = total;
+  *kept_out = (int)kept;
   const double target = absolute ? share : share * total;
-  // the warp in which the running sum passes the target
-  double base = before;
-  int hit = -1;
-  for (int w = 0; w < warps; ++w) {
-    const double next = base + sm.seg[w];
-    if (sm.seg[w] > 0.0 && next > target) {
-      hit = w;
-      break;
+  // the CTA in which the running sum passes the target, the same for all: the
+  // last with any mass if rounding lets none pass
+  int owner = -1;
+  double run = 0.0, before = 0.0;
+  bool passed = false;
+  for (int c = 0; c < row.size && !passed; ++c) {
+    const double m = of_cta[c].x;
+    if (m > 0.0) {
+      owner = c;
+      before = run;
+      passed = run + m > target;
     }
-    base = next;
+    run += m;
   }
-  const bool here = hit >= 0 && !(before > target);
-  if (here && warp == hit) {
-    const int begin = warp * row.per_warp, end = min(row.nvec, begin + row.per_warp);
-    int token = -1, seen = -1;
-    for (int v0 = begin; v0 < end && token < 0; v0 += 32) {
-      const int v = v0 + lane, i0 = v * kE - row.ph + row.start;
-      double w[kE], sum = 0.0;
+  if (owner != row.rank) return -1;
+  // its warp, likewise
+  unsigned pass = __ballot_sync(0xffffffffu, seg > 0.0 && before + upto > target);
+  const unsigned any = __ballot_sync(0xffffffffu, seg > 0.0);
+  const int hit = pass ? __ffs(pass) - 1 : 31 - __clz(any);
+  before += __shfl_sync(0xffffffffu, upto, hit) - __shfl_sync(0xffffffffu, seg, hit);
+  // all warps add up the 32-vector steps of that warp's vectors
+  const int begin = hit * row.per_warp, end = ::min(row.nvec, begin + row.per_warp);
+  const int steps = (end - begin + 31) / 32;
+  double w[kE];
+  auto weigh = [&](int step) {
+    const int v = begin + step * 32 + lane;
+    double sum = 0.0;
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        w[e] = v < end ? f(i0 + e, reinterpret_cast<const Vec<T>*>(row.s)[v].at(e)) : 0.0;
-        w[e] = w[e] > 0.0 ? w[e] : 0.0;
-        sum += w[e];
-      }
-      double incl = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-      }
-      const unsigned pass = __ballot_sync(0xffffffffu, sum > 0.0 && base + incl > target);
-      const unsigned any = __ballot_sync(0xffffffffu, sum > 0.0);
-      const int pick = pass ? __ffs(pass) - 1 : (any ? 31 - __clz(any) : -1);
-      if (pick >= 0) {
-        double run = __shfl_up_sync(0xffffffffu, incl, 1);
-        run = base + (lane == 0 ? 0.0 : run);
-        int t = -1;
-        bool done = false;
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          run += w[e];
-          if (!done && w[e] > 0.0) {
-            t = i0 + e;  // the last one with weight if rounding lets none pass
-            done = run > target;
-          }
-        }
-        t = __shfl_sync(0xffffffffu, t, pick);
-        seen = t;
-        if (pass) token = t;
-      }
-      base += __shfl_sync(0xffffffffu, incl, 31);
+    for (int e = 0; e < kE; ++e) {
+      w[e] = v < end ? f(v * kE - row.ph + row.start + e,
+                         reinterpret_cast<const Vec<T>*>(row.s)[v].at(e))
+                     : 0.0;
+      w[e] = w[e] > 0.0 ? w[e] : 0.0;
+      sum += w[e];
     }
-    if (token < 0) token = seen;
-    if (lane == 0) sm.found = token;
+    return sum;
+  };
+  for (int i = warp; i < steps; i += warps) {
+    double sum = weigh(i);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sm.step[i] = sum;
   }
   __syncthreads();
-  const int found = red.max(sm.found);
-  if (found >= 0) return found;
-  return red.max(last);
+  if (warp != hit) return -1;
+  const double mass = lane < steps ? sm.step[lane] : 0.0;
+  upto = mass;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  pass = __ballot_sync(0xffffffffu, mass > 0.0 && before + upto > target);
+  const unsigned heavy = __ballot_sync(0xffffffffu, mass > 0.0);
+  const int step = pass ? __ffs(pass) - 1 : 31 - __clz(heavy);
+  before += __shfl_sync(0xffffffffu, upto, step) - __shfl_sync(0xffffffffu, mass, step);
+  // its vector and element
+  const double sum = weigh(step);
+  upto = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  pass = __ballot_sync(0xffffffffu, sum > 0.0 && before + upto > target);
+  const unsigned some = __ballot_sync(0xffffffffu, sum > 0.0);
+  const int at = pass ? __ffs(pass) - 1 : 31 - __clz(some);
+  double at_run = before + upto - sum;
+  int token = -1;
+  bool done = false;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    at_run += w[e];
+    if (!done && w[e] > 0.0) {
+      token = (begin + step * 32 + lane) * kE - row.ph + row.start + e;
+      done = at_run > target;
+    }
+  }
+  return __shfl_sync(0xffffffffu, token, at);
 }
 
 // Settings of one row.
@@ -180,12 +216,11 @@ struct RowSettings {
 
 // Weights of a row: exponents relative to the largest logit.
 struct Weights {
-  float xmax;
-  double c2;  // log2(e) / T
+  float xmax;  // finite
+  double c2;   // log2(e) / T
   const Exp2Table* table;
-  __device__ __forceinline__ float below(float x) const { return x == xmax ? 0.0f : xmax - x; }
   __device__ __forceinline__ double exponent(float x) const {
-    return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2;
+    return ((double)x - (double)xmax) * c2;
   }
   __device__ __forceinline__ double weight(float x) const { return (*table)(exponent(x)); }
 };
@@ -314,6 +349,57 @@ __device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowS
   }
 }
 
+// The sums of the threads before this one.
+__device__ __forceinline__ Bounds scan_bounds(Bounds v, SampleSmem& sm) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+  Bounds incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float low = __shfl_up_sync(0xffffffffu, incl.low, o);
+    const float high = __shfl_up_sync(0xffffffffu, incl.high, o);
+    const int number = __shfl_up_sync(0xffffffffu, incl.number, o);
+    if (lane >= o) {
+      incl.low += low;
+      incl.high += high;
+      incl.number += number;
+    }
+  }
+  Bounds before;
+  before.low = __shfl_up_sync(0xffffffffu, incl.low, 1);
+  before.high = __shfl_up_sync(0xffffffffu, incl.high, 1);
+  before.number = __shfl_up_sync(0xffffffffu, incl.number, 1);
+  before.pad = 0;
+  if (lane == 0) before = Bounds{0.0f, 0.0f, 0, 0};
+  if (lane == 31) sm.bounds[warp] = incl;
+  __syncthreads();
+  for (int w = 0; w < warp && w < warps; ++w) {
+    before.low += sm.bounds[w].low;
+    before.high += sm.bounds[w].high;
+    before.number += sm.bounds[w].number;
+  }
+  return before;
+}
+
+// Of the n items of this CTA's list, in order, the one at which the running
+// mass, `above` before the first, reaches `need`; 0 if none does.
+__device__ __noinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights& wt,
+                                                          double above, double need) {
+  const unsigned long long* item = sm.list.item;
+  sort_down(sm.list.item, n);
+  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+  const int i0 = ::min(n, (int)threadIdx.x * per), i1 = ::min(n, i0 + per);
+  double mine = 0.0, total;
+  for (int i = i0; i < i1; ++i) mine += wt.weight(key_value(item_key(item[i])));
+  double run = above + (block_scan(mine, sm.seg, &total) - mine);
+  int under = 0;
+  for (int i = i0; i < i1; ++i) {
+    run += wt.weight(key_value(item_key(item[i])));
+    under += run < need;
+  }
+  under = Reducer<false>(&sm.block).sum(under);
+  return under < n ? item[under] : 0ull;
+}
+
 template <typename T, bool kClustered>
 __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
@@ -351,99 +437,104 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   }
   Reducer<kClustered> red(&sm.red);
 
-  // largest logit and its first place; NaN becomes -inf
+  // Largest logit; a NaN is less than any number in this and every later
+  // comparison, so it is never kept.
   float tmax = -CUDART_INF_F;
-  int ibest = 0x7fffffff;
-  row.for_each([&](int i0, Vec<T>& x) {
-#pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const float v = x.at(e);
-      if (v != v) x.clear(e);
-      if (v > tmax) {
-        tmax = v;
-        ibest = i0 + e;
-      }
-    }
-  });
-  const uint32_t tkey = order_key(tmax);
+  row.for_each([&](int, const Vec<T>& x) { tmax = fmaxf(tmax, x.largest()); });
   // of a row with top-k: a key that ceil(k / C) threads of this CTA reach
   if (s.top_k >= vocab) s.top_k = 0;
   const bool list_k = s.top_k > 0 && s.top_k <= kListCap / 2 && s.temperature > 0.0f;
-  const uint32_t reached = list_k ? reached_by(tkey, (s.top_k + row.size - 1) / row.size) : 0;
-  const ulonglong2 joint = red.all(make_ulonglong2(list_item(tkey, ibest), reached),
+  const uint32_t reached =
+      list_k ? reached_by(order_key(tmax), (s.top_k + row.size - 1) / row.size) : 0;
+  const ulonglong2 joint = red.all(make_ulonglong2(order_key(tmax), reached),
                                    [](ulonglong2 p, ulonglong2 q) {
                                      return make_ulonglong2(p.x > q.x ? p.x : q.x,
                                                             p.y < q.y ? p.y : q.y);
                                    });
-  const unsigned long long best = joint.x;
-  const uint32_t kmax = item_key(best);
-  if (kmax <= kKeyNegInf || s.temperature == 0.0f) {
+  float xmax = key_value((uint32_t)joint.x);
+  if (xmax == -CUDART_INF_F || s.temperature == 0.0f) {
+    const bool none = xmax == -CUDART_INF_F;
+    int first = 0x7fffffff;
+    if (!none) {
+      row.for_each_from(xmax, [&](int i, float x) {
+        if (x == xmax) first = ::min(first, i);
+      });
+      first = red.min(first);
+    }
     if (writer) {
-      const bool none = kmax <= kKeyNegInf;
-      a.tokens[r] = none ? -1 : item_index(best);
+      a.tokens[r] = none ? -1 : first;
       a.log_probs[r] = none ? -CUDART_INF_F : 0.0f;
       a.kept[r] = none ? 0 : 1;
     }
     return;
   }
-  const Weights wt{key_value(kmax), kLog2e / (double)s.temperature, &sm.table};
+  uint32_t bound = (uint32_t)joint.y;
+  double c2 = kLog2e / (double)s.temperature;
+  if (xmax == CUDART_INF_F) {
+    // Logits of +inf share the whole mass: zeros in their places, the finite
+    // ones far below and, by the factor of the exponents, without weight.
+    row.for_each([&](int, Vec<T>& x) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float v = x.at(e);
+        if (v > -CUDART_INF_F)
+          reinterpret_cast<T*>(x.w)[e] = narrow<T>(v == CUDART_INF_F ? 0.0f : -60000.0f);
+      }
+    });
+    xmax = 0.0f;
+    bound = 0;
+    c2 = 1e300;
+    __syncthreads();
+  }
+  const Weights wt{xmax, c2, &sm.table};
 
   // Top-k of a number that fits the list: the k-th largest of the row is no
   // less than the k/C-th largest of the threads' own largest logits in the CTA
   // where that is least, and few more than k tokens reach it.
   if (list_k) {
-    const uint32_t bound = (uint32_t)joint.y;
     const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
-    const int n = collect(row, red, sm.list, [&](int, float x) { return x >= from; });
+    const int n = collect(row, red, sm.list, from, [&](int, float x) { return x >= from; });
     if (n <= kListCap) {
       if (row.rank == 0) finish_list(sm, n, wt, s, -1.0, r, a);
       return;
     }
   }
 
-  // The kept head is { (key, index) : key > t, or key == t and index <= icut },
-  // further cut by min-p and by `reach`, the largest distance from the largest
-  // logit that a kept token can have.
-  uint32_t t = kKeyNegInf + 1;
+  // The kept head so far: x > xt, or x == xt and index <= icut.
+  float xt = -CUDART_MAX_NORMAL_F;
   int icut = 0x7fffffff;
-  auto in_head = [&](int i, uint32_t k) { return k > t || (k == t && i <= icut); };
+  auto in_head = [&](int i, float x) { return x >= xt && !(x == xt && i > icut); };
   if (s.top_k > 0) {
-    // largest key with at least k tokens at or above it, by bisection
-    auto count = [&](uint32_t lo) {
+    // largest value with at least k tokens at or above it, by bisection of keys
+    auto count = [&](uint32_t key) {
+      const float from = key_value(key);
       int c = 0;
-      row.for_each([&](int, const Vec<T>& x) {
-#pragma unroll
-        for (int e = 0; e < kE; ++e) c += order_key(x.at(e)) >= lo;
-      });
+      row.for_each_from(from, [&](int, float x) { c += x >= from; });
       return red.sum(c);
     };
     if (count(kKeyNegInf + 1) > s.top_k) {
-      uint32_t lo = kKeyNegInf + 1, hi = kmax;
+      uint32_t lo = kKeyNegInf + 1, hi = order_key(xmax);
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         if (count(mid) >= s.top_k) lo = mid;
         else hi = mid - 1;
       }
-      t = lo;
-      const int above = t == 0xffffffffu ? 0 : count(t + 1);
+      const int above = lo == order_key(xmax) ? 0 : count(lo + 1);
+      xt = key_value(lo);
       double ties;
       int n;
-      icut = locate(row, red, sm, (double)(s.top_k - above) - 0.5, true, &ties, &n,
-                    [&](int, float x) { return order_key(x) == t ? 1.0 : -1.0; });
+      icut = red.max(locate(row, red, sm, xt, (double)(s.top_k - above) - 0.5, true, &ties, &n,
+                            [&](int, float x) { return x == xt ? 1.0 : -1.0; }));
     }
   }
+  // Distance from the largest logit within which kept tokens lie.
   const double zmin = s.min_p > 0.0f ? log2((double)s.min_p) - 1e-3 : -CUDART_INF;
-  float reach = CUDART_INF_F;
-  if (zmin > -CUDART_INF) reach = (float)(-zmin / wt.c2) * 1.000001f;
+  float reach = s.min_p > 0.0f ? (float)(-zmin / wt.c2) * 1.000001f : CUDART_INF_F;
 
   if (s.top_p < 1.0f) {
     double m = 0.0;
-    row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const float v = x.at(e);
-        if (in_head(i0 + e, order_key(v))) m += wt.weight(v);
-      }
+    row.for_each_from(xt, [&](int i, float x) {
+      if (in_head(i, x)) m += wt.weight(x);
     });
     const double mass = red.sum(m);
     const double need = (double)s.top_p * mass;
@@ -452,26 +543,27 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const double z0 =
         fmax(zmin, log2((1.0 - (double)s.top_p) * mass / (double)vocab) - 1e-3);
     reach = (float)(-z0 / wt.c2) * 1.000001f;
+    // a vector with nothing from here on has nothing within reach
+    const float skip = fmaxf(xt, xmax - reach * 1.00001f);
     // Count the tokens within reach in bins of equal width: a bin's weights lie
     // between those of its ends, so the counts bound the running mass from both
     // sides (1e-4 covers the 32-bit arithmetic), and the border lies in the
     // few bins that the two bounds leave.
     const float scale = (float)kBins / reach;
-    auto bin_of = [&](float x) { return ::min(kBins - 1, (int)(wt.below(x) * scale)); };
-    row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const float v = x.at(e);
-        if (wt.below(v) <= reach && in_head(i0 + e, order_key(v))) atomicAdd(&sm.hist[bin_of(v)], 1u);
-      }
-    });
+    // temperatures at the ends of the type's range leave no finite bin width
+    const bool binned = scale > 0.0f && scale < CUDART_INF_F;
+    auto within = [&](int i, float x) { return xmax - x <= reach && in_head(i, x); };
+    auto bin_of = [&](float x) { return ::min(kBins - 1, (int)((xmax - x) * scale)); };
+    if (binned)
+      row.for_each_from(skip, [&](int i, float x) {
+        if (within(i, x)) atomicAdd(&sm.hist[bin_of(x)], 1u);
+      });
     if (kClustered) cg::this_cluster().sync();
     else __syncthreads();
     // every CTA adds up the whole row's bins and finds the same border
     const int per = kBins / (int)blockDim.x, b0 = (int)threadIdx.x * per;
     const float width2 = (float)(wt.c2 / (double)scale);  // of a bin, in powers of two
-    float low = 0.0f, high = 0.0f, all;
-    int number = 0;
+    Bounds mine{0.0f, 0.0f, 0, 0};
     auto bin_count = [&](int b) {
       if (!kClustered) return (int)sm.hist[b];
       int c = 0;
@@ -479,134 +571,115 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
         c += (int)cg::this_cluster().map_shared_rank(sm.hist, k)[b];
       return c;
     };
-    for (int b = b0; b < b0 + per; ++b) {
-      const float c = (float)bin_count(b);
-      low += c * exp2f(-(float)(b + 1) * width2) * 0.9999f;
-      high += c * exp2f(-(float)b * width2) * 1.0001f;
-      number += (int)c;
-    }
-    float* fscratch = reinterpret_cast<float*>(sm.seg);
-    int* iscratch = reinterpret_cast<int*>(sm.seg);
-    int number_all;
-    float run_low = block_scan(low, fscratch, &all) - low;
-    float run_high = block_scan(high, fscratch, &all) - high;
-    int run_number = block_scan(number, iscratch, &number_all) - number;
-    // last bin that is certainly kept, first bin that certainly ends the head
-    int certain = -1, ends = kBins;
-    for (int b = b0; b < b0 + per; ++b) {
-      const float c = (float)bin_count(b);
-      run_low += c * exp2f(-(float)(b + 1) * width2) * 0.9999f;
-      run_high += c * exp2f(-(float)b * width2) * 1.0001f;
-      if (run_high < (float)need * 0.9999f) certain = b;
-      if (run_low >= (float)need * 1.0001f) ends = ::min(ends, b);
-    }
-    Reducer<false> block(&sm.block);
-    certain = block.max(certain);
-    ends = ::min(kBins - 1, block.min(ends));
-    int upto_certain = 0, upto_ends = 0;
-    for (int b = b0; b < b0 + per; ++b) {
-      run_number += bin_count(b);
-      if (b == certain) upto_certain = run_number;
-      if (b == ends) upto_ends = run_number;
-    }
-    upto_certain = block.sum(upto_certain);
-    upto_ends = block.sum(upto_ends);
-    // (the others may still read this CTA's bins: until their next reduction)
-
-    // temperatures at the ends of the type's range leave no finite bin width
-    const bool binned = scale > 0.0f && scale < CUDART_INF_F;
-    const int list_from = upto_ends <= kListCap ? -1 : certain;
-    if (binned && upto_ends - (list_from < 0 ? 0 : upto_certain) <= kListCap) {
-      double above = 0.0;
-      if (list_from >= 0) {
-        row.for_each([&](int i0, const Vec<T>& x) {
+    constexpr int kKept = 4;  // bins whose counts a thread keeps
+    int counts[kKept];
 #pragma unroll
-          for (int e = 0; e < kE; ++e) {
-            const float v = x.at(e);
-            if (wt.below(v) <= reach && in_head(i0 + e, order_key(v)) && bin_of(v) <= list_from)
-              above += wt.weight(v);
-          }
+    for (int k = 0; k < kKept; ++k) counts[k] = k < per ? bin_count(b0 + k) : 0;
+    auto grow = [&](Bounds& v, int k) {
+      const int c = k < kKept ? counts[k & (kKept - 1)] : bin_count(b0 + k);
+      v.low += (float)c * exp2f(-(float)(b0 + k + 1) * width2) * 0.9999f;
+      v.high += (float)c * exp2f(-(float)(b0 + k) * width2) * 1.0001f;
+      v.number += c;
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+      if (k < per) grow(mine, k);
+    for (int k = kKept; k < per; ++k) grow(mine, k);
+    Bounds run = scan_bounds(mine, sm);
+    // last bin that is certainly kept, first bin that certainly ends the head,
+    // with the tokens up to their ends
+    unsigned long long certain = 0, ends = ~0ull;
+    auto judge = [&](int k) {
+      grow(run, k);
+      const unsigned long long v =
+          ((unsigned long long)(b0 + k + 1) << 32) | (unsigned)run.number;
+      if (run.high < (float)need * 0.9999f) certain = v;
+      if (run.low >= (float)need * 1.0001f || b0 + k == kBins - 1) ends = ::min(ends, v);
+    };
+#pragma unroll
+    for (int k = 0; k < kKept; ++k)
+      if (k < per) judge(k);
+    for (int k = kKept; k < per; ++k) judge(k);
+    Reducer<false> block(&sm.block);
+    const ulonglong2 borders = block.all(make_ulonglong2(certain, ends),
+                                         [](ulonglong2 p, ulonglong2 q) {
+                                           return make_ulonglong2(p.x > q.x ? p.x : q.x,
+                                                                  p.y < q.y ? p.y : q.y);
+                                         });
+    const int last_certain = (int)(borders.x >> 32) - 1, upto_certain = (int)(uint32_t)borders.x;
+    const int end_bin = (int)(borders.y >> 32) - 1, upto_end = (int)(uint32_t)borders.y;
+
+    const bool all_listed = upto_end <= kListCap;
+    const int list_from = all_listed ? -1 : last_certain;
+    if (binned && (all_listed || upto_end - upto_certain <= kListCap)) {
+      double above = 0.0;
+      if (!all_listed) {
+        row.for_each_from(skip, [&](int i, float x) {
+          if (within(i, x) && bin_of(x) <= list_from) above += wt.weight(x);
         });
         above = red.sum(above);
       }
-      const int n = collect(row, red, sm.list, [&](int i, float x) {
-        if (!(wt.below(x) <= reach) || !in_head(i, order_key(x))) return false;
+      const int n = collect(row, red, sm.list, skip, [&](int i, float x) {
+        if (!within(i, x)) return false;
         const int b = bin_of(x);
-        return b > list_from && b <= ends;
+        return b > list_from && b <= end_bin;
       });
-      if (list_from < 0) {
+      if (all_listed) {
         if (row.rank == 0) finish_list(sm, n, wt, s, need, r, a);
         return;
       }
       // the head ends inside the list, or (cut by min-p) nowhere
       unsigned long long border = 0;
-      if (row.rank == 0) {
-        sort_down(sm.list.item, n);
-        const int per_t = (n + (int)blockDim.x - 1) / (int)blockDim.x;
-        const int i0 = ::min(n, (int)threadIdx.x * per_t), i1 = ::min(n, i0 + per_t);
-        double mine = 0.0, total;
-        for (int i = i0; i < i1; ++i) mine += wt.weight(key_value(item_key(sm.list.item[i])));
-        double run = above + (block_scan(mine, sm.seg, &total) - mine);
-        int under = 0;
-        for (int i = i0; i < i1; ++i) {
-          run += wt.weight(key_value(item_key(sm.list.item[i])));
-          under += run < need;
-        }
-        under = block.sum(under);
-        if (under < n) border = sm.list.item[under];
-      }
+      if (row.rank == 0) border = border_in_list(sm, n, wt, above, need);
       border = red.spread(border)[0];
       if (border != 0) {
-        t = item_key(border);
+        xt = key_value(item_key(border));
         icut = item_index(border);
       }
     } else {
-      // equal logits crowd a bin: bisect between its ends
-      auto mass_from = [&](uint32_t lo) {
-        double m = 0.0;
-        row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-          for (int e = 0; e < kE; ++e) {
-            const float v = x.at(e);
-            const uint32_t k = order_key(v);
-            if (k >= lo && in_head(i0 + e, k)) m += wt.weight(v);
-          }
+      // equal logits crowd a bin: bisect
+      auto mass_from = [&](uint32_t key) {
+        const float from = key_value(key);
+        double v = 0.0;
+        row.for_each_from(from, [&](int i, float x) {
+          if (x >= from && in_head(i, x)) v += wt.weight(x);
         });
-        return red.sum(m);
+        return red.sum(v);
       };
-      uint32_t lo = t, hi = kmax;
+      uint32_t lo = order_key(xt), hi = order_key(xmax);
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         if (mass_from(mid) >= need) lo = mid;
         else hi = mid - 1;
       }
       // `lo` is the border's key: of its tokens the first `ties` are kept
-      const double above = lo == kmax ? 0.0 : mass_from(lo + 1);
-      const double w = wt.weight(key_value(lo));
+      const float border = key_value(lo);
+      const double above = lo == order_key(xmax) ? 0.0 : mass_from(lo + 1);
+      const double w = wt.weight(border);
       double ties = w > 0.0 ? ceil((need - above) / w) : 1.0;
       if (ties < 1.0) ties = 1.0;
-      const uint32_t old_t = t;
-      const int old_cut = icut;
-      t = lo;
-      icut = 0x7fffffff;
       double all_ties;
       int n;
-      icut = locate(row, red, sm, ties - 0.5, true, &all_ties, &n, [&](int i, float x) {
-        const uint32_t k = order_key(x);
-        return k == lo && (k > old_t || i <= old_cut) ? 1.0 : -1.0;
-      });
+      icut = red.max(locate(row, red, sm, border, ties - 0.5, true, &all_ties, &n,
+                            [&](int i, float x) {
+                              return x == border && in_head(i, x) ? 1.0 : -1.0;
+                            }));
+      xt = border;
     }
   }
+  // draw among the kept tokens of the whole row
+  const float skip = fmaxf(xt, xmax - reach * 1.00001f);
   double total;
   int n;
-  const int token = locate(row, red, sm, s.u, false, &total, &n, [&](int i, float x) {
-    if (!(wt.below(x) <= reach) || !in_head(i, order_key(x))) return -1.0;
+  const int token = locate(row, red, sm, skip, s.u, false, &total, &n, [&](int i, float x) {
+    if (!in_head(i, x)) return -1.0;
     const double w = wt.weight(x);
     return w >= (double)s.min_p ? w : -1.0;
   });
-  if (writer) {
+  if (token >= 0 && (threadIdx.x & 31) == 0) {
+    const float x = fminf(widen(g[token]), xmax);
     a.tokens[r] = token;
-    a.log_probs[r] = (float)(wt.exponent(widen(g[token])) * kLn2 - log(total));
+    a.log_probs[r] = (float)(wt.exponent(x) * kLn2 - log(total));
     a.kept[r] = n;
   }
 }

@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   const uint32_t mine = reached_by(order_key(tmax), (a.k + row.size - 1) / row.size);
   const uint32_t bound = ~red.max(~mine);
   const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
-  int n = collect(row, red, sm.list, [&](int, float x) { return x >= from; });
+  int n = collect(row, red, sm.list, from, [&](int, float x) { return x >= from; });
   if (n > kListCap) {
     // many equal logits, or a row whose large logits lie side by side: the
     // k-th largest key by bisection, and the last index taken of its tokens
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
       else i_lo = mid + 1;
     }
     icut = i_lo;
-    n = collect(row, red, sm.list, [&](int i, float x) {
+    n = collect(row, red, sm.list, key_value(t), [&](int i, float x) {
       const uint32_t k = order_key(x);
       return k > t || (k == t && i <= icut);
     });
