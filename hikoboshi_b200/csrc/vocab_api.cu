@@ -1,5 +1,6 @@
 // C entry points of the operators on vocabulary rows: argument checks, the
 // device guard and the launch.  No workspace, no state, no synchronisation.
+#include <atomic>
 #include <cmath>
 
 #include "hkb_mpnn.h"
@@ -10,39 +11,40 @@ namespace {
 
 hkb_status invalid(const char* why) { return {HKB_INVALID_ARGUMENT, why}; }
 
+// Whether a device can run this build; the answer is asked for once a device.
+hkb_status usable(int device) {
+  constexpr int kKnown = 64;
+  static std::atomic<int> known[kKnown];  // 0: not asked yet, 1: it can
+  if (device >= 0 && device < kKnown && known[device].load(std::memory_order_relaxed) == 1)
+    return {HKB_OK, ""};
+  int count = 0;
+  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+    cudaGetLastError();
+    return {HKB_UNAVAILABLE, "no CUDA device is available"};
+  }
+  if (device < 0 || device >= count) return invalid("device ordinal out of range");
+  int major = 0;
+  if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess) {
+    cudaGetLastError();
+    return {HKB_UNAVAILABLE, "the CUDA device cannot be used"};
+  }
+  if (major != 10) return {HKB_UNAVAILABLE, "this build targets sm_100a (B200) only"};
+  if (device < kKnown) known[device].store(1, std::memory_order_relaxed);
+  return {HKB_OK, ""};
+}
+
 // Makes `device` current for the call and puts the caller's device back.
 class DeviceGuard {
  public:
-  explicit DeviceGuard(int device) {
-    int count = 0;
-    if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
-      cudaGetLastError();
-      status_ = {HKB_UNAVAILABLE, "no CUDA device is available"};
-      return;
-    }
-    if (device < 0 || device >= count) {
-      status_ = invalid("device ordinal out of range");
-      return;
-    }
-    int major = 0;
+  explicit DeviceGuard(int device) : status_(usable(device)) {
+    if (status_.code != HKB_OK) return;
     if (cudaGetDevice(&previous_) != cudaSuccess ||
-        cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device) != cudaSuccess) {
+        (previous_ != device && cudaSetDevice(device) != cudaSuccess)) {
       cudaGetLastError();
       status_ = {HKB_UNAVAILABLE, "the CUDA device cannot be used"};
       return;
     }
-    if (major != 10) {
-      status_ = {HKB_UNAVAILABLE, "this build targets sm_100a (B200) only"};
-      return;
-    }
-    if (previous_ != device) {
-      if (cudaSetDevice(device) != cudaSuccess) {
-        cudaGetLastError();
-        status_ = {HKB_UNAVAILABLE, "the CUDA device cannot be used"};
-        return;
-      }
-      restore_ = true;
-    }
+    restore_ = previous_ != device;
   }
   ~DeviceGuard() {
     if (restore_) cudaSetDevice(previous_);
@@ -52,7 +54,7 @@ class DeviceGuard {
   const hkb_status& status() const { return status_; }
 
  private:
-  hkb_status status_{HKB_OK, ""};
+  hkb_status status_;
   int previous_ = 0;
   bool restore_ = false;
 };

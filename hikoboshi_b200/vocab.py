@@ -20,8 +20,7 @@ Unfit arguments raise :class:`HkbError` with ``HKB_INVALID_ARGUMENT``.
 """
 from __future__ import annotations
 
-import ctypes
-import math
+from ctypes import byref
 from typing import NamedTuple
 
 import torch
@@ -30,6 +29,9 @@ from . import _lib
 from ._lib import HkbError, check
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_FLOAT = (torch.float32,)
+_INT = (torch.int32,)
+_UNIFORMS = (torch.float32, torch.float64)
 
 
 class SampledTokens(NamedTuple):
@@ -55,61 +57,80 @@ def _is_tensor(x, name: str) -> torch.Tensor:
 
 
 def _rows(x: torch.Tensor, name: str = "logits"):
-    """(2-d view, leading shape) of [.., V] logits; never a copy."""
+    """(rows, leading shape) of [.., V] logits, as the library takes them; never
+    a copy."""
     _is_tensor(x, name)
-    if x.dtype not in _DTYPES:
+    code = _DTYPES.get(x.dtype)
+    if code is None:
         raise _invalid(f"{name} must be float32, float16 or bfloat16")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) == 0 or shape[-1] == 0:
         raise _invalid(f"{name} must have a last dimension of at least one token")
-    if x.layout != torch.strided or x.is_conj() or x.is_neg():
+    if x.layout is not torch.strided or x.is_neg():
         raise _invalid(f"{name} must be a plain strided tensor")
-    lead = x.shape[:-1]
-    if x.dim() == 1:
-        x = x.unsqueeze(0)
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    v = shape[-1]
+    stride = x.stride()
+    if v > 1 and stride[-1] != 1:
         raise _invalid(f"{name} must have a last dimension of stride 1")
-    if x.dim() > 2:
-        try:
-            x = x.view(-1, x.shape[-1]) if x.numel() else x.reshape(0, x.shape[-1])
-        except RuntimeError:
+    if len(shape) == 2:
+        n, step = shape[0], stride[0]
+    else:
+        n, step = _flatten(shape[:-1], stride[:-1])
+        if step is None:
             raise _invalid(f"{name}: the leading dimensions must flatten to rows of one stride")
-    return x, lead
+    return _lib.VocabRows(n, v if v < 2**31 else 2**31 - 1, code, x.data_ptr(),
+                          step if n > 1 else v), shape[:-1]
 
 
-def _struct_rows(x: torch.Tensor) -> _lib.VocabRows:
-    stride = x.stride(0) if x.shape[0] > 1 else x.shape[1]
-    return _lib.VocabRows(x.shape[0], min(x.shape[1], 2**31 - 1), _DTYPES[x.dtype], x.data_ptr(),
-                          stride)
+def _flatten(shape, stride):
+    """(number, stride) of the dimensions taken as one, stride None if they
+    have no common one."""
+    n, step = 1, 0
+    for size, st in zip(reversed(shape), reversed(stride)):
+        if size == 1:
+            continue
+        if n == 1:
+            step = st
+        elif size and n and st != step * n:
+            step = None
+            break
+        n *= size
+    n = 1
+    for size in shape:
+        n *= size
+    return (n, step) if n else (0, 0)
 
 
-def _on(x: torch.Tensor, like: torch.Tensor, name: str) -> None:
-    if x.device != like.device:
-        raise _invalid(f"{name} must be on the logits' device")
-
-
-def _vector(x, lead, like, dtypes, name) -> torch.Tensor:
+def _vector(x, lead, device, dtypes, name) -> torch.Tensor:
     """A dense per-row tensor of the leading shape."""
     _is_tensor(x, name)
-    _on(x, like, name)
+    if x.device != device:
+        raise _invalid(f"{name} must be on the logits' device")
     if x.dtype not in dtypes:
         raise _invalid(f"{name} must be " + " or ".join(str(d).split(".")[1] for d in dtypes))
     if x.shape != lead:
         raise _invalid(f"{name} must have one number per row")
-    if not x.is_contiguous():
+    if not x.is_contiguous() or x.is_neg():
         raise _invalid(f"{name} must be contiguous")
     return x
 
 
-def _call(fn, x: torch.Tensor, *args) -> None:
-    if x.device.type != "cuda":
-        # the library checks the other arguments first, then refuses the device
-        st = fn(-1, *args, None)
-        if st.code == _lib.HKB_INVALID_ARGUMENT and st.detail == b"device ordinal out of range":
-            raise _invalid("logits must be on a CUDA device")
-        check(st)
+# the current stream's handle without a Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(fn, device: torch.device, *args) -> None:
+    if device.type == "cuda":
+        st = fn(device.index, *args, _raw_stream(device.index))
+        if st.code:
+            check(st)
         return
-    stream = torch.cuda.current_stream(x.device).cuda_stream
-    check(fn(x.device.index, *args, ctypes.c_void_p(stream)))
+    # the library checks the other arguments first, then refuses the device
+    st = fn(-1, *args, None)
+    if st.code == _lib.HKB_INVALID_ARGUMENT and st.detail == b"device ordinal out of range":
+        raise _invalid("logits must be on a CUDA device")
+    check(st)
 
 
 def _number(v, name: str) -> float:
@@ -135,31 +156,36 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0,
     give token -1, log_prob NaN and kept 0; rows with no logit above -inf give
     -1, -inf and 0.  A NaN logit counts as -inf.
     """
-    x, lead = _rows(logits)
-    u = _vector(uniforms, lead, x, (torch.float32, torch.float64), "uniforms")
+    rows, lead = _rows(logits)
+    device = logits.device
+    u = _vector(uniforms, lead, device, _UNIFORMS, "uniforms")
     s = _lib.SampleSettings()
-    hold = []
-    for name, v, dtype in (("temperature", temperature, torch.float32),
-                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                           ("min_p", min_p, torch.float32)):
-        if isinstance(v, torch.Tensor):
-            hold.append(_vector(v, lead, x, (dtype,), name))
-            setattr(s, name + "s" if name != "temperature" else "temperatures", v.data_ptr())
-        elif name == "top_k":
-            if isinstance(v, bool) or not isinstance(v, int):
-                raise _invalid("top_k must be a whole number or a tensor of one per row")
-            s.top_k = max(-1, min(v, 2**31 - 1))
-        else:
-            setattr(s, name, _number(v, name))
     s.uniforms = u.data_ptr()
     s.uniforms_dtype = _lib.F64 if u.dtype == torch.float64 else _lib.F32
-    out = SampledTokens(torch.empty(lead, dtype=torch.int32, device=x.device),
-                        torch.empty(lead, dtype=torch.float32, device=x.device),
-                        torch.empty(lead, dtype=torch.int32, device=x.device))
-    rows = _struct_rows(x)
-    o = _lib.SampleOut(out.tokens.data_ptr(), out.log_probs.data_ptr(), out.kept.data_ptr())
-    _call(_lib.load().hkb_sample_tokens, x, ctypes.byref(rows), ctypes.byref(s), ctypes.byref(o))
-    return out
+    if isinstance(temperature, torch.Tensor):
+        s.temperatures = _vector(temperature, lead, device, _FLOAT, "temperature").data_ptr()
+    else:
+        s.temperature = _number(temperature, "temperature")
+    if isinstance(top_k, torch.Tensor):
+        s.top_ks = _vector(top_k, lead, device, _INT, "top_k").data_ptr()
+    elif isinstance(top_k, bool) or not isinstance(top_k, int):
+        raise _invalid("top_k must be a whole number or a tensor of one per row")
+    else:
+        s.top_k = max(-1, min(top_k, 2**31 - 1))
+    if isinstance(top_p, torch.Tensor):
+        s.top_ps = _vector(top_p, lead, device, _FLOAT, "top_p").data_ptr()
+    else:
+        s.top_p = _number(top_p, "top_p")
+    if isinstance(min_p, torch.Tensor):
+        s.min_ps = _vector(min_p, lead, device, _FLOAT, "min_p").data_ptr()
+    else:
+        s.min_p = _number(min_p, "min_p")
+    tokens = torch.empty(lead, dtype=torch.int32, device=device)
+    log_probs = torch.empty(lead, dtype=torch.float32, device=device)
+    kept = torch.empty(lead, dtype=torch.int32, device=device)
+    o = _lib.SampleOut(tokens.data_ptr(), log_probs.data_ptr(), kept.data_ptr())
+    _call(_lib.load().hkb_sample_tokens, device, byref(rows), byref(s), byref(o))
+    return SampledTokens(tokens, log_probs, kept)
 
 
 def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
@@ -167,106 +193,97 @@ def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
     tokens, in the order (logit down, index up), and log sum exp(x / temperature).
     Places past a row's logits above -inf hold (-inf, -1); a NaN logit counts
     as -inf."""
-    x, lead = _rows(logits)
+    rows, lead = _rows(logits)
     if isinstance(k, bool) or not isinstance(k, int):
         raise _invalid("k must be a whole number")
     k = max(-1, min(k, 2**31 - 1))
     n = max(0, min(k, _lib.LISTING_MAX))
-    out = TopLogits(torch.empty((*lead, n), dtype=x.dtype, device=x.device),
-                    torch.empty((*lead, n), dtype=torch.int32, device=x.device),
-                    torch.empty(lead, dtype=torch.float32, device=x.device))
-    rows = _struct_rows(x)
-    o = _lib.TopOut(out.values.data_ptr(), out.tokens.data_ptr(), out.log_norm.data_ptr())
-    _call(_lib.load().hkb_top_logits, x, ctypes.byref(rows), k,
-          _number(temperature, "temperature"), ctypes.byref(o))
-    return out
+    device = logits.device
+    values = torch.empty((*lead, n), dtype=logits.dtype, device=device)
+    tokens = torch.empty((*lead, n), dtype=torch.int32, device=device)
+    log_norm = torch.empty(lead, dtype=torch.float32, device=device)
+    o = _lib.TopOut(values.data_ptr(), tokens.data_ptr(), log_norm.data_ptr())
+    _call(_lib.load().hkb_top_logits, device, byref(rows), k,
+          _number(temperature, "temperature"), byref(o))
+    return TopLogits(values, tokens, log_norm)
 
 
-def _teacher(x, lead, values, tokens, log_norm, temperature) -> _lib.DistillTeacher:
+def _teacher(lead, device, values, tokens, log_norm, temperature) -> _lib.DistillTeacher:
     _is_tensor(values, "teacher_values")
     _is_tensor(tokens, "teacher_tokens")
-    if values.dtype not in _DTYPES:
+    code = _DTYPES.get(values.dtype)
+    if code is None:
         raise _invalid("teacher_values must be float32, float16 or bfloat16")
-    if tokens.dtype != torch.int32:
+    if tokens.dtype is not torch.int32:
         raise _invalid("teacher_tokens must be int32")
-    if values.dim() == 0 or values.shape[:-1] != lead or tokens.shape != values.shape:
+    shape = values.shape
+    if len(shape) == 0 or shape[:-1] != lead or tokens.shape != shape:
         raise _invalid("teacher_values and teacher_tokens must be [.., k] with the logits' rows")
-    _on(values, x, "teacher_values")
-    _on(tokens, x, "teacher_tokens")
-    if not values.is_contiguous() or not tokens.is_contiguous():
+    if values.device != device:
+        raise _invalid("teacher_values must be on the logits' device")
+    if tokens.device != device:
+        raise _invalid("teacher_tokens must be on the logits' device")
+    if not values.is_contiguous() or not tokens.is_contiguous() or values.is_neg():
         raise _invalid("teacher_values and teacher_tokens must be contiguous")
-    t = _lib.DistillTeacher()
-    t.k = min(values.shape[-1], 2**31 - 1)
-    t.dtype = _DTYPES[values.dtype]
-    t.values = values.data_ptr()
-    t.tokens = tokens.data_ptr()
     if log_norm is not None:
-        t.log_norm = _vector(log_norm, lead, x, (torch.float32,), "teacher_log_norm").data_ptr()
-        if t.log_norm is None:  # no rows: keep the form of the loss
-            t.log_norm = 0
-    t.temperature = _number(temperature, "temperature")
-    return t
+        log_norm = _vector(log_norm, lead, device, _FLOAT, "teacher_log_norm").data_ptr()
+    return _lib.DistillTeacher(min(shape[-1], 2**31 - 1), code, values.data_ptr(),
+                               tokens.data_ptr(), log_norm, _number(temperature, "temperature"))
 
 
-def _weights(w, lead, x):
+def _weights(w, lead, device):
     """(pointer, stride) of per-row weights: one stride, 0 where broadcast."""
     if w is None:
         return None, 0
     _is_tensor(w, "row_weights")
-    _on(w, x, "row_weights")
-    if w.dtype != torch.float32:
+    if w.device != device:
+        raise _invalid("row_weights must be on the logits' device")
+    if w.dtype is not torch.float32:
         raise _invalid("row_weights must be float32")
     if w.shape != lead:
         raise _invalid("row_weights must have one number per row")
-    if w.numel() and all(s == 0 or n == 1 for s, n in zip(w.stride(), w.shape)):
-        return w.data_ptr(), 0
-    if w.dim() <= 1:
-        return w.data_ptr(), w.stride(0) if w.dim() else 0
-    try:
-        return w.data_ptr(), w.view(-1).stride(0)
-    except RuntimeError:
+    _, step = _flatten(w.shape, w.stride())
+    if step is None or w.is_neg():
         raise _invalid("row_weights must flatten to one stride")
+    return w.data_ptr(), step
 
 
-def _distill(x, teacher, loss, grad, weights) -> None:
-    rows = _struct_rows(x)
-    o = _lib.DistillOut()
-    if loss is not None:
-        o.loss = loss.data_ptr()
-    if grad is not None:
-        o.grad = grad.data_ptr()
-        o.grad_row_stride = grad.stride(0) if grad.shape[0] > 1 else grad.shape[1]
-    o.row_weights, o.row_weight_stride = weights
-    _call(_lib.load().hkb_distill, x, ctypes.byref(rows), ctypes.byref(teacher), ctypes.byref(o))
+def _backward(logits, values, tokens, log_norm, temperature, grad_loss):
+    rows, lead = _rows(logits)
+    device = logits.device
+    t = _teacher(lead, device, values, tokens, log_norm, temperature)
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    if rows.rows:
+        _, step = _flatten(grad_loss.shape, grad_loss.stride())
+        if step is None or grad_loss.is_neg():
+            grad_loss = grad_loss.clone(memory_format=torch.contiguous_format).resolve_neg()
+        pointer, step = _weights(grad_loss, lead, device)
+        o = _lib.DistillOut(None, grad.data_ptr(), logits.shape[-1], pointer, step)
+        _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
+    return grad
+
+
+def _forward(logits, values, tokens, log_norm, temperature):
+    rows, lead = _rows(logits)
+    device = logits.device
+    t = _teacher(lead, device, values, tokens, log_norm, temperature)
+    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    o = _lib.DistillOut(loss.data_ptr(), None, 0, None, 0)
+    _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
+    return loss
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, tokens, log_norm, temperature):
-        x, lead = _rows(logits)
-        t = _teacher(x, lead, values, tokens, log_norm, temperature)
-        loss = torch.empty(lead, dtype=torch.float32, device=x.device)
-        if x.shape[0]:
-            _distill(x, t, loss, None, (None, 0))
         ctx.save_for_backward(logits, values, tokens, log_norm)
         ctx.temperature = temperature
-        return loss
+        return _forward(logits, values, tokens, log_norm, temperature)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, values, tokens, log_norm = ctx.saved_tensors
-        x, lead = _rows(logits)
-        t = _teacher(x, lead, values, tokens, log_norm, ctx.temperature)
-        grad = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
-        if x.shape[0]:
-            try:
-                w = _weights(grad_loss, lead, x)
-            except HkbError:
-                grad_loss = grad_loss.contiguous()
-                w = _weights(grad_loss, lead, x)
-            _distill(x, t, None, grad.view(x.shape), w)
-        return grad, None, None, None, None
+        return _backward(*ctx.saved_tensors, ctx.temperature, grad_loss), None, None, None, None
 
 
 def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=None,
@@ -288,9 +305,10 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     graph (an eager graph of the same leaves would break the capture): there
     it raises HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.
     """
-    _rows(logits)
-    if (torch.is_grad_enabled() and logits.requires_grad and logits.is_cuda
-            and torch.cuda.is_current_stream_capturing()):
+    if not (isinstance(logits, torch.Tensor) and logits.requires_grad
+            and torch.is_grad_enabled()):
+        return _forward(logits, teacher_values, teacher_tokens, teacher_log_norm, temperature)
+    if logits.is_cuda and torch.cuda.is_current_stream_capturing():
         raise HkbError(_lib.HKB_FAILED_PRECONDITION,
                        "autograd through distill_loss cannot be captured; capture "
                        "distill_loss_and_grad")
@@ -305,20 +323,23 @@ def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log
     (weights 1 by default), in the logits' type.  A row of weight 0 has gradient
     0.  ``grad_out`` receives the gradient and may be ``logits`` itself, whose
     memory the gradient then takes; autograd does not see this call."""
-    x, lead = _rows(logits)
-    x = x.detach()
-    t = _teacher(x, lead, teacher_values, teacher_tokens, teacher_log_norm, temperature)
-    w = _weights(row_weights, lead, x)
-    loss = torch.empty(lead, dtype=torch.float32, device=x.device)
+    rows, lead = _rows(logits)
+    device = logits.device
+    t = _teacher(lead, device, teacher_values, teacher_tokens, teacher_log_norm, temperature)
+    pointer, step = _weights(row_weights, lead, device)
     if grad_out is None:
-        grad_out = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
+        grad_out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        grad_stride = logits.shape[-1]
     else:
         _is_tensor(grad_out, "grad_out")
-        _on(grad_out, x, "grad_out")
-        if grad_out.dtype != x.dtype or grad_out.shape != logits.shape:
+        if grad_out.device != device:
+            raise _invalid("grad_out must be on the logits' device")
+        if grad_out.dtype is not logits.dtype or grad_out.shape != logits.shape:
             raise _invalid("grad_out must have the logits' type and shape")
-    g, _ = _rows(grad_out.detach(), "grad_out")
-    _distill(x, t, loss, g, w)
+        grad_stride = _rows(grad_out, "grad_out")[0].row_stride
+    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    o = _lib.DistillOut(loss.data_ptr(), grad_out.data_ptr(), grad_stride, pointer, step)
+    _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
     return loss, grad_out
 
 
