@@ -180,9 +180,9 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0,
         s.min_ps = _vector(min_p, lead, device, _FLOAT, "min_p").data_ptr()
     else:
         s.min_p = _number(min_p, "min_p")
-    tokens = torch.empty(lead, dtype=torch.int32, device=device)
-    log_probs = torch.empty(lead, dtype=torch.float32, device=device)
-    kept = torch.empty(lead, dtype=torch.int32, device=device)
+    tokens = logits.new_empty(lead, dtype=torch.int32)
+    log_probs = logits.new_empty(lead, dtype=torch.float32)
+    kept = logits.new_empty(lead, dtype=torch.int32)
     o = _lib.SampleOut(tokens.data_ptr(), log_probs.data_ptr(), kept.data_ptr())
     _call(_lib.load().hkb_sample_tokens, device, byref(rows), byref(s), byref(o))
     return SampledTokens(tokens, log_probs, kept)
@@ -199,9 +199,9 @@ def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
     k = max(-1, min(k, 2**31 - 1))
     n = max(0, min(k, _lib.LISTING_MAX))
     device = logits.device
-    values = torch.empty((*lead, n), dtype=logits.dtype, device=device)
-    tokens = torch.empty((*lead, n), dtype=torch.int32, device=device)
-    log_norm = torch.empty(lead, dtype=torch.float32, device=device)
+    values = logits.new_empty((*lead, n), dtype=logits.dtype)
+    tokens = logits.new_empty((*lead, n), dtype=torch.int32)
+    log_norm = logits.new_empty(lead, dtype=torch.float32)
     o = _lib.TopOut(values.data_ptr(), tokens.data_ptr(), log_norm.data_ptr())
     _call(_lib.load().hkb_top_logits, device, byref(rows), k,
           _number(temperature, "temperature"), byref(o))
@@ -252,7 +252,7 @@ def _backward(logits, values, tokens, log_norm, temperature, grad_loss):
     rows, lead = _rows(logits)
     device = logits.device
     t = _teacher(lead, device, values, tokens, log_norm, temperature)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    grad = logits.new_empty(logits.shape)
     if rows.rows:
         _, step = _flatten(grad_loss.shape, grad_loss.stride())
         if step is None or grad_loss.is_neg():
@@ -267,7 +267,7 @@ def _forward(logits, values, tokens, log_norm, temperature):
     rows, lead = _rows(logits)
     device = logits.device
     t = _teacher(lead, device, values, tokens, log_norm, temperature)
-    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    loss = logits.new_empty(lead, dtype=torch.float32)
     o = _lib.DistillOut(loss.data_ptr(), None, 0, None, 0)
     _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
     return loss
@@ -328,7 +328,7 @@ def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log
     t = _teacher(lead, device, teacher_values, teacher_tokens, teacher_log_norm, temperature)
     pointer, step = _weights(row_weights, lead, device)
     if grad_out is None:
-        grad_out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+        grad_out = logits.new_empty(logits.shape)
         grad_stride = logits.shape[-1]
     else:
         _is_tensor(grad_out, "grad_out")
@@ -337,7 +337,7 @@ def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log
         if grad_out.dtype is not logits.dtype or grad_out.shape != logits.shape:
             raise _invalid("grad_out must have the logits' type and shape")
         grad_stride = _rows(grad_out, "grad_out")[0].row_stride
-    loss = torch.empty(lead, dtype=torch.float32, device=device)
+    loss = logits.new_empty(lead, dtype=torch.float32)
     o = _lib.DistillOut(loss.data_ptr(), grad_out.data_ptr(), grad_stride, pointer, step)
     _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
     return loss, grad_out
