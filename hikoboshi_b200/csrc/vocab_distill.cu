@@ -456,125 +456,156 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
   }
 }
 
+// f(value, token) over the entries of row r, in order; rows of 32-bit values in
+// multiples of four entries are read 16 bytes at a time.
+template <typename F>
+__device__ __forceinline__ void for_each_entry(const DistillArgs& a, int64_t r, F f) {
+  const int64_t at = r * a.k;
+  if (a.teacher_dtype == HKB_F32 && (a.k & 3) == 0 &&
+      ((reinterpret_cast<uintptr_t>(a.values) | reinterpret_cast<uintptr_t>(a.tokens)) & 15) == 0) {
+    const float4* v = reinterpret_cast<const float4*>(static_cast<const float*>(a.values) + at);
+    const int4* t = reinterpret_cast<const int4*>(a.tokens + at);
+    for (int k = 0; k < a.k / 4; ++k) {
+      const float4 x = v[k];
+      const int4 y = t[k];
+      f(x.x, y.x);
+      f(x.y, y.y);
+      f(x.z, y.z);
+      f(x.w, y.w);
+    }
+  } else {
+    for (int k = 0; k < a.k; ++k)
+      f(load_value(a.values, a.teacher_dtype, at + k), a.tokens[at + k]);
+  }
+}
+
 // Short rows, one thread each.  The masses of a row's tokens are added up in
-// shared memory, so a token listed twice needs no special case; the gradient
-// replaces the row's copy and leaves coalesced.
-template <typename T>
+// shared memory, so a token listed twice needs no special case; the weights
+// stay in registers between the sum and the gradient, which replaces the row's
+// copy and leaves as the row came.
+template <typename T, int kPad>
 __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logits,
                                                                    int64_t row_stride,
                                                                    int64_t n_rows, int vocab,
                                                                    DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  double* qs = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
-  float* xs = reinterpret_cast<float*>(smem_raw + sizeof(double) * kShortRows * vocab);
-  const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
+  __shared__ Exp2Table table;
+  const int tid = threadIdx.x;
+  float* qs = reinterpret_cast<float*>(smem_raw + ShortRows<T>::bytes(vocab)) + tid;
+  const int64_t r0 = (int64_t)blockIdx.x * kShortRows, r = r0 + tid;
   const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
-  load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, false);
-  __syncthreads();
-  if ((int)threadIdx.x < rows) {
-    const int64_t r = r0 + threadIdx.x;
-    float* x = xs + threadIdx.x;  // [i * kShortPitch]
-    const bool tail = a.log_norm != nullptr;
-    const double inv_tau = 1.0 / (double)a.temperature;
-    unsigned listed = 0;
-    bool bad = false;
-    float amax = -CUDART_INF_F;
-    for (int i = 0; i < vocab; ++i) qs[i * kShortRows] = 0.0;
-    for (int k = 0; k < a.k; ++k) {
-      const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
-      const int token = a.tokens[r * a.k + k];
-      if (token < 0 || v == -CUDART_INF_F) continue;
-      if (token >= vocab) {
-        bad = true;
-        continue;
-      }
-      listed |= 1u << token;
+  ShortRows<T> sr;
+  sr.load(reinterpret_cast<T*>(smem_raw), logits + r0 * row_stride, row_stride, rows, vocab);
+  table.fill();
+  const bool tail = a.log_norm != nullptr;
+  const double inv_tau = 1.0 / (double)a.temperature;
+  unsigned listed = 0;
+  bool bad = false;
+  float amax = -CUDART_INF_F;
+  if (tid < rows)
+    for_each_entry(a, r, [&](float v, int token) {
+      if (token < 0 || v == -CUDART_INF_F) return;
+      bad |= token >= vocab;
+      listed |= token < vocab ? 1u << token : 0u;
       amax = fmaxf(amax, v);
-    }
+    });
+  cp_async_wait_all();
+  __syncthreads();
+  if (tid < rows) {
+    auto value = [&](int i) { return widen(sr.at(tid, i)); };
     const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
     if (bad || listed == 0) {
       const float v = bad ? CUDART_NAN_F : 0.0f;
       if (a.loss) a.loss[r] = v;
       if (a.grad)
-        for (int i = 0; i < vocab; ++i) x[i * kShortPitch] = weight == 0.0f ? 0.0f : v;
+        for (int i = 0; i < vocab; ++i) sr.at(tid, i) = narrow<T>(weight == 0.0f ? 0.0f : v);
     } else {
-      double norm;
-      if (tail) {
-        norm = (double)a.log_norm[r];
-      } else {
-        double e = 0.0;
-        for (int k = 0; k < a.k; ++k) {
-          const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
-          if (a.tokens[r * a.k + k] >= 0 && v != -CUDART_INF_F)
-            e += exp(((double)v - (double)amax) * inv_tau);
-        }
-        norm = log(e);
-      }
-      double q_sum = 0.0, dot = 0.0;
-      for (int k = 0; k < a.k; ++k) {
-        const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
-        const int token = a.tokens[r * a.k + k];
-        if (token < 0 || v == -CUDART_INF_F) continue;
-        const double log_q = ((double)v - (tail ? 0.0 : (double)amax)) * inv_tau - norm;
-        const double q = exp(log_q);
-        q_sum += q;
-        if (q != 0.0) dot += q * log_q;
-        qs[token * kShortRows] += q;
-      }
-      // the body is the whole row, or its unlisted tokens; the rest of the
-      // row is added in 64 bits relative to the same largest logit
-      const unsigned body_mask = tail ? ~listed : ~0u;
+      // the body is the whole row, or its unlisted tokens
+      const unsigned body = tail ? ~listed : ~0u;
       float bmax = -CUDART_INF_F, lmax = -CUDART_INF_F;
-      for (int i = 0; i < vocab; ++i) {
-        const float v = x[i * kShortPitch];
-        if (body_mask >> i & 1u) bmax = fmaxf(bmax, v);
-        else lmax = fmaxf(lmax, v);
-      }
+#pragma unroll
+      for (int i = 0; i < kPad; ++i)
+        if (i < vocab) {
+          const float v = value(i);
+          if (body >> i & 1u) bmax = fmaxf(bmax, v);
+          else lmax = fmaxf(lmax, v);
+          qs[i * kShortPitch] = 0.0f;
+        }
       const float xmax = fmaxf(bmax, lmax);
+      // masses exp(a / tau - norm), or relative to the largest until their sum
+      // is known, and sum q (log q - (x - xmax) / tau)
+      const double norm = tail ? (double)a.log_norm[r] : 0.0, from = tail ? 0.0 : (double)amax;
+      double q_sum = 0.0, dot = 0.0;
+      for_each_entry(a, r, [&](float v, int token) {
+        if (token < 0 || v == -CUDART_INF_F) return;
+        const double log_q = ((double)v - from) * inv_tau - norm;
+        const double t = log_q * kLog2e;
+        const double q = t <= 0.0 ? table(t) : exp2(t);
+        q_sum += q;
+        // a mass that underflows counts nothing, also on a masked token
+        if (q != 0.0) dot += q * (log_q - ((double)value(token) - (double)xmax) * inv_tau);
+        qs[token * kShortPitch] += (float)q;
+      });
+      double q_scale = 1.0;
+      if (!tail) {
+        q_scale = 1.0 / q_sum;
+        dot = dot * q_scale - log(q_sum);
+        q_sum *= q_scale;
+      }
       const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
       const float c = (float)(kLog2e * inv_tau);
-      float s = 0.0f;
-      double rest = 0.0;
-      for (int i = 0; i < vocab; ++i) {
-        const float v = x[i * kShortPitch];
-        const double q = qs[i * kShortRows];
-        // a mass that underflows counts nothing, also on a masked token
-        if (q != 0.0) dot -= q * (((double)v - (double)xmax) * inv_tau);
-        if (body_mask >> i & 1u) s += exp2_fast((v - base) * c);
-        else rest += exp(((double)v - (double)xmax) * inv_tau);
-      }
-      const RowFactors f = row_factors(tail, bmax, (double)s, lmax, rest, q_sum, dot, inv_tau,
-                                       a.temperature, weight, a.loss ? a.loss + r : nullptr);
-      if (a.grad) {
-        for (int i = 0; i < vocab; ++i) {
-          const float v = x[i * kShortPitch];
-          float g;
-          if (weight == 0.0f) g = 0.0f;
-          else if (listed >> i & 1u)
-            g = (float)(f.P * exp(((double)v - f.shift) * inv_tau) - f.Q * qs[i * kShortRows]);
-          else g = exp2_fast((v - base) * c) * f.G;
-          x[i * kShortPitch] = g;
+      float e[kPad], sum = 0.0f, rest = 0.0f;  // of the body and, relative to xmax, of the list
+#pragma unroll
+      for (int i = 0; i < kPad; ++i) {
+        e[i] = 0.0f;
+        if (i < vocab) {
+          const bool in_body = body >> i & 1u;
+          e[i] = exp2_fast((value(i) - (in_body ? base : xmax)) * c);
+          if (in_body) sum += e[i];
+          else rest += e[i];
         }
+      }
+      const float lift = bmax == -CUDART_INF_F ? 0.0f
+                         : bmax == xmax        ? 1.0f
+                                               : exp2_fast((bmax - xmax) * c);
+      const double total = fma((double)sum, (double)lift, (double)rest);
+      double rest_q = 0.0;
+      if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
+      const double mass = q_sum + rest_q;
+      const double share = rest_q > 0.0 ? rest_q / (double)sum : 0.0;
+      if (a.loss) {
+        double l = dot + mass * log(total);
+        if (rest_q > 0.0) l += rest_q * (log(share) - ((double)bmax - (double)xmax) * inv_tau);
+        a.loss[r] = (float)((double)a.temperature * (double)a.temperature * l);
+      }
+      if (a.grad) {
+        const double wt = (double)weight * (double)a.temperature;
+        const double each = mass / total;
+        // gradient: e G off the list, e P - q Q on it (the body's e G where
+        // listed tokens are part of the body: lift is 1 then)
+        const float G = (float)(wt * (each * (double)lift - share));
+        const float P = (float)(wt * each), Q = (float)(wt * q_scale);
+#pragma unroll
+        for (int i = 0; i < kPad; ++i)
+          if (i < vocab) {
+            const float y = listed >> i & 1u ? e[i] * P - qs[i * kShortPitch] * Q : e[i] * G;
+            sr.at(tid, i) = narrow<T>(weight == 0.0f ? 0.0f : y);
+          }
       }
     }
   }
   if (a.grad == nullptr) return;
   __syncthreads();
-  T* grad = static_cast<T*>(a.grad) + r0 * a.grad_row_stride;
-  for_each_short(rows, vocab, [&](int row, int col, int) {
-    grad[row * a.grad_row_stride + col] = narrow<T>(xs[col * kShortPitch + row]);
-  });
+  sr.store(static_cast<T*>(a.grad) + r0 * a.grad_row_stride, a.grad_row_stride);
 }
 
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   if (v.vocab <= kShortVocab) {
-    const int smem = v.vocab * (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch);
-    ensure_dynamic_smem((const void*)distill_short_kernel<T>, kShortVocab *
-                        (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch));
+    const int smem = ShortRows<T>::bytes(v.vocab) + (int)sizeof(float) * kShortPitch * v.vocab;
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
-    distill_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
-        static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    HKB_SHORT_WIDTH(v.vocab, (distill_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
+                                 static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a)));
     return cudaGetLastError();
   }
   if (v.rows >= kStreamRows) {

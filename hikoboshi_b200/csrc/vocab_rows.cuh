@@ -568,10 +568,13 @@ inline int stream_threads(int vocab, int elem_bytes) {
   return t;
 }
 
-// Short rows (at most kShortVocab tokens): a thread owns a row, a CTA kShortRows
-// of them.  The rows are staged through shared memory token by token, element
-// (row, i) at [i * kShortPitch + row], so that global accesses are coalesced
-// and a thread walking its row meets no bank conflict.
+// ---- short rows -------------------------------------------------------------
+//
+// Rows of at most kShortVocab tokens: a thread owns a row, a CTA kShortRows of
+// them, staged through shared memory.  Rows that lie one after another are
+// copied as they are, in 16-byte pieces; with an odd number of tokens the
+// threads' walks over their rows then meet (almost) no bank conflict.  Other
+// rows are staged token by token, element (row, i) at [i * kShortPitch + row].
 constexpr int kShortVocab = 32;
 constexpr int kShortRows = 128;
 constexpr int kShortPitch = kShortRows + 1;
@@ -595,15 +598,128 @@ __device__ __forceinline__ void for_each_short(int rows, int width, F f) {
   }
 }
 
-// Stages the CTA's rows; with `clean` a NaN becomes -inf.
 template <typename T>
-__device__ __forceinline__ void load_short(float* x, const T* g, int64_t row_stride, int rows,
-                                           int vocab, bool clean) {
-  for_each_short(rows, vocab, [&](int row, int col, int) {
-    const float v = widen(g[row * row_stride + col]);
-    x[col * kShortPitch + row] = clean && v != v ? -CUDART_INF_F : v;
-  });
+struct ShortRows {
+  T* s;
+  int rows, vocab;
+  int row_step, col_step;
+
+  __host__ __device__ static constexpr int bytes(int vocab) {
+    return (vocab * kShortPitch * (int)sizeof(T) + 15) / 16 * 16;
+  }
+  __device__ __forceinline__ static bool dense(const T* g, int64_t row_stride, int vocab) {
+    return row_stride == vocab && (vocab & 1) && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  }
+  // Starts the copy of the CTA's rows; the caller waits with cp_async_wait_all
+  // and a barrier.
+  __device__ __forceinline__ void load(T* smem, const T* g, int64_t row_stride, int n, int v) {
+    s = smem;
+    rows = n;
+    vocab = v;
+    if (dense(g, row_stride, v)) {
+      row_step = v;
+      col_step = 1;
+      const int bytes = n * v * (int)sizeof(T);
+      const char* from = reinterpret_cast<const char*>(g);
+      char* to = reinterpret_cast<char*>(s);
+      for (int b = 16 * (int)threadIdx.x; b + 16 <= bytes; b += 16 * kShortRows)
+        cp_async16(to + b, from + b, true);
+      const int whole = bytes / 16 * 16 / (int)sizeof(T);
+      if (whole + (int)threadIdx.x < n * v) s[whole + threadIdx.x] = g[whole + threadIdx.x];
+    } else {
+      row_step = 1;
+      col_step = kShortPitch;
+      for_each_short(n, v, [&](int row, int col, int) {
+        s[col * kShortPitch + row] = g[row * row_stride + col];
+      });
+    }
+    cp_async_commit();
+  }
+  __device__ __forceinline__ T& at(int row, int i) const { return s[row * row_step + i * col_step]; }
+  // Writes the rows out of shared memory.
+  __device__ __forceinline__ void store(T* g, int64_t row_stride) const {
+    if (col_step == 1 && dense(g, row_stride, vocab)) {
+      const int bytes = rows * vocab * (int)sizeof(T);
+      for (int b = 16 * (int)threadIdx.x; b + 16 <= bytes; b += 16 * kShortRows)
+        __stcs(reinterpret_cast<uint4*>(reinterpret_cast<char*>(g) + b),
+               *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(s) + b));
+      const int whole = bytes / 16 * 16 / (int)sizeof(T);
+      if (whole + (int)threadIdx.x < rows * vocab) g[whole + threadIdx.x] = s[whole + threadIdx.x];
+    } else {
+      for_each_short(rows, vocab,
+                     [&](int row, int col, int) { g[row * row_stride + col] = at(row, col); });
+    }
+  }
+};
+
+// The comparators of the network's stage (P, K) and of the stages after it.
+template <int kPad, int P, int K>
+__device__ __forceinline__ void merge_stages(uint32_t (&key)[kPad]) {
+#pragma unroll
+  for (int j = K % P; j + K < kPad; j += 2 * K)
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+      if (i + j + K < kPad && (i + j) / (2 * P) == (i + j + K) / (2 * P)) {
+        const uint32_t a = key[i + j], b = key[i + j + K];
+        key[i + j] = ::max(a, b);
+        key[i + j + K] = ::min(a, b);
+      }
+  if constexpr (K > 1) merge_stages<kPad, P, K / 2>(key);
+  else if constexpr (2 * P < kPad) merge_stages<kPad, 2 * P, 2 * P>(key);
 }
+
+// The order of a short row in registers: key[j] holds, in its lower 5 bits, 31
+// minus the index of the j-th token of the order (value down, index up), 0 past
+// the tokens above -inf.  The values' keys lose their lower 5 bits to the index,
+// so the network (odd-even merge sort, K. E. Batcher 1968; two instructions a
+// comparator) may leave values that agree in 27 bits in the wrong order: such
+// neighbours are compared in full and swapped.  16-bit logits have no lower
+// bits to lose.
+template <int kPad, typename F>
+__device__ __forceinline__ void sort_short(uint32_t (&key)[kPad], int vocab, bool exact, F value) {
+#pragma unroll
+  for (int i = 0; i < kPad; ++i) {
+    const float x = i < vocab ? value(i) : -CUDART_INF_F;
+    key[i] = x > -CUDART_INF_F ? (order_key(x) & ~31u) | (31 - i) : 0u;
+  }
+  merge_stages<kPad, 1, 1>(key);
+  if (exact) return;
+  bool close = false;
+#pragma unroll
+  for (int j = 0; j + 1 < kPad; ++j) close |= (key[j] ^ key[j + 1]) < 32u && key[j + 1] != 0;
+  while (close) {
+    close = false;
+#pragma unroll
+    for (int j = 0; j + 1 < kPad; ++j) {
+      if ((key[j] ^ key[j + 1]) >= 32u || key[j + 1] == 0) continue;
+      const float a = value(31 - (int)(key[j] & 31)), b = value(31 - (int)(key[j + 1] & 31));
+      if (b > a || (b == a && (key[j + 1] & 31) > (key[j] & 31))) {
+        const uint32_t k = key[j];
+        key[j] = key[j + 1];
+        key[j + 1] = k;
+        close = true;
+      }
+    }
+  }
+}
+
+// kernel<kPad> for the smallest of the compiled widths that holds `vocab`.
+#define HKB_SHORT_WIDTH(vocab, ...)       \
+  do {                                    \
+    if ((vocab) <= 8) {                   \
+      constexpr int kPad = 8;             \
+      __VA_ARGS__;                        \
+    } else if ((vocab) <= 16) {           \
+      constexpr int kPad = 16;            \
+      __VA_ARGS__;                        \
+    } else if ((vocab) <= 24) {           \
+      constexpr int kPad = 24;            \
+      __VA_ARGS__;                        \
+    } else {                              \
+      constexpr int kPad = 32;            \
+      __VA_ARGS__;                        \
+    }                                     \
+  } while (0)
 
 }  // namespace vocab
 }  // namespace hkb

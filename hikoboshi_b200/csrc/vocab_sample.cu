@@ -49,10 +49,29 @@ namespace {
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr double kLn2 = 0.69314718055994530942;
 
-__device__ __forceinline__ bool settings_valid(float T, int top_k, float top_p, float min_p,
-                                               double u) {
-  return T >= 0.0f && T < CUDART_INF_F && top_k >= 0 && top_p >= 0.0f && top_p <= 1.0f &&
-         min_p >= 0.0f && min_p <= 1.0f && u >= 0.0 && u <= 1.0;
+// Settings of one row.
+struct RowSettings {
+  float temperature;
+  int top_k;
+  float top_p, min_p;
+  double u;
+};
+
+__device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, int64_t r) {
+  RowSettings s;
+  s.temperature = a.temperatures ? a.temperatures[r] : a.temperature;
+  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
+  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
+  s.min_p = a.min_ps ? a.min_ps[r] : a.min_p;
+  s.u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
+                       : (double)static_cast<const float*>(a.uniforms)[r];
+  return s;
+}
+
+__device__ __forceinline__ bool settings_valid(const RowSettings& s) {
+  return s.temperature >= 0.0f && s.temperature < CUDART_INF_F && s.top_k >= 0 &&
+         s.top_p >= 0.0f && s.top_p <= 1.0f && s.min_p >= 0.0f && s.min_p <= 1.0f &&
+         s.u >= 0.0 && s.u <= 1.0;
 }
 
 constexpr int kBins = 1024;
@@ -205,14 +224,6 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
   }
   return __shfl_sync(0xffffffffu, token, at);
 }
-
-// Settings of one row.
-struct RowSettings {
-  float temperature;
-  int top_k;
-  float top_p, min_p;
-  double u;
-};
 
 // Weights of a row: exponents relative to the largest logit.
 struct Weights {
@@ -413,14 +424,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   row.init(reinterpret_cast<T*>(smem_raw), g, vocab, chunk);
   row.load(g);
 
-  RowSettings s;
-  s.temperature = a.temperatures ? a.temperatures[r] : a.temperature;
-  s.top_k = a.top_ks ? a.top_ks[r] : a.top_k;
-  s.top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  s.min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-  s.u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
-                       : (double)static_cast<const float*>(a.uniforms)[r];
-  const bool valid = settings_valid(s.temperature, s.top_k, s.top_p, s.min_p, s.u);
+  RowSettings s = row_settings(a, r);
+  const bool valid = settings_valid(s);
   const bool writer = threadIdx.x == 0 && row.rank == 0;
   for (int b = threadIdx.x; b < kBins; b += blockDim.x) sm.hist[b] = 0;
   sm.table.fill();
@@ -684,125 +689,146 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   }
 }
 
-// Short rows, one thread each: 64-bit weights in shared memory; the head is
-// found by taking the largest remaining token until a filter stops it, which
-// ends early on the peaked rows that filters are for.
-template <typename T>
+// Short rows, one thread each.  The head is found with 32-bit weights, whose
+// sums are off by less than 2e-6 of the mass (2 ulp of the function, three
+// roundings of an exponent, 31 of the sum); a row where a comparison with a
+// border is closer than twice that repeats it with 64-bit weights.  The kept
+// tokens' mass and the draw are in 64 bits, so their number sets the time on
+// the 64-bit pipe, not V.
+template <typename T, int kPad>
 __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __restrict__ logits,
                                                                   int64_t row_stride, int64_t n_rows,
                                                                   int vocab, SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ Exp2Table table;
-  double* w = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
-  float* xs = reinterpret_cast<float*>(smem_raw + sizeof(double) * kShortRows * vocab);
-  const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
-  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
+  double* weight = reinterpret_cast<double*>(smem_raw) + threadIdx.x;  // [i * kShortRows]
+  const int64_t r0 = (int64_t)blockIdx.x * kShortRows, r = r0 + threadIdx.x;
+  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0), tid = threadIdx.x;
+  ShortRows<T> sr;
+  sr.load(reinterpret_cast<T*>(smem_raw + sizeof(double) * kShortRows * vocab),
+          logits + r0 * row_stride, row_stride, rows, vocab);
   table.fill();
-  load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, true);
+  RowSettings s{};
+  if (tid < rows) s = row_settings(a, r);
+  cp_async_wait_all();
   __syncthreads();
-  if ((int)threadIdx.x >= rows) return;
-  const int64_t r = r0 + threadIdx.x;
-  const float* x = xs + threadIdx.x;  // [i * kShortPitch]
-  const float Tf = a.temperatures ? a.temperatures[r] : a.temperature;
-  const int topk = a.top_ks ? a.top_ks[r] : a.top_k;
-  const float top_p = a.top_ps ? a.top_ps[r] : a.top_p;
-  const float min_p = a.min_ps ? a.min_ps[r] : a.min_p;
-  const double u = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[r]
-                                  : (double)static_cast<const float*>(a.uniforms)[r];
-  if (!settings_valid(Tf, topk, top_p, min_p, u)) {
+  if (tid >= rows) return;
+  if (!settings_valid(s)) {
     a.tokens[r] = -1;
     a.log_probs[r] = CUDART_NAN_F;
     a.kept[r] = 0;
     return;
   }
+  auto value = [&](int i) { return widen(sr.at(tid, i)); };
   float xmax = -CUDART_INF_F;
-  int best = -1, live = 0;
-  for (int i = 0; i < vocab; ++i) {
-    const float v = x[i * kShortPitch];
-    if (v > xmax) {
-      xmax = v;
-      best = i;
+  int best = -1;
+  unsigned live = 0;  // tokens above -inf
+#pragma unroll
+  for (int i = 0; i < kPad; ++i)
+    if (i < vocab) {
+      const float v = value(i);
+      if (v > xmax) {
+        xmax = v;
+        best = i;
+      }
+      live |= (v > -CUDART_INF_F ? 1u : 0u) << i;
     }
-    live += v > -CUDART_INF_F;
-  }
-  if (best < 0 || Tf == 0.0f) {
+  if (best < 0 || s.temperature == 0.0f) {
     a.tokens[r] = best;
     a.log_probs[r] = best < 0 ? -CUDART_INF_F : 0.0f;
     a.kept[r] = best < 0 ? 0 : 1;
     return;
   }
-  const double c2 = kLog2e / (double)Tf;
-  double sum = 0.0;
-  for (int i = 0; i < vocab; ++i) {
-    const float v = x[i * kShortPitch];
-    const double wi = table(v == xmax ? 0.0 : ((double)v - (double)xmax) * c2);
-    w[i * kShortRows] = wi;
-    sum += wi;
-  }
-  unsigned keep = 0;  // the kept tokens
-  const bool cut_k = topk > 0 && topk < live;
-  if (cut_k || top_p < 1.0f) {
-    // takes tokens in the head's order while `more` says so; their mass goes to `sum`
-    auto head = [&](auto more) {
-      unsigned taken = 0;
-      int n = 0;
-      double mass = 0.0;
-      while (n < live && more(n, mass)) {
-        float top = -CUDART_INF_F;
-        int at = 0;
-        for (int i = 0; i < vocab; ++i) {
-          const float v = x[i * kShortPitch];
-          if (v > top && !(taken >> i & 1u)) {
-            top = v;
-            at = i;
-          }
-        }
-        taken |= 1u << at;
-        mass += w[at * kShortRows];
-        ++n;
-      }
-      sum = mass;
-      return taken;
+  const double c2 = kLog2e / (double)s.temperature;
+  auto exponent = [&](float x) { return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2; };
+  unsigned keep = live;
+  const bool cut_k = s.top_k > 0 && s.top_k < __popc(live);
+  if (cut_k || s.top_p < 1.0f) {
+    uint32_t key[kPad];
+    sort_short(key, vocab, sizeof(T) == 2, value);
+    const int nk = cut_k ? s.top_k : __popc(live);
+    const float c = (float)c2;
+    auto light = [&](int i) {
+      const float x = value(i);
+      return exp2_fast((x == xmax ? 0.0f : x - xmax) * c);
     };
-    if (cut_k) keep = head([&](int n, double) { return n < topk; });
-    if (top_p < 1.0f) {
-      const double need = (double)top_p * sum;
-      keep = head([&](int n, double mass) {
-        return n == 0 || (mass < need && !(cut_k && n >= topk));
-      });
+    float sum = 0.0f;
+    keep = 0;
+#pragma unroll
+    for (int j = 0; j < kPad; ++j)
+      if (j < nk) {
+        const int i = 31 - (int)(key[j] & 31);
+        keep |= 1u << i;
+        if (s.top_p < 1.0f) sum += light(i);
+      }
+    if (s.top_p < 1.0f) {
+      const float need = s.top_p * sum, slack = 4e-6f * sum;
+      unsigned head = 0;
+      float run = 0.0f;
+      bool close = s.temperature > 1e30f;  // 32-bit differences of logits may overflow
+#pragma unroll
+      for (int j = 0; j < kPad; ++j)
+        if (j < nk && (j == 0 || run < need)) {
+          const int i = 31 - (int)(key[j] & 31);
+          head |= 1u << i;
+          run += light(i);
+          close |= fabsf(run - need) < slack;
+        }
+      if (close) {
+        // in 64 bits, over the order in shared memory
+        signed char* order = reinterpret_cast<signed char*>(weight);
+        double mass = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPad; ++j)
+          if (j < vocab) order[j / 8 * kShortRows * 8 + j % 8] = (signed char)(31 - (key[j] & 31));
+        for (int j = 0; j < nk; ++j)
+          mass += table(exponent(value(order[j / 8 * kShortRows * 8 + j % 8])));
+        const double border = (double)s.top_p * mass;
+        double upto = 0.0;
+        head = 0;
+        for (int j = 0; j < nk && (j == 0 || upto < border); ++j) {
+          const int i = order[j / 8 * kShortRows * 8 + j % 8];
+          head |= 1u << i;
+          upto += table(exponent(value(i)));
+        }
+      }
+      keep = head;
     }
-  } else {
-    for (int i = 0; i < vocab; ++i)
-      if (x[i * kShortPitch] > -CUDART_INF_F) keep |= 1u << i;
   }
+  // the kept tokens' mass in index order; with min-p, of those heavy enough
   double total = 0.0;
-  for (int i = 0; i < vocab; ++i) {
-    const double wi = w[i * kShortRows];
-    if (wi < (double)min_p) keep &= ~(1u << i);
-    if (keep >> i & 1u) total += wi;
+  for (unsigned m = keep; m != 0; m &= m - 1) {
+    const int i = __ffs(m) - 1;
+    const double w = table(exponent(value(i)));
+    weight[i * kShortRows] = w;
+    if (w >= (double)s.min_p) total += w;
+    else keep &= ~(1u << i);
   }
-  const double target = u * total;
+  const double target = s.u * total;
   double run = 0.0;
   int token = best;
-  for (int i = 0; i < vocab && !(run > target); ++i) {
-    const double wi = keep >> i & 1u ? w[i * kShortRows] : 0.0;
-    run += wi;
-    if (wi > 0.0) token = i;
+  for (unsigned m = keep; m != 0 && !(run > target); m &= m - 1) {
+    const int i = __ffs(m) - 1;
+    const double w = weight[i * kShortRows];
+    run += w;
+    if (w > 0.0) token = i;
   }
   a.tokens[r] = token;
-  a.log_probs[r] = (float)log(w[token * kShortRows] / total);
+  a.log_probs[r] = (float)(exponent(value(token)) * kLn2 - log(total));
   a.kept[r] = __popc(keep);
 }
 
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const SampleArgs& a) {
   if (v.vocab <= kShortVocab) {
-    const int smem = v.vocab * (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch);
-    ensure_dynamic_smem((const void*)sample_short_kernel<T>, kShortVocab *
-                        (int)(sizeof(double) * kShortRows + sizeof(float) * kShortPitch));
+    const int smem = ShortRows<T>::bytes(v.vocab) + (int)sizeof(double) * kShortRows * v.vocab;
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
-    sample_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
-        static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    HKB_SHORT_WIDTH(v.vocab, {
+      ensure_dynamic_smem((const void*)sample_short_kernel<T, kPad>,
+                          ShortRows<T>::bytes(kPad) + (int)sizeof(double) * kShortRows * kPad);
+      sample_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
+          static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    });
     return cudaGetLastError();
   }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));

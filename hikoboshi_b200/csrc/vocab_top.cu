@@ -274,48 +274,41 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
   }
 }
 
-// Short rows, one thread each: takes the largest remaining token k times.  The
-// row's listing replaces its logits' copy place by place and leaves coalesced.
-template <typename T>
+// Short rows, one thread each: sorts the row in registers.  The listing goes
+// through shared memory, so that it leaves coalesced.
+template <typename T, int kPad>
 __global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restrict__ logits,
                                                                int64_t row_stride, int64_t n_rows,
                                                                int vocab, TopArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* xs = reinterpret_cast<float*>(smem_raw);
-  signed char* places = reinterpret_cast<signed char*>(xs + vocab * kShortPitch);
+  signed char* places = reinterpret_cast<signed char*>(smem_raw + ShortRows<T>::bytes(vocab));
   const int64_t r0 = (int64_t)blockIdx.x * kShortRows;
-  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
-  load_short(xs, logits + r0 * row_stride, row_stride, rows, vocab, true);
+  const int rows = (int)::min((int64_t)kShortRows, n_rows - r0), tid = threadIdx.x;
+  ShortRows<T> sr;
+  sr.load(reinterpret_cast<T*>(smem_raw), logits + r0 * row_stride, row_stride, rows, vocab);
+  cp_async_wait_all();
   __syncthreads();
   const int listed = ::min(a.k, vocab);
-  if ((int)threadIdx.x < rows) {
-    const float* x = xs + threadIdx.x;
-    unsigned taken = 0;
-    float xmax = -CUDART_INF_F;
-    for (int j = 0; j < listed; ++j) {
-      float top = -CUDART_INF_F;
-      int at = -1;
-      for (int i = 0; i < vocab; ++i) {
-        const float v = x[i * kShortPitch];
-        if (v > top && !(taken >> i & 1u)) {
-          top = v;
-          at = i;
-        }
-      }
-      if (j == 0) xmax = top;
-      if (at >= 0) taken |= 1u << at;
-      places[j * kShortRows + threadIdx.x] = (signed char)at;
-    }
+  if (tid < rows) {
+    auto value = [&](int i) { return widen(sr.at(tid, i)); };
+    uint32_t key[kPad];
+    sort_short(key, vocab, sizeof(T) == 2, value);
+#pragma unroll
+    for (int j = 0; j < kPad; ++j)
+      if (j < listed) places[j * kShortRows + tid] = key[j] ? (signed char)(31 - (key[j] & 31)) : -1;
     if (a.log_norm) {
       const float c = kLog2ef / a.temperature;
+      const float xmax = key[0] ? value(31 - (int)(key[0] & 31)) : -CUDART_INF_F;
       float s = 0.0f;
-      for (int i = 0; i < vocab; ++i) {
-        const float v = x[i * kShortPitch];
-        s += exp2_fast((v == xmax ? 0.0f : v - xmax) * c);
-      }
-      a.log_norm[r0 + threadIdx.x] =
-          xmax == -CUDART_INF_F ? xmax
-                                : (float)((double)xmax / (double)a.temperature + log((double)s));
+#pragma unroll
+      for (int i = 0; i < kPad; ++i)
+        if (i < vocab) {
+          const float v = value(i);
+          if (v > -CUDART_INF_F) s += exp2_fast((v == xmax ? 0.0f : v - xmax) * c);
+        }
+      a.log_norm[r0 + tid] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
+                                 ? xmax
+                                 : (float)((double)xmax / (double)a.temperature + log((double)s));
     }
   }
   __syncthreads();
@@ -323,7 +316,7 @@ __global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restri
   int32_t* tokens = a.tokens + r0 * a.k;
   for_each_short(rows, a.k, [&](int row, int j, int i) {
     const int at = j < listed ? places[j * kShortRows + row] : -1;
-    values[i] = narrow<T>(at >= 0 ? xs[at * kShortPitch + row] : -CUDART_INF_F);
+    values[i] = at >= 0 ? sr.at(row, at) : narrow<T>(-CUDART_INF_F);
     tokens[i] = at;
   });
 }
@@ -331,10 +324,10 @@ __global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restri
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
   if (v.vocab <= kShortVocab) {
-    const int smem = v.vocab * (int)(sizeof(float) * kShortPitch + kShortRows);
+    const int smem = ShortRows<T>::bytes(v.vocab) + kShortRows * v.vocab;
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
-    top_short_kernel<T><<<blocks, kShortRows, smem, st>>>(
-        static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    HKB_SHORT_WIDTH(v.vocab, (top_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
+                                 static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a)));
     return cudaGetLastError();
   }
   if (v.rows >= kStreamRows) {
