@@ -568,6 +568,123 @@ inline int stream_threads(int vocab, int elem_bytes) {
   return t;
 }
 
+// ---- rows of a warp -----------------------------------------------------------
+//
+// Rows of at most kWarpVocab tokens: a warp owns a row, lane l its tokens
+// [l * kPer, (l + 1) * kPer) in registers, so that a lane's number orders
+// tokens and ballots find the first of them.  kPer is odd: the lanes' walks
+// over the staged row then start in different banks.
+constexpr int kWarpVocab = 31 * 32;
+constexpr int kWarpRows = 4;  // warps of a CTA
+
+template <typename T, int kPer>
+struct WarpRow {
+  static constexpr int kE = Vec<T>::kN;
+  const T* s;       // shared memory
+  int ph, vocab;
+  float x[kPer];    // -inf past the row and for a NaN
+
+  __host__ __device__ static constexpr int bytes(int vocab) { return (vocab / kE + 2) * 16; }
+  __device__ __forceinline__ void stage(T* smem, const T* g, int v) {
+    const int lane = threadIdx.x & 31;
+    vocab = v;
+    ph = (int)((reinterpret_cast<uintptr_t>(g) & 15) / sizeof(T));
+    s = smem;
+    const T* from = g - ph;
+    for (int e0 = lane * kE; e0 < ph + v; e0 += 32 * kE) {
+      if (e0 >= ph && e0 + kE <= ph + v) {
+        cp_async16(smem + e0, from + e0, true);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kE; ++e)
+          if (e0 + e >= ph && e0 + e < ph + v) smem[e0 + e] = from[e0 + e];
+      }
+    }
+    cp_async_commit();
+  }
+  // after cp_async_wait_all and a barrier
+  __device__ __forceinline__ void read() {
+    const int first = (threadIdx.x & 31) * kPer;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float v = first + e < vocab ? widen(s[ph + first + e]) : -CUDART_INF_F;
+      x[e] = v > -CUDART_INF_F ? v : -CUDART_INF_F;
+    }
+  }
+  __device__ __forceinline__ float largest() const {
+    float m = x[0];
+#pragma unroll
+    for (int e = 1; e < kPer; ++e) m = fmaxf(m, x[e]);
+    return key_value(__reduce_max_sync(0xffffffffu, order_key(m)));
+  }
+  // tokens of the row at or above `from`
+  __device__ __forceinline__ int count(float from) const {
+    int n = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) n += x[e] >= from;
+    return __reduce_add_sync(0xffffffffu, n);
+  }
+  // largest value that at least n tokens reach (n of the row's are above -inf)
+  __device__ __forceinline__ float nth_largest(int n, float xmax) const {
+    uint32_t lo = kKeyNegInf + 1, hi = order_key(xmax);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      if (count(key_value(mid)) >= n) lo = mid;
+      else hi = mid - 1;
+    }
+    return key_value(lo);
+  }
+  // this lane's part of `from`: its tokens above t and, of the row's first
+  // `ties` tokens of `from` that equal t, those that are its own
+  __device__ __forceinline__ unsigned head(unsigned from, float t, int ties) const {
+    const int lane = threadIdx.x & 31;
+    unsigned above = 0, equal = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      above |= (x[e] > t ? 1u : 0u) << e;
+      equal |= (x[e] == t ? 1u : 0u) << e;
+    }
+    above &= from;
+    equal &= from;
+    int before = __popc(equal);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    for (int left = ties - (before - __popc(equal)); left > 0 && equal != 0; --left) {
+      above |= equal & (0u - equal);
+      equal &= equal - 1;
+    }
+    return above;
+  }
+};
+
+template <typename V>
+__device__ __forceinline__ V warp_total(V v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// kernel<kPer> for the smallest of the compiled widths that holds `vocab`.
+#define HKB_WARP_WIDTH(vocab, ...)        \
+  do {                                    \
+    if ((vocab) <= 3 * 32) {              \
+      constexpr int kPer = 3;             \
+      __VA_ARGS__;                        \
+    } else if ((vocab) <= 7 * 32) {       \
+      constexpr int kPer = 7;             \
+      __VA_ARGS__;                        \
+    } else if ((vocab) <= 15 * 32) {      \
+      constexpr int kPer = 15;            \
+      __VA_ARGS__;                        \
+    } else {                              \
+      constexpr int kPer = 31;            \
+      __VA_ARGS__;                        \
+    }                                     \
+  } while (0)
+
 // ---- short rows -------------------------------------------------------------
 //
 // Rows of at most kShortVocab tokens: a thread owns a row, a CTA kShortRows of

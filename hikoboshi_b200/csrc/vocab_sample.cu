@@ -689,6 +689,175 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   }
 }
 
+// Rows of up to kWarpVocab tokens, a warp each.  As for the short rows below,
+// the head is found with 32-bit weights, by bisection of the logits' keys, and
+// again with 64-bit ones where a comparison with the border is too close (or
+// where equal logits share the border: their number needs the exact masses).
+template <typename T, int kPer>
+__global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
+    const T* __restrict__ logits, int64_t row_stride, int64_t n_rows, int vocab, SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ Exp2Table table;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kWarpRows + warp;
+  WarpRow<T, kPer> row;
+  RowSettings s{};
+  if (r < n_rows) {
+    row.stage(reinterpret_cast<T*>(smem_raw + warp * WarpRow<T, kPer>::bytes(vocab)),
+              logits + r * row_stride, vocab);
+    s = row_settings(a, r);
+  }
+  table.fill();
+  cp_async_wait_all();
+  __syncthreads();
+  if (r >= n_rows) return;
+  if (!settings_valid(s)) {
+    if (lane == 0) {
+      a.tokens[r] = -1;
+      a.log_probs[r] = CUDART_NAN_F;
+      a.kept[r] = 0;
+    }
+    return;
+  }
+  row.read();
+  const float xmax = row.largest();
+  if (xmax == -CUDART_INF_F || s.temperature == 0.0f) {
+    int first = -1;
+#pragma unroll
+    for (int e = kPer - 1; e >= 0; --e)
+      if (row.x[e] == xmax) first = lane * kPer + e;
+    const bool none = xmax == -CUDART_INF_F;
+    const unsigned has = __ballot_sync(0xffffffffu, first >= 0);
+    if (lane == (none ? 0 : __ffs(has) - 1)) {
+      a.tokens[r] = none ? -1 : first;
+      a.log_probs[r] = none ? -CUDART_INF_F : 0.0f;
+      a.kept[r] = none ? 0 : 1;
+    }
+    return;
+  }
+  const double c2 = kLog2e / (double)s.temperature;
+  auto exponent = [&](float x) { return x == xmax ? 0.0 : ((double)x - (double)xmax) * c2; };
+  unsigned keep = 0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e) keep |= (row.x[e] > -CUDART_INF_F ? 1u : 0u) << e;
+  if (s.top_k > 0 && s.top_k < (int)__reduce_add_sync(0xffffffffu, __popc(keep))) {
+    const float t = row.nth_largest(s.top_k, xmax);
+    int above = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) above += row.x[e] > t;
+    above = __reduce_add_sync(0xffffffffu, above);
+    keep = row.head(keep, t, s.top_k - above);
+  }
+  if (s.top_p < 1.0f) {
+    const float c = (float)c2;
+    float w[kPer], sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const float x = row.x[e];
+      w[e] = keep >> e & 1u ? exp2_fast((x == xmax ? 0.0f : x - xmax) * c) : 0.0f;
+      sum += w[e];
+    }
+    sum = warp_total(sum);
+    const float need = s.top_p * sum, slack = 4e-6f * sum;
+    uint32_t lo = kKeyNegInf + 1, hi = order_key(xmax);
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      const float from = key_value(mid);
+      float m = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) m += row.x[e] >= from ? w[e] : 0.0f;
+      if (warp_total(m) >= need) lo = mid;
+      else hi = mid - 1;
+    }
+    float t = key_value(lo), at = 0.0f, over = 0.0f;
+    int ties = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      at += row.x[e] >= t ? w[e] : 0.0f;
+      over += row.x[e] > t ? w[e] : 0.0f;
+      ties += row.x[e] == t && (keep >> e & 1u);
+    }
+    at = warp_total(at);
+    over = warp_total(over);
+    ties = __reduce_add_sync(0xffffffffu, ties);
+    // 32-bit differences of logits may overflow at the largest temperatures
+    const bool close =
+        !(at - need > slack && need - over > slack) || s.temperature > 1e30f;
+    if (close || ties > 1) {
+      auto mass = [&](auto in) {
+        double m = 0.0;
+#pragma unroll 1
+        for (unsigned b = keep; b != 0; b &= b - 1) {
+          const float x = widen(row.s[row.ph + lane * kPer + __ffs(b) - 1]);
+          if (in(x)) m += table(exponent(x));
+        }
+        return warp_total(m);
+      };
+      const double border = (double)s.top_p * mass([](float) { return true; });
+      if (close) {
+        lo = kKeyNegInf + 1;
+        hi = order_key(xmax);
+        while (lo < hi) {
+          const uint32_t mid = lo + (hi - lo + 1) / 2;
+          const float from = key_value(mid);
+          if (mass([from](float x) { return x >= from; }) >= border) lo = mid;
+          else hi = mid - 1;
+        }
+        t = key_value(lo);
+      }
+      const double above = mass([t](float x) { return x > t; });
+      const double each = table(exponent(t));
+      const double n = each > 0.0 ? ceil((border - above) / each) : 1.0;
+      ties = (int)fmin(fmax(n, 1.0), (double)vocab);
+    }
+    keep = row.head(keep, t, ties);
+  }
+  // the kept mass; with min-p, of those heavy enough
+  double mine = 0.0;
+#pragma unroll
+  for (int e = 0; e < kPer; ++e)
+    if (keep >> e & 1u) {
+      const double w = table(exponent(row.x[e]));
+      if (w >= (double)s.min_p) mine += w;
+      else keep &= ~(1u << e);
+    }
+  const int kept = __reduce_add_sync(0xffffffffu, __popc(keep));
+  double upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  const double total = __shfl_sync(0xffffffffu, upto, 31), target = s.u * total;
+  // the lane in which the running mass passes the target (rounding, or u = 1,
+  // may leave none: the last with any mass), then its token, a lane for each
+  const unsigned pass = __ballot_sync(0xffffffffu, mine > 0.0 && upto > target);
+  const unsigned any = __ballot_sync(0xffffffffu, mine > 0.0);
+  const int hit = pass ? __ffs(pass) - 1 : 31 - __clz(any);
+  const double before = __shfl_sync(0xffffffffu, upto - mine, hit);
+  const unsigned bits = __shfl_sync(0xffffffffu, keep, hit);
+  const int token = hit * kPer + lane;
+  float x = -CUDART_INF_F;
+  double w = 0.0;
+  if (lane < kPer && (bits >> lane & 1u)) {
+    x = widen(row.s[row.ph + token]);
+    w = table(exponent(x));
+  }
+  double run = w;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += y;
+  }
+  const unsigned over = __ballot_sync(0xffffffffu, w > 0.0 && before + run > target);
+  const unsigned some = __ballot_sync(0xffffffffu, w > 0.0);
+  if (lane == (over ? __ffs(over) - 1 : 31 - __clz(some))) {
+    a.tokens[r] = token;
+    a.log_probs[r] = (float)(exponent(x) * kLn2 - log(total));
+    a.kept[r] = kept;
+  }
+}
+
 // Short rows, one thread each.  The head is found with 32-bit weights, whose
 // sums are off by less than 2e-6 of the mass (2 ulp of the function, three
 // roundings of an exponent, 31 of the sum); a row where a comparison with a
@@ -829,6 +998,13 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const SampleArgs& a) {
       sample_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
           static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
     });
+    return cudaGetLastError();
+  }
+  if (v.vocab <= kWarpVocab) {
+    const int smem = kWarpRows * WarpRow<T, 1>::bytes(v.vocab);
+    const unsigned blocks = (unsigned)((v.rows + kWarpRows - 1) / kWarpRows);
+    HKB_WARP_WIDTH(v.vocab, (sample_warp_kernel<T, kPer><<<blocks, 32 * kWarpRows, smem, st>>>(
+                                static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a)));
     return cudaGetLastError();
   }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));

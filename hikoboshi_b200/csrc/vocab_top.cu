@@ -274,6 +274,115 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
   }
 }
 
+// Rows of up to kWarpVocab tokens, a warp each.  A short listing takes the
+// largest remaining token k times; a longer one finds the k-th largest by
+// bisection of keys and puts the k tokens in order in shared memory.
+constexpr int kTakeOneByOne = 16;
+
+template <typename T, int kPer>
+__global__ void __launch_bounds__(32 * kWarpRows) top_warp_kernel(const T* __restrict__ logits,
+                                                                  int64_t row_stride,
+                                                                  int64_t n_rows, int vocab,
+                                                                  int list_size, TopArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t r = (int64_t)blockIdx.x * kWarpRows + warp;
+  if (r >= n_rows) return;  // warps share nothing
+  const int row_bytes = WarpRow<T, kPer>::bytes(vocab);
+  WarpRow<T, kPer> row;
+  row.stage(reinterpret_cast<T*>(smem_raw + warp * row_bytes), logits + r * row_stride, vocab);
+  cp_async_wait_all();
+  __syncwarp();
+  row.read();
+  const float xmax = row.largest();
+  if (a.log_norm) {
+    const float c = kLog2ef / a.temperature;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      s += exp2_fast((row.x[e] == xmax ? 0.0f : row.x[e] - xmax) * c);
+    const double total = warp_total((double)s);
+    if (lane == 0)
+      a.log_norm[r] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
+                          ? xmax
+                          : (float)((double)xmax / (double)a.temperature + log(total));
+  }
+  T* values = static_cast<T*>(a.values) + r * a.k;
+  int32_t* tokens = a.tokens + r * a.k;
+  int n = 0;
+  if (a.k <= kTakeOneByOne) {
+    for (; n < a.k; ++n) {
+      float best = -CUDART_INF_F;
+      int at = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e)
+        if (row.x[e] > best) {
+          best = row.x[e];
+          at = e;
+        }
+      const uint32_t key = order_key(best), most = __reduce_max_sync(0xffffffffu, key);
+      if (most <= kKeyNegInf) break;
+      if (lane == __ffs(__ballot_sync(0xffffffffu, key == most)) - 1) {
+        const int index = lane * kPer + at;
+        values[n] = row.s[row.ph + index];
+        tokens[n] = index;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e)
+          if (e == at) row.x[e] = -CUDART_INF_F;
+      }
+    }
+  } else {
+    unsigned keep = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) keep |= (row.x[e] > -CUDART_INF_F ? 1u : 0u) << e;
+    if ((int)__reduce_add_sync(0xffffffffu, __popc(keep)) > a.k) {
+      const float t = row.nth_largest(a.k, xmax);
+      int above = 0;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) above += row.x[e] > t;
+      keep = row.head(keep, t, a.k - (int)__reduce_add_sync(0xffffffffu, above));
+    }
+    int at = __popc(keep);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += y;
+    }
+    n = __shfl_sync(0xffffffffu, at, 31);
+    at -= __popc(keep);
+    unsigned long long* item =
+        reinterpret_cast<unsigned long long*>(smem_raw + kWarpRows * row_bytes) + warp * list_size;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e)
+      if (keep >> e & 1u) item[at++] = list_item(order_key(row.x[e]), lane * kPer + e);
+    int size = 32;
+    while (size < n) size <<= 1;  // list_size is a power of two of at least k
+    for (int i = n + lane; i < size; i += 32) item[i] = 0;
+    __syncwarp();
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        for (int p = lane; p < size / 2; p += 32) {
+          const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1)), l = i | j;
+          const unsigned long long u = item[i], w = item[l];
+          if ((u < w) == ((i & k) == 0)) {
+            item[i] = w;
+            item[l] = u;
+          }
+        }
+        __syncwarp();
+      }
+    for (int i = lane; i < n; i += 32) {
+      const int index = item_index(item[i]);
+      values[i] = row.s[row.ph + index];
+      tokens[i] = index;
+    }
+  }
+  for (int i = n + lane; i < a.k; i += 32) {
+    values[i] = narrow<T>(-CUDART_INF_F);
+    tokens[i] = -1;
+  }
+}
+
 // Short rows, one thread each: sorts the row in registers.  The listing goes
 // through shared memory, so that it leaves coalesced.
 template <typename T, int kPad>
@@ -328,6 +437,18 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
     HKB_SHORT_WIDTH(v.vocab, (top_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
                                  static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a)));
+    return cudaGetLastError();
+  }
+  if (v.vocab <= kWarpVocab) {
+    // the kept items: at most k of them, and of the row
+    int list_size = 0;
+    if (a.k > kTakeOneByOne)
+      for (list_size = 32; list_size < a.k && list_size < v.vocab;) list_size *= 2;
+    const int smem = kWarpRows * (WarpRow<T, 1>::bytes(v.vocab) + list_size * 8);
+    const unsigned blocks = (unsigned)((v.rows + kWarpRows - 1) / kWarpRows);
+    HKB_WARP_WIDTH(v.vocab, (top_warp_kernel<T, kPer><<<blocks, 32 * kWarpRows, smem, st>>>(
+                                static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab,
+                                list_size, a)));
     return cudaGetLastError();
   }
   if (v.rows >= kStreamRows) {

@@ -653,3 +653,44 @@ def test_many_rows_at_any_offset_and_stride(vocab, size, dtype):
         check_distill(loss[at], grad[at], x[at], v[at], t[at], norm[at], 1.0)
         g.fill_(7.0)
         assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("size", [3, 8, 9, 21, 24, 25, 32, 60, 96, 97, 224, 225, 480, 481, 992, 993])
+def test_near_ties_and_near_borders(vocab, size):
+    # neighbours in the type: their order needs every bit, their sums borders
+    # that 32 bits cannot tell apart
+    rows = 200
+    g = gen(size)
+    step = torch.randint(0, 40, (rows, size), generator=g, device="cuda")
+    x = (torch.full((rows, size), 1.0, device="cuda").view(torch.int32) + step.int()).view(F32)
+    x[: rows // 2] = torch.where(step[: rows // 2] % 2 == 0, x[: rows // 2], -x[: rows // 2])
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    for k in (1, 5, 16, 17, 40, size):
+        check_top(vocab.top_logits(x, k), x, k)
+    for f in (dict(top_k=5), dict(top_p=0.5), dict(top_k=7, top_p=0.6), dict(top_p=0.9, min_p=0.9),
+              dict(top_k=max(1, size // 2))):
+        check_sample(vocab.sample_tokens(x, u, **f), x, u, **f)
+    # borders that lie exactly between two tokens, and a hair beside
+    flat = torch.zeros(3, size, device="cuda")
+    for n in {1, size // 2, size}:
+        for p in (n / size, np.nextafter(np.float32(n / size), np.float32(2)),
+                  np.nextafter(np.float32(n / size), np.float32(0))):
+            p = float(min(1.0, p))
+            v = torch.tensor([0.0, 0.5, 0.999], device="cuda")
+            got = vocab.sample_tokens(flat, v, top_p=p)
+            # p is a 32-bit number: the head is the least n with n / size >= p
+            want = size if p == 1.0 else max(1, int(np.ceil(np.float64(np.float32(p)) * size)))
+            assert (got.kept == want).all(), (size, p, got.kept, want)
+
+
+def test_extreme_temperatures(vocab):
+    for size in (21, 300, 5000, 70000):
+        x = logits(4, size, F32, 1)
+        x[1] *= 1e30
+        x[2] = torch.finfo(F32).min
+        x[2, 3] = torch.finfo(F32).max
+        x[3] *= 1e-38
+        u = torch.tensor([0.1, 0.5, 0.7, 0.9], device="cuda")
+        for t in (1e-45, 1e-38, 1e-20, 1e20, 1e30, 3e38):
+            for f in (dict(), dict(top_p=0.7), dict(top_k=5), dict(min_p=0.5), dict(top_p=0.3, top_k=9)):
+                check_sample(vocab.sample_tokens(x, u, temperature=t, **f), x, u, temperature=t, **f)
