@@ -37,55 +37,51 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
 }
 
 
-// What a row's loss and gradient need beside the row, from one thread.
+// What a row's loss and gradient need beside the row.
 struct RowFactors {
-  float base;    // of the body's exponents
-  float G;       // gradient of an unlisted token: exp2((x - base) c) * G
-  double shift;  // largest logit, of which p is formed on the list
-  double P;      // gradient on the list: P exp((x - shift) / tau) - Q q
-  double Q;
+  float base;     // of the body's exponents
+  float G;        // gradient of an unlisted token: exp2((x - base) c) * G
+  double P, Q;    // gradient on the list: P exp((x - xmax) / tau) - Q q
+  double total;   // of the row's weights, relative to its largest logit
+  double mass;    // the teacher's
+  double rest_q;  // of it, the unlisted tokens' where they are a class
 };
 
-// The body's largest logit and sum (relative to it), the listed tokens' largest
-// logit and, where the unlisted tokens are a class of their own, their sum
-// relative to the row's largest; q_sum the listed masses' sum (1, or NaN, without
-// the class) and dot = sum q (log q - (x - xmax) / tau).  Everything is relative
-// to the row's largest logit, so logits of any size leave the loss its digits.
-__device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double body, float lmax,
-                                                  double listed, double q_sum, double dot,
-                                                  double inv_tau, float temperature, float weight,
-                                                  float* loss) {
+// The body's largest logit and sum (relative to it), the row's largest logit
+// and, where the unlisted tokens are a class of their own (the body), the sum of
+// the listed ones relative to it; q_sum is the listed masses' sum: 1, or NaN,
+// without the class.
+__device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double body, float xmax,
+                                                  double listed, double q_sum, double inv_tau,
+                                                  float temperature, float weight) {
   RowFactors f;
-  const float xmax = fmaxf(bmax, lmax);
-  const double lift =
-      bmax == -CUDART_INF_F ? 0.0 : exp(((double)bmax - (double)xmax) * inv_tau);
-  const double total = body * lift + listed;  // relative to xmax
-  double rest_q = 0.0;
-  if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
-  const double mass = q_sum + rest_q;
-  if (loss) {
-    const double log_total = log(total);
-    double l = dot + q_sum * log_total;
-    if (rest_q > 0.0)
-      l += rest_q * (log(rest_q) - log(body) + log_total -
-                     ((double)bmax - (double)xmax) * inv_tau);
-    *loss = (float)((double)temperature * (double)temperature * l);
-  }
-  const double wt = (double)weight * (double)temperature;
-  double factor = mass * lift / total;
-  if (rest_q > 0.0) factor -= rest_q / body;
+  const double lift = bmax == xmax           ? 1.0
+                      : bmax == -CUDART_INF_F ? 0.0
+                                              : exp(((double)bmax - (double)xmax) * inv_tau);
+  f.total = body * lift + listed;
+  f.rest_q = tail && bmax != -CUDART_INF_F ? fmax(0.0, 1.0 - q_sum) : 0.0;
+  f.mass = q_sum + f.rest_q;
+  const double wt = (double)weight * (double)temperature, each = f.mass / f.total;
   f.base = bmax == -CUDART_INF_F ? 0.0f : bmax;
-  f.G = (float)(wt * factor);
-  f.shift = (double)xmax;
-  f.P = wt * mass / total;
+  f.G = (float)(wt * (each * lift - (f.rest_q > 0.0 ? f.rest_q / body : 0.0)));
+  f.P = wt * each;
   f.Q = wt;
   return f;
+}
+
+// dot = sum q (log q - (x - xmax) / tau).  Everything is relative to the row's
+// largest logit, so logits of any size leave the loss its digits.
+__device__ __forceinline__ float row_loss(const RowFactors& f, double dot, float bmax, float xmax,
+                                          double body, double inv_tau, float temperature) {
+  double l = dot + f.mass * log(f.total);
+  if (f.rest_q > 0.0)
+    l += f.rest_q * (log(f.rest_q / body) - ((double)bmax - (double)xmax) * inv_tau);
+  return (float)((double)temperature * (double)temperature * l);
 }
 
 struct DistillSmem {
   ReduceScratch cluster;
   ReduceScratch block;
-  RowFactors f;
 };
 
 // Listing of a row in shared memory, behind the slice's buffer.
@@ -235,16 +231,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   listed = sums.x;
   dot = sums.y;
   const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
-  if (threadIdx.x == 0)
-    sm.f = row_factors(tail, bmax, body, listed_max, listed, q_sum, dot, inv_tau,
-                       a.temperature, weight, writer && a.loss ? a.loss + r : nullptr);
+  const RowFactors f =
+      row_factors(tail, bmax, body, xmax, listed, q_sum, inv_tau, a.temperature, weight);
+  if (writer && a.loss) a.loss[r] = row_loss(f, dot, bmax, xmax, body, inv_tau, a.temperature);
   if (grad == nullptr) return;
   if (weight == 0.0f) {
     fill_slice(row, grad, 0.0f);
     return;
   }
-  __syncthreads();
-  const RowFactors f = sm.f;
   T* gs = grad + row.start - row.ph;  // element e0 of the slice's vectors goes to gs[e0]
   const bool same_phase = (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
   row.for_each([&](int i0, const Vec<T>& x) {
@@ -272,25 +266,64 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
       for (int j = 0; j < a.k; ++j)
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
-    const double e = exp(((double)ls.x[k] - f.shift) * inv_tau);
+    const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
     grad[ls.token[k]] = narrow<T>((float)(f.P * e - f.Q * q));
   }
 }
 
+
+// A row's sum and its largest listed logit.
+struct RowSum {
+  SoftSum soft;
+  float lmax;
+};
+
+// Sums over a row's entries: masses, q (log q - (x - xmax) / tau), and
+// exp((x - xmax) / tau) of the listed tokens where they are left out of the
+// row's sum; whether a token is listed twice rides along.
+struct EntrySums {
+  double q, dot, listed;
+  int twice;
+};
+
+}  // namespace
+
+template <>
+__device__ __forceinline__ RowSum shfl_xor(RowSum v, int o) {
+  v.soft = shfl_xor(v.soft, o);
+  v.lmax = __shfl_xor_sync(0xffffffffu, v.lmax, o);
+  return v;
+}
+template <>
+__device__ __forceinline__ EntrySums shfl_xor(EntrySums v, int o) {
+  EntrySums r;
+  r.q = __shfl_xor_sync(0xffffffffu, v.q, o);
+  r.dot = __shfl_xor_sync(0xffffffffu, v.dot, o);
+  r.listed = __shfl_xor_sync(0xffffffffu, v.listed, o);
+  r.twice = __shfl_xor_sync(0xffffffffu, v.twice, o);
+  return r;
+}
+
+namespace {
+
 struct StreamSmem {
   ReduceScratch red;
+  Exp2Table table;
   RowFactors f;
+  EntrySums sums;
 };
 
 // Many rows: a CTA streams a row for its sum, then again for the gradient.  The
 // listed tokens are marked in a bit map in the phase of the row's vectors, a
 // vector's marks in one byte or half a byte, so that the first pass leaves them
 // out where the unlisted ones form a class; the entry that sets a mark stands
-// for its token.
+// for its token.  The entries' own work comes between the two passes: the row
+// is on its way all the while, and a barrier costs as much as a tenth of a row.
 template <typename T>
 __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T* logits,
-                                                                        int64_t row_stride,
-                                                                        int vocab, DistillArgs a) {
+                                                                           int64_t row_stride,
+                                                                           int vocab,
+                                                                           DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ StreamSmem sm;
   constexpr int kE = Vec<T>::kN, kU = 4;
@@ -305,10 +338,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
   ls.own = ls.token + a.k;
   uint32_t* marks = reinterpret_cast<uint32_t*>(ls.own + a.k);
   Reducer<false> red(&sm.red);
+  sm.table.fill();
 
   const bool tail = a.log_norm != nullptr;
-  const double inv_tau = 1.0 / (double)a.temperature;
-  for (int w = tid; w < (row.end + 31) / 32; w += threads) marks[w] = 0;
+  T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
+  const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+  const bool marked = tail || grad != nullptr;
+  if (marked)
+    for (int w = tid; w < (row.end + 31) / 32; w += threads) marks[w] = 0;
   unsigned flags = 0;  // 1: an entry, 2: a token outside the vocabulary
   float amax = -CUDART_INF_F;
   for (int k = tid; k < a.k; k += threads) {
@@ -327,8 +364,6 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
               [](unsigned long long p, unsigned long long q) {
                 return (p > q ? p : q) | (p & 3) | (q & 3);
               });
-  T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
-  const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
   const bool row_bad = head & 2, row_any = head & 1;
   if (row_bad || !row_any) {
     const float v = row_bad ? CUDART_NAN_F : 0.0f;
@@ -338,46 +373,23 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
     return;
   }
   amax = key_value((uint32_t)(head >> 32));
-  // masses: exp(a / tau - norm), or relative to the largest until their sum is known
-  const double norm = tail ? (double)a.log_norm[r] : (double)amax * inv_tau;
-  double q_sum = 0.0, dot = 0.0;
-  float lmax = -CUDART_INF_F;
-  bool twice = false;
-  for (int k = tid; k < a.k; k += threads) {
-    const int token = ls.token[k];
-    double q = 0.0;
-    int own = 0;
-    if (token >= 0) {
-      const double log_q = tail ? (double)ls.x[k] * inv_tau - norm
-                                : ((double)ls.x[k] - (double)amax) * inv_tau;
-      q = exp(log_q);
-      const float x = widen(g[token]);
-      ls.x[k] = x;
-      lmax = fmaxf(lmax, x);
-      q_sum += q;
-      if (q != 0.0) dot += q * log_q;
+  EntrySums sums{0.0, 0.0, 0.0, 0};
+  if (marked) {
+    for (int k = tid; k < a.k; k += threads) {
+      const int token = ls.token[k];
+      if (token < 0) continue;
       const int bit = token + row.ph;
-      own = !(atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u);
-      twice |= !own;
+      const int own = !(atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u);
+      sums.twice |= !own;
+      ls.own[k] = own;
     }
-    ls.q[k] = q;
-    ls.own[k] = own;
-  }
-  const double2 masses = red.sum(make_double2(q_sum, dot));
-  q_sum = masses.x;
-  dot = masses.y;
-  const bool row_twice = __syncthreads_or(twice);
-  double q_scale = 1.0;
-  if (!tail) {
-    q_scale = 1.0 / q_sum;
-    dot = dot * q_scale - log(q_sum);
-    q_sum *= q_scale;
-    lmax = -CUDART_INF_F;
+    if (tail) __syncthreads();  // the marks are read
   }
 
+  const double inv_tau = 1.0 / (double)a.temperature;
   const float c = (float)(kLog2e * inv_tau);
   SoftSum soft;
-  row.template walk<kU>([&](auto& x, int v, int step, bool) {
+  row.template walk<kU>([&](auto& x, int v, int step, bool, int) {
     if (tail) {
       constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
@@ -392,37 +404,59 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
     }
     soft.add(x, c);
   });
-  soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
-    return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
-  }));
-  if (tail) lmax = red.max(lmax);
-  const float xmax = fmaxf(soft.m, lmax);
-  double listed = 0.0, cross = 0.0;
+
+  RowSum sum{soft, -CUDART_INF_F};
   for (int k = tid; k < a.k; k += threads) {
     if (ls.token[k] < 0) continue;
-    const double z = ((double)ls.x[k] - (double)xmax) * inv_tau, q = ls.q[k];
-    // a mass that underflows counts nothing, also on a masked token
-    if (q != 0.0) cross += q * z;
-    if (tail && ls.own[k]) listed += exp(z);
+    const float x = widen(g[ls.token[k]]);
+    ls.q[k] = (double)x;
+    sum.lmax = fmaxf(sum.lmax, x);
   }
-  const double2 sums = red.sum(make_double2(listed, cross));
-  listed = sums.x;
-  dot -= sums.y * q_scale;
-  if (tid == 0)
-    sm.f = row_factors(tail, soft.m, (double)soft.s, lmax, listed, q_sum, dot, inv_tau,
-                       a.temperature, weight, a.loss ? a.loss + r : nullptr);
-  if (grad == nullptr) return;
-  if (weight == 0.0f) {
-    for (int i = tid; i < vocab; i += threads) grad[i] = narrow<T>(0.0f);
+  sum = red.all(sum, [c](RowSum p, RowSum q) {
+    return RowSum{SoftSum::join(p.soft, q.soft, c), fmaxf(p.lmax, q.lmax)};
+  });
+  const float bmax = sum.soft.m, xmax = fmaxf(bmax, sum.lmax);
+  const double body = (double)sum.soft.s;
+  // masses: exp(a / tau - norm), or relative to the largest until their sum is known
+  const double from = tail ? 0.0 : (double)amax, norm = tail ? (double)a.log_norm[r] : 0.0;
+  for (int k = tid; k < a.k; k += threads) {
+    if (ls.token[k] < 0) continue;
+    const double log_q = ((double)ls.x[k] - from) * inv_tau - norm, t = log_q * kLog2e;
+    const double q = t <= 0.0 ? sm.table(t) : exp2(t);
+    const double z = (ls.q[k] - (double)xmax) * inv_tau;
+    sums.q += q;
+    // a mass that underflows counts nothing, also on a masked token
+    if (q != 0.0) sums.dot += q * (log_q - z);
+    if (tail && ls.own[k]) sums.listed += exp(z);
+    ls.x[k] = (float)ls.q[k];
+    ls.q[k] = q;
+  }
+  sums = red.all(sums, [](EntrySums p, EntrySums q) {
+    return EntrySums{p.q + q.q, p.dot + q.dot, p.listed + q.listed, p.twice | q.twice};
+  });
+  const double q_scale = tail ? 1.0 : 1.0 / sums.q;
+  const RowFactors f = row_factors(tail, bmax, body, xmax, sums.listed, sums.q * q_scale, inv_tau,
+                                   a.temperature, weight);
+  if (tid == 0) {
+    // what the list and the loss need waits in shared memory
+    sm.f = f;
+    sm.sums = sums;
+  }
+  auto write_loss = [&] {
+    const double dot = tail ? sums.dot : sums.dot * q_scale - log(sums.q);
+    a.loss[r] = row_loss(f, dot, bmax, xmax, body, inv_tau, a.temperature);
+  };
+  if (grad == nullptr || weight == 0.0f) {
+    if (tid == 0 && a.loss) write_loss();
+    if (grad)
+      for (int i = tid; i < vocab; i += threads) grad[i] = narrow<T>(0.0f);
     return;
   }
-  __syncthreads();
-  const RowFactors f = sm.f;
   T* gv = grad - row.ph;  // vector v of the row goes to gv[v * kE ..]
   const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
   const float2 minus = make_float2(-f.base, -f.base), scale = make_float2(c, c),
                G = make_float2(f.G, f.G);
-  row.template walk<kU>([&](auto& x, int v, int step, bool whole) {
+  row.template walk<kU>([&](auto& x, int v, int step, bool whole, int) {
     constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
     for (int u = 0; u < n; ++u) {
@@ -443,16 +477,23 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T*
     }
   });
   __syncthreads();
+  const bool twice = sm.sums.twice;
+  const double sum_q = sm.sums.q, scale_q = tail ? 1.0 : 1.0 / sum_q;
   for (int k = tid; k < a.k; k += threads) {
-    if (!ls.own[k]) continue;
+    if (ls.token[k] < 0 || !ls.own[k]) continue;
     double q = ls.q[k];
-    if (row_twice) {
+    if (twice) {
       q = 0.0;
       for (int j = 0; j < a.k; ++j)
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
-    const double e = exp(((double)ls.x[k] - f.shift) * inv_tau);
-    grad[ls.token[k]] = narrow<T>((float)(f.P * e - f.Q * (q * q_scale)));
+    const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
+    grad[ls.token[k]] = narrow<T>((float)(sm.f.P * e - sm.f.Q * (q * scale_q)));
+  }
+  // the last warp has fewest entries to see to
+  if (tid == threads - 1 && a.loss) {
+    const double dot = tail ? sm.sums.dot : sm.sums.dot * scale_q - log(sum_q);
+    a.loss[r] = row_loss(sm.f, dot, bmax, xmax, body, inv_tau, a.temperature);
   }
 }
 

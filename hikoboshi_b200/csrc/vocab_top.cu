@@ -136,13 +136,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
 
   const float c = kLog2ef / a.temperature;
   SoftSum soft;
-  float part[kU];  // largest logit of every kU-th of the thread's vectors
+  float part[kU];  // largest logit of the vectors in each slot
 #pragma unroll
   for (int u = 0; u < kU; ++u) part[u] = -CUDART_INF_F;
-  row.template walk<kU>([&](auto& x, int, int, bool) {
+  row.template walk<kU>([&](auto& x, int, int, bool, int slot) {
     constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-    for (int u = 0; u < n; ++u) part[u] = fmaxf(part[u], x[u].largest());
+    for (int u = 0; u < n; ++u) part[(slot + u) % kU] = fmaxf(part[(slot + u) % kU], x[u].largest());
     if (a.log_norm) soft.add(x, c);
   });
   const float tmax = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
       // the NaN (with a +inf the sum is not used)
       soft = SoftSum();
       soft.m = tmax;
-      row.template walk<1>([&](auto& x, int, int, bool) {
+      row.template walk<1>([&](auto& x, int, int, bool, int) {
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const float y = x[0].at(e);
@@ -160,9 +160,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
         }
       });
     }
-    soft = SoftSum::unpack(red.all(soft.pack(), [c](unsigned long long p, unsigned long long q) {
-      return SoftSum::join(SoftSum::unpack(p), SoftSum::unpack(q), c).pack();
-    }));
+    soft = red.all(soft, [c](SoftSum p, SoftSum q) { return SoftSum::join(p, q, c); });
     if (tid == 0) {
       const bool inf = soft.m == -CUDART_INF_F || soft.m == CUDART_INF_F;
       a.log_norm[r] =
@@ -170,7 +168,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
     }
   }
   // a lower bound of the k-th largest logit: one that k of the threads' own
-  // maxima reach, or k of the maxima of quarters of their logits
+  // maxima reach, or k of the maxima of their slots
   uint32_t bound = 0;
   if (a.k <= threads / 2) {
     bound = reached_by(order_key(tmax), a.k);
@@ -184,7 +182,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
   }
   const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
   __syncthreads();
-  row.template walk<kU>([&](auto& x, int v, int step, bool) {
+  row.template walk<kU>([&](auto& x, int v, int step, bool, int) {
     constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
     for (int u = 0; u < n; ++u) {
@@ -207,7 +205,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
     // the last index taken of its tokens
     auto count = [&](uint32_t lo, int last) {
       int m = 0;
-      row.template walk<1>([&](auto& x, int v, int, bool) {
+      row.template walk<1>([&](auto& x, int v, int, bool, int) {
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const float y = x[0].at(e);
@@ -231,7 +229,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __r
     }
     if (tid == 0) sm.list.count = 0;
     __syncthreads();
-    row.template walk<1>([&](auto& x, int v, int, bool) {
+    row.template walk<1>([&](auto& x, int v, int, bool, int) {
 #pragma unroll
       for (int e = 0; e < kE; ++e) {
         const float y = x[0].at(e);
@@ -452,7 +450,12 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
     return cudaGetLastError();
   }
   if (v.rows >= kStreamRows) {
-    top_stream_kernel<T><<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), 0, st>>>(
+    // twice as many threads as tokens wanted, where the row has work for them:
+    // the bound then comes from the threads' own maxima and is a close one
+    int threads = stream_threads(v.vocab, (int)sizeof(T));
+    const int vectors = v.vocab / (16 / (int)sizeof(T)) + 1;
+    while (threads < kMaxThreads && threads < 2 * a.k && threads < vectors) threads *= 2;
+    top_stream_kernel<T><<<(unsigned)v.rows, threads, 0, st>>>(
         static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
     return cudaGetLastError();
   }
