@@ -256,8 +256,9 @@ struct RowSlice {
   }
 };
 
-// Reductions over the CTA and its cluster; every thread gets the result, the
-// same bits in every CTA.  The partial results are added in a fixed order.
+// Reductions over the CTA and its cluster by a commutative operation; every
+// thread gets the result, the same bits in every CTA: the order of the
+// operations is fixed.  CTAs have a power of two of warps.
 constexpr int kSlotBytes = 32;
 struct ReduceScratch {
   alignas(16) unsigned char warp[2][kMaxWarps * kSlotBytes];
@@ -296,8 +297,10 @@ struct Reducer {
     V* part = reinterpret_cast<V*>(sc->warp[buf]);
     if (lane == 0) part[warp] = v;
     __syncthreads();
-    V r = part[0];
-    for (int w = 1; w < warps; ++w) r = op(r, part[w]);
+    // every warp joins the warps' values (their number is a power of two) in
+    // the same tree
+    V r = part[lane & (warps - 1)];
+    for (int o = 1; o < warps; o <<= 1) r = op(r, shfl_xor(r, o));
     if (kClustered) {
       // each CTA writes its value into every CTA's slots; two buffers, so a
       // slot is written again only after the next reduction's barrier

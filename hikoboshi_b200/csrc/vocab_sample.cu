@@ -36,10 +36,8 @@ RowShape row_shape(int64_t rows, int vocab, int elem_bytes) {
   s.chunk = (chunk + per16 - 1) / per16 * per16;
   const int vecs = s.chunk / per16 + 1;
   s.smem = (size_t)vecs * 16;
-  // a power of two (the bins of the sampler are dealt out evenly), about two
-  // vectors a thread
-  s.threads = 32;
-  while (s.threads < vocab::kMaxThreads && s.threads * 2 < vecs) s.threads *= 2;
+  // 256 or 512, about two vectors a thread
+  s.threads = vecs > 2 * 256 ? 512 : 256;
   return s;
 }
 
@@ -82,12 +80,33 @@ struct alignas(16) Bounds {
   int number, pad;
 };
 
+// Mass of some tokens and the span of some others.
+struct Extent {
+  double mass;
+  float most, least;
+};
+
+}  // namespace
+
+template <>
+__device__ __forceinline__ Extent shfl_xor(Extent v, int o) {
+  Extent r;
+  r.mass = __shfl_xor_sync(0xffffffffu, v.mass, o);
+  r.most = __shfl_xor_sync(0xffffffffu, v.most, o);
+  r.least = __shfl_xor_sync(0xffffffffu, v.least, o);
+  return r;
+}
+
+namespace {
+
 struct SampleSmem {
   Bounds bounds[kMaxWarps];
   ReduceScratch red;
   ReduceScratch block;
   double seg[kMaxWarps];
   int number[kMaxWarps];
+  unsigned sub_count;
+  unsigned long long sub[192];
   double step[32];  // a warp owns at most 17 steps of 32 vectors
   double total;
   Exp2Table table;
@@ -111,10 +130,8 @@ __device__ int locate(const RowSlice<T, kClustered>& row, Reducer<kClustered>& r
   int n = 0;
   row.for_each_from(skip, [&](int i, float x) {
     const double w = f(i, x);
-    if (w >= 0.0) {
-      mine += w;
-      ++n;
-    }
+    mine += w >= 0.0 ? w : 0.0;
+    n += w >= 0.0;
   });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -236,76 +253,405 @@ struct Weights {
   __device__ __forceinline__ double weight(float x) const { return (*table)(exponent(x)); }
 };
 
-// finish_list for more items than threads: sorts them, twice.
-__device__ __noinline__ void finish_long_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
-                            double need, int64_t r, const SampleArgs& a) {
-  unsigned long long* item = sm.list.item;
+// The sums of the threads before this one.
+__device__ __forceinline__ Bounds scan_bounds(Bounds v, SampleSmem& sm) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
+  Bounds incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float low = __shfl_up_sync(0xffffffffu, incl.low, o);
+    const float high = __shfl_up_sync(0xffffffffu, incl.high, o);
+    const int number = __shfl_up_sync(0xffffffffu, incl.number, o);
+    if (lane >= o) {
+      incl.low += low;
+      incl.high += high;
+      incl.number += number;
+    }
+  }
+  Bounds before;
+  before.low = __shfl_up_sync(0xffffffffu, incl.low, 1);
+  before.high = __shfl_up_sync(0xffffffffu, incl.high, 1);
+  before.number = __shfl_up_sync(0xffffffffu, incl.number, 1);
+  before.pad = 0;
+  if (lane == 0) before = Bounds{0.0f, 0.0f, 0, 0};
+  if (lane == 31) sm.bounds[warp] = incl;
+  __syncthreads();
+  for (int w = 0; w < warp && w < warps; ++w) {
+    before.low += sm.bounds[w].low;
+    before.high += sm.bounds[w].high;
+    before.number += sm.bounds[w].number;
+  }
+  return before;
+}
+
+// Bins of falling value from xhi on: the last that certainly belongs to the
+// head and the first that certainly ends it, with the tokens up to their ends.
+struct Bracket {
+  int certain, upto_certain, end, upto_end;
+};
+
+// Where the running mass from xhi on reaches `rest`, as far as the bins'
+// counts tell.  The bounds leave 1e-5 for the 32-bit arithmetic (exponents of at
+// most 45: 3e-6; sums: 1e-6).  Called by all threads of the CTA.
+template <typename F>
+__device__ __forceinline__ Bracket bracket(SampleSmem& sm, float scale, const Weights& wt,
+                                           float xhi, double rest64, F bin_count) {
+  constexpr int kPerThread = kBins / 256;  // CTAs have 256 threads or more
+  const int per = kBins / (int)blockDim.x, b0 = (int)threadIdx.x * per;
+  const float width2 = (float)(wt.c2 / (double)scale);  // of a bin, in powers of two
+  const float first = (float)wt.weight(xhi), rest = (float)rest64;
+  float low[kPerThread], high[kPerThread];
+  int number[kPerThread];
+  Bounds sum{0.0f, 0.0f, 0, 0};
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k) {
+    number[k] = k < per ? bin_count(b0 + k) : 0;
+    low[k] = (float)number[k] * first * exp2_fast(-(float)(b0 + k + 1) * width2) * 0.99999f;
+    high[k] = (float)number[k] * first * exp2_fast(-(float)(b0 + k) * width2) * 1.00001f;
+    sum.low += low[k];
+    sum.high += high[k];
+    sum.number += number[k];
+  }
+  Bounds run = scan_bounds(sum, sm);
+  unsigned long long certain = 0, ends = ~0ull;
+#pragma unroll
+  for (int k = 0; k < kPerThread; ++k)
+    if (k < per) {
+      run.low += low[k];
+      run.high += high[k];
+      run.number += number[k];
+      const unsigned long long v =
+          ((unsigned long long)(b0 + k + 1) << 32) | (unsigned)run.number;
+      if (run.high < rest * 0.999999f) certain = v;
+      if (run.low >= rest * 1.000001f || b0 + k == kBins - 1) ends = ::min(ends, v);
+    }
+  const ulonglong2 both = Reducer<false>(&sm.block).all(
+      make_ulonglong2(certain, ends), [](ulonglong2 p, ulonglong2 q) {
+        return make_ulonglong2(p.x > q.x ? p.x : q.x, p.y < q.y ? p.y : q.y);
+      });
+  __syncthreads();  // the reduction's scratch is free again
+  return {(int)(both.x >> 32) - 1, (int)(uint32_t)both.x, (int)(both.y >> 32) - 1,
+          (int)(uint32_t)both.y};
+}
+
+// Three counts of up to kListCap in one word.
+__device__ __forceinline__ unsigned long long three_counts(bool a, bool b, bool c) {
+  return (a ? 1ull : 0ull) | (b ? 1ull << 20 : 0ull) | (c ? 1ull << 40 : 0ull);
+}
+__device__ __forceinline__ int count_of(unsigned long long v, int i) {
+  return (int)(v >> (20 * i) & 0xfffffu);
+}
+
+// Smallest index up to which `want` of the list's n items with that key lie.
+__device__ __noinline__ int nth_index(SampleSmem& sm, int n, uint32_t key, int want) {
   Reducer<false> red(&sm.block);
-  sort_down(item, n);
-  const int nk = s.top_k > 0 ? ::min(n, s.top_k) : n;
-  const int per = (nk + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int i0 = ::min(nk, (int)threadIdx.x * per), i1 = ::min(nk, i0 + per);
-  auto weight = [&](int i) { return wt.weight(key_value(item_key(item[i]))); };
-  int n_kept = nk;
-  if (s.top_p < 1.0f || s.min_p > 0.0f) {
-    double mine = 0.0, total;
-    for (int i = i0; i < i1; ++i) mine += weight(i);
-    double run = block_scan(mine, sm.seg, &total) - mine;
-    if (need < 0.0) need = (double)s.top_p * total;
-    int under = 0, heavy = 0;
-    for (int i = i0; i < i1; ++i) {
-      const double w = weight(i);
-      run += w;
-      under += run < need;
-      heavy += w >= (double)s.min_p;
+  int from = 0, to = HKB_VOCAB_MAX - 1;
+  while (from < to) {
+    const int step = (to - from) / 4 + 1;
+    unsigned long long c = 0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const unsigned long long it = sm.list.item[i];
+      const int at = item_index(it);
+      if (item_key(it) == key)
+        c += three_counts(at < from + step, at < from + 2 * step, at < from + 3 * step);
     }
-    under = red.sum(under);
-    heavy = red.sum(heavy);
-    if (s.top_p < 1.0f) n_kept = ::min(n_kept, under + 1);
-    n_kept = ::max(1, ::min(n_kept, heavy));
+    c = red.sum(c);
+    const int k = count_of(c, 0) >= want ? 0 : count_of(c, 1) >= want ? 1 : count_of(c, 2) >= want ? 2 : 3;
+    const int end = ::min(to, from + step * (k + 1) - 1);
+    from = ::min(from + step * k, to);
+    if (k < 3) to = end;
   }
-  // the kept items in index order: (~index, key) downwards
   __syncthreads();
-  for (int i = threadIdx.x; i < n_kept; i += blockDim.x) item[i] = item[i] << 32 | item[i] >> 32;
+  return from;
+}
+
+// Of the n items of this CTA's list, in order, the one at which the running
+// mass, `above` before the first, reaches `need`; 0 if none does.  The bins of
+// the row's search again, now of the list's own span, leave a few items; each
+// of these adds up what comes before it.
+constexpr int kSubList = 192;
+
+__device__ __noinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights& wt,
+                                                          double above, double need) {
+  Reducer<false> red(&sm.block);
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const unsigned long long* item = sm.list.item;
+  float xhi = CUDART_INF_F, xlo = -CUDART_INF_F;
+  int left = n;
+  for (int round = 0; left > kSubList; ++round) {
+    // span of the items that are left
+    Extent ext{0.0, -CUDART_INF_F, CUDART_INF_F};
+    for (int i = tid; i < n; i += threads) {
+      const float x = key_value(item_key(item[i]));
+      if (x > xhi || x < xlo) continue;
+      ext.most = fmaxf(ext.most, x);
+      ext.least = fminf(ext.least, x);
+    }
+    ext = red.all(ext, [](Extent p, Extent q) {
+      return Extent{0.0, fmaxf(p.most, q.most), fminf(p.least, q.least)};
+    });
+    xhi = ext.most;
+    xlo = ext.least;
+    const float scale = (float)kBins / (xhi - xlo);
+    if (xlo < xhi && (!(scale > 0.0f && scale < CUDART_INF_F) || round == 16)) {
+      // no width of bins tells them apart (spans near the type's smallest
+      // numbers): the border's key by bisection
+      auto mass_from = [&](uint32_t key) {
+        double m = 0.0;
+        for (int i = tid; i < n; i += threads) {
+          const uint32_t k = item_key(item[i]);
+          if (k >= key && key_value(k) <= xhi) m += wt.weight(key_value(k));
+        }
+        return red.sum(m);
+      };
+      uint32_t lo = order_key(xlo), hi = order_key(xhi);
+      while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        if (above + mass_from(mid) >= need) lo = mid;
+        else hi = mid - 1;
+      }
+      if (key_value(lo) < xhi) above += mass_from(lo + 1);
+      xhi = xlo = key_value(lo);
+    }
+    if (xlo == xhi) {
+      // equal logits: by their number
+      const double w = wt.weight(xhi);
+      const double ties = w > 0.0 ? fmax(1.0, ceil((need - above) / w)) : 1.0;
+      if (ties > (double)left) return 0;
+      __syncthreads();
+      return list_item(order_key(xhi), nth_index(sm, n, order_key(xhi), (int)ties));
+    }
+    auto bin_of = [&](float x) { return ::min(kBins - 1, (int)((xhi - x) * scale)); };
+    for (int b = tid; b < kBins; b += threads) sm.hist[b] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += threads) {
+      const float x = key_value(item_key(item[i]));
+      if (x <= xhi && x >= xlo) atomicAdd(&sm.hist[bin_of(x)], 1u);
+    }
+    __syncthreads();
+    const Bracket br =
+        bracket(sm, scale, wt, xhi, need - above, [&](int b) { return (int)sm.hist[b]; });
+    ext = Extent{0.0, -CUDART_INF_F, CUDART_INF_F};
+    for (int i = tid; i < n; i += threads) {
+      const float x = key_value(item_key(item[i]));
+      if (x > xhi || x < xlo) continue;
+      const int b = bin_of(x);
+      if (b <= br.certain) {
+        ext.mass += wt.weight(x);
+      } else if (b <= br.end) {
+        ext.most = fmaxf(ext.most, x);
+        ext.least = fminf(ext.least, x);
+      }
+    }
+    ext = red.all(ext, [](Extent p, Extent q) {
+      return Extent{p.mass + q.mass, fmaxf(p.most, q.most), fminf(p.least, q.least)};
+    });
+    above += ext.mass;
+    left = br.upto_end - br.upto_certain;
+    xhi = ext.most;
+    xlo = ext.least;
+  }
+  // the items that are left, and the running mass at each of them
+  if (tid == 0) sm.sub_count = 0;
   __syncthreads();
-  sort_down(item, n_kept);
-  const int per2 = (n_kept + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int j0 = ::min(n_kept, (int)threadIdx.x * per2), j1 = ::min(n_kept, j0 + per2);
-  auto weight2 = [&](int i) { return wt.weight(key_value((uint32_t)item[i])); };
-  double mine = 0.0, total;
-  for (int i = j0; i < j1; ++i) mine += weight2(i);
-  double run = block_scan(mine, sm.seg, &total) - mine;
+  for (int i = tid; i < n; i += threads) {
+    const float x = key_value(item_key(item[i]));
+    if (x <= xhi && x >= xlo) sm.sub[atomicAdd(&sm.sub_count, 1u)] = item[i];
+  }
+  __syncthreads();
+  unsigned long long border = 0;
+  if (tid < left) {
+    const unsigned long long me = sm.sub[tid];
+    double run = above;
+    for (int j = 0; j < left; ++j) {
+      const unsigned long long it = sm.sub[j];
+      const double w = wt.weight(key_value(item_key(it)));
+      run += it >= me ? w : 0.0;
+    }
+    if (run >= need) border = me;
+  }
+  return red.max(border);
+}
+
+// The items of this CTA's list in registers, with their weights.
+constexpr int kOwnItems = 8;  // kListCap items over at least 256 threads
+
+struct Three {
+  double v[3];
+};
+
+}  // namespace
+
+template <>
+__device__ __forceinline__ Three shfl_xor(Three a, int o) {
+  Three r;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) r.v[i] = __shfl_xor_sync(0xffffffffu, a.v[i], o);
+  return r;
+}
+
+namespace {
+
+struct OwnItems {
+  uint32_t key[kOwnItems];
+  int index[kOwnItems];
+  double w[kOwnItems];  // 0 where the thread has no item
+  bool has[kOwnItems];
+
+  __device__ __forceinline__ void read(const SampleSmem& sm, int n, const Weights& wt) {
+#pragma unroll
+    for (int j = 0; j < kOwnItems; ++j) {
+      const int i = (int)threadIdx.x + j * (int)blockDim.x;
+      has[j] = i < n;
+      key[j] = 0;
+      index[j] = 0x7fffffff;
+      w[j] = 0.0;
+      if (has[j]) {
+        const unsigned long long it = sm.list.item[i];
+        key[j] = item_key(it);
+        index[j] = item_index(it);
+        w[j] = wt.weight(key_value(key[j]));
+      }
+    }
+  }
+  // The sum of f(j) over the items for which in(j) holds, for three tests at
+  // once: the barrier is the same.
+  template <typename In, typename F>
+  __device__ __forceinline__ Three sums(Reducer<false>& red, In in, F f) const {
+    Three t{{0.0, 0.0, 0.0}};
+#pragma unroll
+    for (int j = 0; j < kOwnItems; ++j)
+      if (has[j]) {
+        const double v = f(j);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) t.v[i] += in(j, i) ? v : 0.0;
+      }
+    return red.all(t, [](Three p, Three q) {
+      return Three{{p.v[0] + q.v[0], p.v[1] + q.v[1], p.v[2] + q.v[2]}};
+    });
+  }
+};
+
+// Of the list's n items, more than `want`, the want-th of the order.
+__device__ __noinline__ unsigned long long nth_item(SampleSmem& sm, int n, int want) {
+  Reducer<false> red(&sm.block);
+  uint32_t lo = 0, hi = 0xffffffffu;
+  while (lo < hi) {  // largest key that `want` items reach
+    const uint32_t step = (hi - lo) / 4 + 1;
+    const unsigned long long p = lo;
+    unsigned long long c = 0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const unsigned long long k = item_key(sm.list.item[i]);
+      c += three_counts(k >= p + step, k >= p + 2ull * step, k >= p + 3ull * step);
+    }
+    c = red.sum(c);
+    const int k = count_of(c, 2) >= want ? 3 : count_of(c, 1) >= want ? 2 : count_of(c, 0) >= want ? 1 : 0;
+    const uint32_t end = (uint32_t)::min((unsigned long long)hi, p + (unsigned long long)step * (k + 1) - 1);
+    lo += step * k;
+    if (k < 3) hi = end;
+  }
+  int above = 0;
+  for (int i = threadIdx.x; i < n; i += blockDim.x) above += item_key(sm.list.item[i]) > lo;
+  above = red.sum(above);
+  __syncthreads();
+  return list_item(lo, nth_index(sm, n, lo, want - above));
+}
+
+// finish_list for long lists: no order, but the borders and the token by
+// searches over the items' values, keys and indices.
+__device__ __noinline__ void finish_long_list(SampleSmem& sm, int n, const Weights& wt,
+                                              const RowSettings& s, double need, int64_t r,
+                                              const SampleArgs& a) {
+  Reducer<false> red(&sm.block);
+  // the items from the border on leave the list
+  auto cut = [&](unsigned long long border) {
+    unsigned long long mine[kOwnItems];
+    int left = 0;
+#pragma unroll
+    for (int j = 0; j < kOwnItems; ++j) {
+      const int i = (int)threadIdx.x + j * (int)blockDim.x;
+      mine[j] = i < n ? sm.list.item[i] : 0ull;
+    }
+    if (threadIdx.x == 0) sm.list.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kOwnItems; ++j)
+      if (mine[j] >= border && mine[j] != 0) {
+        sm.list.item[atomicAdd(&sm.list.count, 1u)] = mine[j];
+        ++left;
+      }
+    n = red.sum(left);
+    __syncthreads();
+  };
+  if (s.top_k > 0 && n > s.top_k) cut(nth_item(sm, n, s.top_k));
+  if (s.top_p < 1.0f) {
+    if (need < 0.0) {
+      double mass = 0.0;
+      for (int i = threadIdx.x; i < n; i += blockDim.x)
+        mass += wt.weight(key_value(item_key(sm.list.item[i])));
+      need = (double)s.top_p * red.sum(mass);
+      __syncthreads();
+    }
+    const unsigned long long border = border_in_list(sm, n, wt, 0.0, fmax(need, 1e-300));
+    __syncthreads();
+    if (border != 0) cut(border);
+  }
+  OwnItems own;
+  own.read(sm, n, wt);
+  auto weight = [&](int j) { return own.w[j]; };
+  int kept = 0;
+#pragma unroll
+  for (int j = 0; j < kOwnItems; ++j) {
+    own.has[j] = own.has[j] && own.w[j] >= (double)s.min_p;
+    kept += own.has[j];
+  }
+  kept = red.sum(kept);
+  const double total = own.sums(red, [](int, int) { return true; }, weight).v[0];
   const double target = s.u * total;
-  int hit = 0x7fffffff, last = -1;
-  for (int i = j0; i < j1; ++i) {
-    const double w = weight2(i);
-    run += w;
-    if (w > 0.0) {
-      last = i;
-      if (run > target && hit == 0x7fffffff) hit = i;
+  // smallest index up to which the mass exceeds the target (rounding, or u = 1,
+  // may leave none: the last with any)
+  int from = 0x7fffffff, to = -1;
+#pragma unroll
+  for (int j = 0; j < kOwnItems; ++j)
+    if (own.has[j] && own.w[j] > 0.0) {
+      from = ::min(from, own.index[j]);
+      to = ::max(to, own.index[j]);
     }
+  from = red.min(from);
+  to = red.max(to);
+  while (from < to) {
+    const int step = (to - from) / 4 + 1;
+    const Three t = own.sums(red, [&](int j, int i) { return own.index[j] < from + step * (i + 1); },
+                             weight);
+    int k = 3;
+#pragma unroll
+    for (int i = 2; i >= 0; --i)
+      if (t.v[i] > target) k = i;
+    const int end = ::min(to, from + step * (k + 1) - 1);
+    from += step * k;
+    if (k < 3) to = end;
+    else from = ::min(from, to);
   }
-  hit = red.min(hit);
-  last = red.max(last);
-  if (threadIdx.x == 0) {
-    const unsigned long long it = item[hit != 0x7fffffff ? hit : last];
-    const float x = key_value((uint32_t)it);
-    a.tokens[r] = (int)~(uint32_t)(it >> 32);
-    a.log_probs[r] = (float)(wt.exponent(x) * kLn2 - log(total));
-    a.kept[r] = n_kept;
-  }
+#pragma unroll
+  for (int j = 0; j < kOwnItems; ++j)
+    if (own.has[j] && own.index[j] == from) {
+      a.tokens[r] = from;
+      a.log_probs[r] = (float)(wt.exponent(key_value(own.key[j])) * kLn2 - log(total));
+      a.kept[r] = kept;
+    }
 }
 
 // Finishes a row whose kept tokens are all among the n items of this CTA's
 // list: puts them in order, cuts them to the shortest head and draws.  `need`
 // is the mass that ends the top-p head, or negative: top_p of the mass of the
-// first top_k items.  No more items than threads: each item's place in the
-// order, and its running mass in index order, is counted over all items by a
-// group of threads, which takes few barriers.
+// first top_k items.  Of a short list each item's place in the order, and its
+// running mass in index order, is counted over all items by a group of threads,
+// which takes few barriers.
+constexpr int kCountedItems = 192;
 __device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
                             double need, int64_t r, const SampleArgs& a) {
   const int threads = blockDim.x, tid = threadIdx.x;
-  if (n > threads) {
+  if (n > kCountedItems) {
     finish_long_list(sm, n, wt, s, need, r, a);
     return;
   }
@@ -360,57 +706,6 @@ __device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowS
   }
 }
 
-// The sums of the threads before this one.
-__device__ __forceinline__ Bounds scan_bounds(Bounds v, SampleSmem& sm) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (int)blockDim.x >> 5;
-  Bounds incl = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const float low = __shfl_up_sync(0xffffffffu, incl.low, o);
-    const float high = __shfl_up_sync(0xffffffffu, incl.high, o);
-    const int number = __shfl_up_sync(0xffffffffu, incl.number, o);
-    if (lane >= o) {
-      incl.low += low;
-      incl.high += high;
-      incl.number += number;
-    }
-  }
-  Bounds before;
-  before.low = __shfl_up_sync(0xffffffffu, incl.low, 1);
-  before.high = __shfl_up_sync(0xffffffffu, incl.high, 1);
-  before.number = __shfl_up_sync(0xffffffffu, incl.number, 1);
-  before.pad = 0;
-  if (lane == 0) before = Bounds{0.0f, 0.0f, 0, 0};
-  if (lane == 31) sm.bounds[warp] = incl;
-  __syncthreads();
-  for (int w = 0; w < warp && w < warps; ++w) {
-    before.low += sm.bounds[w].low;
-    before.high += sm.bounds[w].high;
-    before.number += sm.bounds[w].number;
-  }
-  return before;
-}
-
-// Of the n items of this CTA's list, in order, the one at which the running
-// mass, `above` before the first, reaches `need`; 0 if none does.
-__device__ __noinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights& wt,
-                                                          double above, double need) {
-  const unsigned long long* item = sm.list.item;
-  sort_down(sm.list.item, n);
-  const int per = (n + (int)blockDim.x - 1) / (int)blockDim.x;
-  const int i0 = ::min(n, (int)threadIdx.x * per), i1 = ::min(n, i0 + per);
-  double mine = 0.0, total;
-  for (int i = i0; i < i1; ++i) mine += wt.weight(key_value(item_key(item[i])));
-  double run = above + (block_scan(mine, sm.seg, &total) - mine);
-  int under = 0;
-  for (int i = i0; i < i1; ++i) {
-    run += wt.weight(key_value(item_key(item[i])));
-    under += run < need;
-  }
-  under = Reducer<false>(&sm.block).sum(under);
-  return under < n ? item[under] : 0ull;
-}
-
 template <typename T, bool kClustered>
 __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
@@ -427,7 +722,6 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   RowSettings s = row_settings(a, r);
   const bool valid = settings_valid(s);
   const bool writer = threadIdx.x == 0 && row.rank == 0;
-  for (int b = threadIdx.x; b < kBins; b += blockDim.x) sm.hist[b] = 0;
   sm.table.fill();
   cp_async_wait_all();
   if (kClustered) cg::this_cluster().sync();  // every CTA of the row runs from here on
@@ -539,7 +833,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   if (s.top_p < 1.0f) {
     double m = 0.0;
     row.for_each_from(xt, [&](int i, float x) {
-      if (in_head(i, x)) m += wt.weight(x);
+      const double w = wt.weight(x);
+      m += in_head(i, x) ? w : 0.0;
     });
     const double mass = red.sum(m);
     const double need = (double)s.top_p * mass;
@@ -548,128 +843,104 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const double z0 =
         fmax(zmin, log2((1.0 - (double)s.top_p) * mass / (double)vocab) - 1e-3);
     reach = (float)(-z0 / wt.c2) * 1.000001f;
-    // a vector with nothing from here on has nothing within reach
-    const float skip = fmaxf(xt, xmax - reach * 1.00001f);
-    // Count the tokens within reach in bins of equal width: a bin's weights lie
-    // between those of its ends, so the counts bound the running mass from both
-    // sides (1e-4 covers the 32-bit arithmetic), and the border lies in the
-    // few bins that the two bounds leave.
-    const float scale = (float)kBins / reach;
-    // temperatures at the ends of the type's range leave no finite bin width
-    const bool binned = scale > 0.0f && scale < CUDART_INF_F;
-    auto within = [&](int i, float x) { return xmax - x <= reach && in_head(i, x); };
-    auto bin_of = [&](float x) { return ::min(kBins - 1, (int)((xmax - x) * scale)); };
-    if (binned)
-      row.for_each_from(skip, [&](int i, float x) {
+    // The border lies between xhi and xlo, `above` is the mass of the head
+    // before xhi.  The tokens between are counted in bins of equal width: a
+    // bin's weights lie between those of its ends, so the counts bound the
+    // running mass from both sides, and the border lies in the few bins that
+    // the two bounds leave.  They are put in
+    // order, or divided again while they are too many for the list.
+    float xhi = xmax, xlo = fmaxf(xt, xmax - reach * 1.00001f);
+    double above = 0.0;
+    bool found = false;
+    for (int round = 0; round < 8 && !found && xlo < xhi; ++round) {
+      const float scale = (float)kBins / (xhi - xlo);
+      // temperatures at the ends of the type's range leave no finite bin width
+      if (!(scale > 0.0f && scale < CUDART_INF_F)) break;
+      auto within = [&](int i, float x) { return x >= xlo && x <= xhi && in_head(i, x); };
+      auto bin_of = [&](float x) { return ::min(kBins - 1, (int)((xhi - x) * scale)); };
+      for (int b = threadIdx.x; b < kBins; b += blockDim.x) sm.hist[b] = 0;
+      __syncthreads();
+      row.for_each_from(xlo, [&](int i, float x) {
         if (within(i, x)) atomicAdd(&sm.hist[bin_of(x)], 1u);
       });
-    if (kClustered) cg::this_cluster().sync();
-    else __syncthreads();
-    // every CTA adds up the whole row's bins and finds the same border
-    const int per = kBins / (int)blockDim.x, b0 = (int)threadIdx.x * per;
-    const float width2 = (float)(wt.c2 / (double)scale);  // of a bin, in powers of two
-    Bounds mine{0.0f, 0.0f, 0, 0};
-    auto bin_count = [&](int b) {
-      if (!kClustered) return (int)sm.hist[b];
-      int c = 0;
-      for (int k = 0; k < row.size; ++k)
-        c += (int)cg::this_cluster().map_shared_rank(sm.hist, k)[b];
-      return c;
-    };
-    constexpr int kKept = 4;  // bins whose counts a thread keeps
-    int counts[kKept];
-#pragma unroll
-    for (int k = 0; k < kKept; ++k) counts[k] = k < per ? bin_count(b0 + k) : 0;
-    auto grow = [&](Bounds& v, int k) {
-      const int c = k < kKept ? counts[k & (kKept - 1)] : bin_count(b0 + k);
-      v.low += (float)c * exp2f(-(float)(b0 + k + 1) * width2) * 0.9999f;
-      v.high += (float)c * exp2f(-(float)(b0 + k) * width2) * 1.0001f;
-      v.number += c;
-    };
-#pragma unroll
-    for (int k = 0; k < kKept; ++k)
-      if (k < per) grow(mine, k);
-    for (int k = kKept; k < per; ++k) grow(mine, k);
-    Bounds run = scan_bounds(mine, sm);
-    // last bin that is certainly kept, first bin that certainly ends the head,
-    // with the tokens up to their ends
-    unsigned long long certain = 0, ends = ~0ull;
-    auto judge = [&](int k) {
-      grow(run, k);
-      const unsigned long long v =
-          ((unsigned long long)(b0 + k + 1) << 32) | (unsigned)run.number;
-      if (run.high < (float)need * 0.9999f) certain = v;
-      if (run.low >= (float)need * 1.0001f || b0 + k == kBins - 1) ends = ::min(ends, v);
-    };
-#pragma unroll
-    for (int k = 0; k < kKept; ++k)
-      if (k < per) judge(k);
-    for (int k = kKept; k < per; ++k) judge(k);
-    Reducer<false> block(&sm.block);
-    const ulonglong2 borders = block.all(make_ulonglong2(certain, ends),
-                                         [](ulonglong2 p, ulonglong2 q) {
-                                           return make_ulonglong2(p.x > q.x ? p.x : q.x,
-                                                                  p.y < q.y ? p.y : q.y);
-                                         });
-    const int last_certain = (int)(borders.x >> 32) - 1, upto_certain = (int)(uint32_t)borders.x;
-    const int end_bin = (int)(borders.y >> 32) - 1, upto_end = (int)(uint32_t)borders.y;
-
-    const bool all_listed = upto_end <= kListCap;
-    const int list_from = all_listed ? -1 : last_certain;
-    if (binned && (all_listed || upto_end - upto_certain <= kListCap)) {
-      double above = 0.0;
-      if (!all_listed) {
-        row.for_each_from(skip, [&](int i, float x) {
-          if (within(i, x) && bin_of(x) <= list_from) above += wt.weight(x);
+      if (kClustered) cg::this_cluster().sync();
+      else __syncthreads();
+      // every CTA adds up the whole row's bins and finds the same border
+      const Bracket br = bracket(
+          sm, scale, wt, xhi, need - above, [&](int b) {
+            if (!kClustered) return (int)sm.hist[b];
+            int c = 0;
+            for (int k = 0; k < row.size; ++k)
+              c += (int)cg::this_cluster().map_shared_rank(sm.hist, k)[b];
+            return c;
+          });
+      if (round == 0 && br.upto_end <= kListCap) {
+        const int n = collect(row, red, sm.list, xlo, [&](int i, float x) {
+          return within(i, x) && bin_of(x) <= br.end;
         });
-        above = red.sum(above);
-      }
-      const int n = collect(row, red, sm.list, skip, [&](int i, float x) {
-        if (!within(i, x)) return false;
-        const int b = bin_of(x);
-        return b > list_from && b <= end_bin;
-      });
-      if (all_listed) {
         if (row.rank == 0) finish_list(sm, n, wt, s, need, r, a);
         return;
       }
-      // the head ends inside the list, or (cut by min-p) nowhere
-      unsigned long long border = 0;
-      if (row.rank == 0) border = border_in_list(sm, n, wt, above, need);
-      border = red.spread(border)[0];
-      if (border != 0) {
-        xt = key_value(item_key(border));
-        icut = item_index(border);
+      // the mass before the uncertain bins, and the tokens in them or their span
+      const bool listed = br.upto_end - br.upto_certain <= kListCap;
+      Extent ext{0.0, -CUDART_INF_F, CUDART_INF_F};
+      const int n = collect(row, red, sm.list, xlo, [&](int i, float x) {
+        const bool in = within(i, x);
+        const int b = in ? bin_of(x) : kBins;
+        const double w = wt.weight(x);
+        ext.mass += b <= br.certain ? w : 0.0;
+        const bool open = b > br.certain && b <= br.end;
+        ext.most = open ? fmaxf(ext.most, x) : ext.most;
+        ext.least = open ? fminf(ext.least, x) : ext.least;
+        return open && listed;
+      });
+      ext = red.all(ext, [](Extent p, Extent q) {
+        return Extent{p.mass + q.mass, fmaxf(p.most, q.most), fminf(p.least, q.least)};
+      });
+      above += ext.mass;
+      if (listed) {
+        // the head ends inside the list, or (cut by min-p) nowhere
+        unsigned long long border = 0;
+        if (row.rank == 0) border = border_in_list(sm, n, wt, above, need);
+        border = red.spread(border)[0];
+        if (border != 0) {
+          xt = key_value(item_key(border));
+          icut = item_index(border);
+        }
+        found = true;
       }
-    } else {
-      // equal logits crowd a bin: bisect
-      auto mass_from = [&](uint32_t key) {
-        const float from = key_value(key);
-        double v = 0.0;
-        row.for_each_from(from, [&](int i, float x) {
-          if (x >= from && in_head(i, x)) v += wt.weight(x);
-        });
-        return red.sum(v);
-      };
-      uint32_t lo = order_key(xt), hi = order_key(xmax);
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (mass_from(mid) >= need) lo = mid;
-        else hi = mid - 1;
+      xhi = ext.most;
+      xlo = ext.least;
+    }
+    if (!found) {
+      if (xlo < xhi) {
+        // by bisection of keys; only for temperatures without a bin width
+        auto mass_from = [&](uint32_t key) {
+          const float from = key_value(key);
+          double v = 0.0;
+          row.for_each_from(from, [&](int i, float x) {
+            if (x >= from && in_head(i, x)) v += wt.weight(x);
+          });
+          return red.sum(v);
+        };
+        uint32_t lo = order_key(xlo), hi = order_key(xhi);
+        while (lo < hi) {
+          const uint32_t mid = lo + (hi - lo + 1) / 2;
+          if (mass_from(mid) >= need) lo = mid;
+          else hi = mid - 1;
+        }
+        xhi = key_value(lo);
+        above = lo == order_key(xmax) ? 0.0 : mass_from(lo + 1);
       }
-      // `lo` is the border's key: of its tokens the first `ties` are kept
-      const float border = key_value(lo);
-      const double above = lo == order_key(xmax) ? 0.0 : mass_from(lo + 1);
-      const double w = wt.weight(border);
+      // the head ends among the tokens that equal xhi: the first `ties` are kept
+      const double w = wt.weight(xhi);
       double ties = w > 0.0 ? ceil((need - above) / w) : 1.0;
       if (ties < 1.0) ties = 1.0;
       double all_ties;
       int n;
-      icut = red.max(locate(row, red, sm, border, ties - 0.5, true, &all_ties, &n,
-                            [&](int i, float x) {
-                              return x == border && in_head(i, x) ? 1.0 : -1.0;
-                            }));
-      xt = border;
+      icut = red.max(locate(row, red, sm, xhi, ties - 0.5, true, &all_ties, &n,
+                            [&](int i, float x) { return x == xhi && in_head(i, x) ? 1.0 : -1.0; }));
+      xt = xhi;
     }
   }
   // draw among the kept tokens of the whole row
@@ -677,9 +948,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   double total;
   int n;
   const int token = locate(row, red, sm, skip, s.u, false, &total, &n, [&](int i, float x) {
-    if (!in_head(i, x)) return -1.0;
     const double w = wt.weight(x);
-    return w >= (double)s.min_p ? w : -1.0;
+    return in_head(i, x) && w >= (double)s.min_p ? w : -1.0;
   });
   if (token >= 0 && (threadIdx.x & 31) == 0) {
     const float x = fminf(widen(g[token]), xmax);
