@@ -320,7 +320,7 @@ struct StreamSmem {
 // for its token.  The entries' own work comes between the two passes: the row
 // is on its way all the while, and a barrier costs as much as a tenth of a row.
 template <typename T>
-__global__ void __launch_bounds__(kMaxThreads, 2) distill_stream_kernel(const T* logits,
+__global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const T* logits,
                                                                            int64_t row_stride,
                                                                            int vocab,
                                                                            DistillArgs a) {

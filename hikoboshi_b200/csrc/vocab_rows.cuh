@@ -577,10 +577,11 @@ __device__ __forceinline__ SoftSum shfl_xor(SoftSum v, int o) {
 // Threads for a CTA that streams rows: a power of two, 20 to 40 vectors a thread.  Fewer threads a row leave room for more CTAs, whose
 // barriers then cover each other.  Measured (loss and gradient, us): 2000 x
 // 50001 bf16 243 with 512 threads, 172 with 256; 4096 x 131072 bf16 478 and 484.
+constexpr int kStreamThreads = 512;
 inline int stream_threads(int vocab, int elem_bytes) {
   const int nvec = vocab / (16 / elem_bytes) + 1;
   int t = 32;
-  while (t < kMaxThreads && t * 40 < nvec) t *= 2;
+  while (t < kStreamThreads && t * 40 < nvec) t *= 2;
   return t;
 }
 

@@ -36,7 +36,8 @@ RowShape row_shape(int64_t rows, int vocab, int elem_bytes) {
   s.chunk = (chunk + per16 - 1) / per16 * per16;
   const int vecs = s.chunk / per16 + 1;
   s.smem = (size_t)vecs * 16;
-  // 256 or 512, about two vectors a thread
+  // 256 or 512, about two vectors a thread (1024 is no faster for a single row:
+  // the barriers take longer)
   s.threads = vecs > 2 * 256 ? 512 : 256;
   return s;
 }
@@ -66,13 +67,14 @@ __device__ __forceinline__ RowSettings row_settings(const SampleArgs& a, int64_t
   return s;
 }
 
-__device__ __forceinline__ bool settings_valid(const RowSettings& s) {
+__device__ __forceinline__ bool settings_valid(const RowSettings s) {
   return s.temperature >= 0.0f && s.temperature < CUDART_INF_F && s.top_k >= 0 &&
          s.top_p >= 0.0f && s.top_p <= 1.0f && s.min_p >= 0.0f && s.min_p <= 1.0f &&
          s.u >= 0.0 && s.u <= 1.0;
 }
 
 constexpr int kBins = 1024;
+constexpr int kSubList = 192;  // items of a list whose order is found by counting
 
 // Bounds of the running mass and the number of tokens up to a bin.
 struct alignas(16) Bounds {
@@ -106,7 +108,8 @@ struct SampleSmem {
   double seg[kMaxWarps];
   int number[kMaxWarps];
   unsigned sub_count;
-  unsigned long long sub[192];
+  unsigned long long sub[kSubList];
+  double sub_weight[kSubList];
   double step[32];  // a warp owns at most 17 steps of 32 vectors
   double total;
   Exp2Table table;
@@ -294,7 +297,7 @@ struct Bracket {
 // counts tell.  The bounds leave 1e-5 for the 32-bit arithmetic (exponents of at
 // most 45: 3e-6; sums: 1e-6).  Called by all threads of the CTA.
 template <typename F>
-__device__ __forceinline__ Bracket bracket(SampleSmem& sm, float scale, const Weights& wt,
+__device__ __forceinline__ Bracket bracket(SampleSmem& sm, float scale, const Weights wt,
                                            float xhi, double rest64, F bin_count) {
   constexpr int kPerThread = kBins / 256;  // CTAs have 256 threads or more
   const int per = kBins / (int)blockDim.x, b0 = (int)threadIdx.x * per;
@@ -343,7 +346,7 @@ __device__ __forceinline__ int count_of(unsigned long long v, int i) {
 }
 
 // Smallest index up to which `want` of the list's n items with that key lie.
-__device__ __noinline__ int nth_index(SampleSmem& sm, int n, uint32_t key, int want) {
+__device__ __forceinline__ int nth_index(SampleSmem& sm, int n, uint32_t key, int want) {
   Reducer<false> red(&sm.block);
   int from = 0, to = HKB_VOCAB_MAX - 1;
   while (from < to) {
@@ -369,9 +372,7 @@ __device__ __noinline__ int nth_index(SampleSmem& sm, int n, uint32_t key, int w
 // mass, `above` before the first, reaches `need`; 0 if none does.  The bins of
 // the row's search again, now of the list's own span, leave a few items; each
 // of these adds up what comes before it.
-constexpr int kSubList = 192;
-
-__device__ __noinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights& wt,
+__device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights wt,
                                                           double above, double need) {
   Reducer<false> red(&sm.block);
   const int tid = threadIdx.x, threads = blockDim.x;
@@ -456,18 +457,18 @@ __device__ __noinline__ unsigned long long border_in_list(SampleSmem& sm, int n,
   __syncthreads();
   for (int i = tid; i < n; i += threads) {
     const float x = key_value(item_key(item[i]));
-    if (x <= xhi && x >= xlo) sm.sub[atomicAdd(&sm.sub_count, 1u)] = item[i];
+    if (x > xhi || x < xlo) continue;
+    const unsigned at = atomicAdd(&sm.sub_count, 1u);
+    sm.sub[at] = item[i];
+    sm.sub_weight[at] = wt.weight(x);
   }
   __syncthreads();
   unsigned long long border = 0;
   if (tid < left) {
     const unsigned long long me = sm.sub[tid];
     double run = above;
-    for (int j = 0; j < left; ++j) {
-      const unsigned long long it = sm.sub[j];
-      const double w = wt.weight(key_value(item_key(it)));
-      run += it >= me ? w : 0.0;
-    }
+#pragma unroll 4
+    for (int j = 0; j < left; ++j) run += sm.sub[j] >= me ? sm.sub_weight[j] : 0.0;
     if (run >= need) border = me;
   }
   return red.max(border);
@@ -498,7 +499,7 @@ struct OwnItems {
   double w[kOwnItems];  // 0 where the thread has no item
   bool has[kOwnItems];
 
-  __device__ __forceinline__ void read(const SampleSmem& sm, int n, const Weights& wt) {
+  __device__ __forceinline__ void read(const SampleSmem& sm, int n, const Weights wt) {
 #pragma unroll
     for (int j = 0; j < kOwnItems; ++j) {
       const int i = (int)threadIdx.x + j * (int)blockDim.x;
@@ -533,7 +534,7 @@ struct OwnItems {
 };
 
 // Of the list's n items, more than `want`, the want-th of the order.
-__device__ __noinline__ unsigned long long nth_item(SampleSmem& sm, int n, int want) {
+__device__ __forceinline__ unsigned long long nth_item(SampleSmem& sm, int n, int want) {
   Reducer<false> red(&sm.block);
   uint32_t lo = 0, hi = 0xffffffffu;
   while (lo < hi) {  // largest key that `want` items reach
@@ -559,8 +560,8 @@ __device__ __noinline__ unsigned long long nth_item(SampleSmem& sm, int n, int w
 
 // finish_list for long lists: no order, but the borders and the token by
 // searches over the items' values, keys and indices.
-__device__ __noinline__ void finish_long_list(SampleSmem& sm, int n, const Weights& wt,
-                                              const RowSettings& s, double need, int64_t r,
+__device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const Weights wt,
+                                              const RowSettings s, double need, int64_t r,
                                               const SampleArgs& a) {
   Reducer<false> red(&sm.block);
   // the items from the border on leave the list
@@ -647,18 +648,17 @@ __device__ __noinline__ void finish_long_list(SampleSmem& sm, int n, const Weigh
 // first top_k items.  Of a short list each item's place in the order, and its
 // running mass in index order, is counted over all items by a group of threads,
 // which takes few barriers.
-constexpr int kCountedItems = 192;
-__device__ void finish_list(SampleSmem& sm, int n, const Weights& wt, const RowSettings& s,
+__device__ __forceinline__ void finish_list(SampleSmem& sm, int n, const Weights wt, const RowSettings s,
                             double need, int64_t r, const SampleArgs& a) {
   const int threads = blockDim.x, tid = threadIdx.x;
-  if (n > kCountedItems) {
+  if (n > kSubList) {
     finish_long_list(sm, n, wt, s, need, r, a);
     return;
   }
   Reducer<false> red(&sm.block);
   const unsigned long long* item = sm.list.item;
-  unsigned long long* sorted = sm.list.item + kMaxThreads;
-  double* weight = reinterpret_cast<double*>(sm.list.item + 2 * kMaxThreads);
+  unsigned long long* sorted = sm.list.item + kListCap / 4;
+  double* weight = reinterpret_cast<double*>(sm.list.item + kListCap / 2);
   int group = 32;  // threads an item, a power of two
   while (group > 1 && n * group > threads) group >>= 1;
   const int i = tid / group, part = tid % group;
@@ -787,23 +787,23 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   }
   const Weights wt{xmax, c2, &sm.table};
 
+  int listed = -1;  // tokens of rank 0's list, where it holds all that can be kept
+
   // Top-k of a number that fits the list: the k-th largest of the row is no
   // less than the k/C-th largest of the threads' own largest logits in the CTA
   // where that is least, and few more than k tokens reach it.
   if (list_k) {
     const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
     const int n = collect(row, red, sm.list, from, [&](int, float x) { return x >= from; });
-    if (n <= kListCap) {
-      if (row.rank == 0) finish_list(sm, n, wt, s, -1.0, r, a);
-      return;
-    }
+    if (n <= kListCap) listed = n;
   }
+  double list_need = -1.0;  // top_p of the list's own mass
 
   // The kept head so far: x > xt, or x == xt and index <= icut.
   float xt = -CUDART_MAX_NORMAL_F;
   int icut = 0x7fffffff;
   auto in_head = [&](int i, float x) { return x >= xt && !(x == xt && i > icut); };
-  if (s.top_k > 0) {
+  if (listed < 0 && s.top_k > 0) {
     // largest value with at least k tokens at or above it, by bisection of keys
     auto count = [&](uint32_t key) {
       const float from = key_value(key);
@@ -830,7 +830,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   const double zmin = s.min_p > 0.0f ? log2((double)s.min_p) - 1e-3 : -CUDART_INF;
   float reach = s.min_p > 0.0f ? (float)(-zmin / wt.c2) * 1.000001f : CUDART_INF_F;
 
-  if (s.top_p < 1.0f) {
+  if (listed < 0 && s.top_p < 1.0f) {
     double m = 0.0;
     row.for_each_from(xt, [&](int i, float x) {
       const double w = wt.weight(x);
@@ -852,7 +852,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     float xhi = xmax, xlo = fmaxf(xt, xmax - reach * 1.00001f);
     double above = 0.0;
     bool found = false;
-    for (int round = 0; round < 8 && !found && xlo < xhi; ++round) {
+    for (int round = 0; round < 8 && !found && listed < 0 && xlo < xhi; ++round) {
       const float scale = (float)kBins / (xhi - xlo);
       // temperatures at the ends of the type's range leave no finite bin width
       if (!(scale > 0.0f && scale < CUDART_INF_F)) break;
@@ -878,11 +878,12 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
         const int n = collect(row, red, sm.list, xlo, [&](int i, float x) {
           return within(i, x) && bin_of(x) <= br.end;
         });
-        if (row.rank == 0) finish_list(sm, n, wt, s, need, r, a);
-        return;
+        listed = n;
+        list_need = need;
+        break;
       }
       // the mass before the uncertain bins, and the tokens in them or their span
-      const bool listed = br.upto_end - br.upto_certain <= kListCap;
+      const bool fits = br.upto_end - br.upto_certain <= kListCap;
       Extent ext{0.0, -CUDART_INF_F, CUDART_INF_F};
       const int n = collect(row, red, sm.list, xlo, [&](int i, float x) {
         const bool in = within(i, x);
@@ -892,13 +893,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
         const bool open = b > br.certain && b <= br.end;
         ext.most = open ? fmaxf(ext.most, x) : ext.most;
         ext.least = open ? fminf(ext.least, x) : ext.least;
-        return open && listed;
+        return open && fits;
       });
       ext = red.all(ext, [](Extent p, Extent q) {
         return Extent{p.mass + q.mass, fmaxf(p.most, q.most), fminf(p.least, q.least)};
       });
       above += ext.mass;
-      if (listed) {
+      if (fits) {
         // the head ends inside the list, or (cut by min-p) nowhere
         unsigned long long border = 0;
         if (row.rank == 0) border = border_in_list(sm, n, wt, above, need);
@@ -912,7 +913,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
       xhi = ext.most;
       xlo = ext.least;
     }
-    if (!found) {
+    if (!found && listed < 0) {
       if (xlo < xhi) {
         // by bisection of keys; only for temperatures without a bin width
         auto mass_from = [&](uint32_t key) {
@@ -942,6 +943,10 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
                             [&](int i, float x) { return x == xhi && in_head(i, x) ? 1.0 : -1.0; }));
       xt = xhi;
     }
+  }
+  if (listed >= 0) {
+    if (row.rank == 0) finish_list(sm, listed, wt, s, list_need, r, a);
+    return;
   }
   // draw among the kept tokens of the whole row
   const float skip = fmaxf(xt, xmax - reach * 1.00001f);

@@ -122,7 +122,7 @@ struct TopStreamSmem {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(kMaxThreads, 2) top_stream_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* __restrict__ logits,
                                                                     int64_t row_stride, int vocab,
                                                                     TopArgs a) {
   __shared__ TopStreamSmem sm;
@@ -454,7 +454,7 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
     // the bound then comes from the threads' own maxima and is a close one
     int threads = stream_threads(v.vocab, (int)sizeof(T));
     const int vectors = v.vocab / (16 / (int)sizeof(T)) + 1;
-    while (threads < kMaxThreads && threads < 2 * a.k && threads < vectors) threads *= 2;
+    while (threads < kStreamThreads && threads < 2 * a.k && threads < vectors) threads *= 2;
     top_stream_kernel<T><<<(unsigned)v.rows, threads, 0, st>>>(
         static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
     return cudaGetLastError();
