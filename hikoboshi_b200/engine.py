@@ -4,7 +4,8 @@ Mirrors the reference's module-level entry points for the design path
 (cpp/include/hikoboshi/modules/mpnn/inverse_fold.hpp:113-147 and the
 algorithms-layer loop of cpp/algorithms/inverse_fold.cpp:221-356) for batches
 of proteins: ``design`` (autoregressive sampling), ``score`` (teacher-forced),
-``encode`` and ``knn`` (intermediates), plus the host-only ``decode_order``
+``resample`` and ``distill_targets`` (new tokens and a student's targets from
+scored rows), ``encode`` and ``knn`` (intermediates), plus the host-only ``decode_order``
 and ``synthetic_backbone``.  Errors surface as ``HkbError`` carrying the
 reference's status code and static detail string.
 """
@@ -184,6 +185,67 @@ class DesignEngine:
                         scores[sq:sq + S[b]]))
             q += n
             sq += int(S[b])
+        return res
+
+    # -- from scored rows to new tokens and to a student's targets -------------
+    def _scored_rows(self, coords, sources, tokens, orders, seeds):
+        """Unscaled log-probs of all proteins' rows, [Q, 21] on the engine's device."""
+        import torch
+        res = self.score(coords, sources, tokens, orders=orders, seeds=seeds)
+        rows = np.concatenate([lp.reshape(-1, V) for lp, _, _ in res])
+        shapes = [lp.shape[:2] for lp, _, _ in res]
+        return torch.from_numpy(rows).to(torch.device("cuda", self.device)), shapes
+
+    def resample(self, coords: Sequence[np.ndarray], sources: Sequence[np.ndarray],
+                 tokens: Sequence[np.ndarray], uniforms: Sequence[np.ndarray], *,
+                 temperature: float = 0.1, top_k: int = 0, top_p: float = 1.0,
+                 min_p: float = 0.0, orders: Sequence[np.ndarray] | None = None,
+                 seeds: Sequence[int] | int = 0):
+        """Draws every position of given sequences anew from its teacher-forced
+        distribution, cut by ``top_k``, ``top_p`` and ``min_p``
+        (:func:`hikoboshi_b200.vocab.sample_tokens`).  ``tokens[b]`` and
+        ``uniforms[b]`` (in [0, 1]) are [S_b, L_b].  Returns per protein
+        (tokens [S, L] int32, log_probs [S, L], kept [S, L] int32)."""
+        import torch
+
+        from . import vocab
+        rows, shapes = self._scored_rows(coords, sources, tokens, orders, seeds)
+        us = [np.asarray(u, np.float64) for u in uniforms]
+        if len(us) != len(shapes) or any(u.size != s * n for u, (s, n) in zip(us, shapes)):
+            raise _lib.HkbError(_lib.HKB_INVALID_ARGUMENT,
+                                "uniforms must have one number per position")
+        u = torch.from_numpy(np.concatenate([u.reshape(-1) for u in us])).to(rows.device)
+        with torch.cuda.device(rows.device):
+            got = vocab.sample_tokens(rows, u, temperature=temperature, top_k=top_k, top_p=top_p,
+                                      min_p=min_p)
+        t, lp, kept = (a.cpu().numpy() for a in got)
+        res = []
+        q = 0
+        for s, n in shapes:
+            res.append(tuple(a[q:q + s * n].reshape(s, n) for a in (t, lp, kept)))
+            q += s * n
+        return res
+
+    def distill_targets(self, coords: Sequence[np.ndarray], sources: Sequence[np.ndarray],
+                        tokens: Sequence[np.ndarray], k: int, *, temperature: float = 1.0,
+                        orders: Sequence[np.ndarray] | None = None,
+                        seeds: Sequence[int] | int = 0):
+        """What a student learns of this engine's teacher-forced answers: per
+        protein the ``k`` largest log-probs of every position with their tokens
+        and the row's log-norm at ``temperature``, [S, L, k] and [S, L] torch
+        tensors on the engine's device (:class:`hikoboshi_b200.vocab.TopLogits`),
+        as :func:`hikoboshi_b200.vocab.distill_loss` takes them."""
+        import torch
+
+        from . import vocab
+        rows, shapes = self._scored_rows(coords, sources, tokens, orders, seeds)
+        with torch.cuda.device(rows.device):
+            top = vocab.top_logits(rows, k, temperature=temperature)
+        res = []
+        q = 0
+        for s, n in shapes:
+            res.append(vocab.TopLogits(*(a[q:q + s * n].view(s, n, *a.shape[1:]) for a in top)))
+            q += s * n
         return res
 
     def encode(self, coords: np.ndarray, sources: np.ndarray):
