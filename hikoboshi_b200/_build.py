@@ -67,7 +67,38 @@ def build_library(verbose: bool = False) -> Path:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
     build_cli(verbose)
+    build_vocab_module(verbose)
     return LIB
+
+
+VOCAB_MODULE = PKG / "_vocab.so"
+
+
+def build_vocab_module(verbose: bool = False) -> Path:
+    """``hikoboshi_b200._vocab`` (csrc/torch_vocab.cpp): the torch binding of the
+    operators on vocabulary rows, linked to the in-tree library and to torch."""
+    import sysconfig
+
+    import torch
+    src = CSRC / "torch_vocab.cpp"
+    deps = [src, ROOT / "include" / "hkb_mpnn.h"]
+    # the library is linked by name: a rebuilt one needs no new module
+    if VOCAB_MODULE.exists() and VOCAB_MODULE.stat().st_mtime >= max(d.stat().st_mtime
+                                                                     for d in deps):
+        return VOCAB_MODULE
+    t = Path(torch.__file__).resolve().parent
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-I{ROOT / 'include'}", f"-isystem{t / 'include'}",
+           f"-isystem{t / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+           f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{CUDA_HOME / 'include'}",
+           str(src), "-o", str(VOCAB_MODULE), f"-L{PKG}", "-lhkb_mpnn", f"-L{t / 'lib'}",
+           "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return VOCAB_MODULE
 
 
 CLI = PKG / "bin" / "hikoboshi"

@@ -20,18 +20,18 @@ Unfit arguments raise :class:`HkbError` with ``HKB_INVALID_ARGUMENT``.
 """
 from __future__ import annotations
 
-from ctypes import byref
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import HkbError, check
 
-_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
-_FLOAT = (torch.float32,)
-_INT = (torch.int32,)
-_UNIFORMS = (torch.float32, torch.float64)
+_lib.load()  # the operators' library, which the module below calls
+try:
+    from . import _vocab
+except ImportError as e:
+    raise ImportError("hikoboshi_b200/_vocab.so is not built for this torch; run "
+                      "__graft_entry__.build() (or python hikoboshi_b200/_build.py)") from e
 
 
 class SampledTokens(NamedTuple):
@@ -44,99 +44,6 @@ class TopLogits(NamedTuple):
     values: torch.Tensor     # [.., k] in the logits' type, largest first
     tokens: torch.Tensor     # [.., k] i32
     log_norm: torch.Tensor   # [..] f32: log sum exp(x / temperature)
-
-
-def _invalid(why: str) -> HkbError:
-    return HkbError(_lib.HKB_INVALID_ARGUMENT, why)
-
-
-def _is_tensor(x, name: str) -> torch.Tensor:
-    if not isinstance(x, torch.Tensor):
-        raise _invalid(f"{name} must be a tensor")
-    return x
-
-
-def _rows(x: torch.Tensor, name: str = "logits"):
-    """(rows, leading shape) of [.., V] logits, as the library takes them; never
-    a copy."""
-    _is_tensor(x, name)
-    code = _DTYPES.get(x.dtype)
-    if code is None:
-        raise _invalid(f"{name} must be float32, float16 or bfloat16")
-    shape = x.shape
-    if len(shape) == 0 or shape[-1] == 0:
-        raise _invalid(f"{name} must have a last dimension of at least one token")
-    if x.layout is not torch.strided or x.is_neg():
-        raise _invalid(f"{name} must be a plain strided tensor")
-    v = shape[-1]
-    stride = x.stride()
-    if v > 1 and stride[-1] != 1:
-        raise _invalid(f"{name} must have a last dimension of stride 1")
-    if len(shape) == 2:
-        n, step = shape[0], stride[0]
-    else:
-        n, step = _flatten(shape[:-1], stride[:-1])
-        if step is None:
-            raise _invalid(f"{name}: the leading dimensions must flatten to rows of one stride")
-    return _lib.VocabRows(n, v if v < 2**31 else 2**31 - 1, code, x.data_ptr(),
-                          step if n > 1 else v), shape[:-1]
-
-
-def _flatten(shape, stride):
-    """(number, stride) of the dimensions taken as one, stride None if they
-    have no common one."""
-    n, step = 1, 0
-    for size, st in zip(reversed(shape), reversed(stride)):
-        if size == 1:
-            continue
-        if n == 1:
-            step = st
-        elif size and n and st != step * n:
-            step = None
-            break
-        n *= size
-    n = 1
-    for size in shape:
-        n *= size
-    return (n, step) if n else (0, 0)
-
-
-def _vector(x, lead, device, dtypes, name) -> torch.Tensor:
-    """A dense per-row tensor of the leading shape."""
-    _is_tensor(x, name)
-    if x.device != device:
-        raise _invalid(f"{name} must be on the logits' device")
-    if x.dtype not in dtypes:
-        raise _invalid(f"{name} must be " + " or ".join(str(d).split(".")[1] for d in dtypes))
-    if x.shape != lead:
-        raise _invalid(f"{name} must have one number per row")
-    if not x.is_contiguous() or x.is_neg():
-        raise _invalid(f"{name} must be contiguous")
-    return x
-
-
-# the current stream's handle without a Stream object around it
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda index: torch.cuda.current_stream(index).cuda_stream)
-
-
-def _call(fn, device: torch.device, *args) -> None:
-    if device.type == "cuda":
-        st = fn(device.index, *args, _raw_stream(device.index))
-        if st.code:
-            check(st)
-        return
-    # the library checks the other arguments first, then refuses the device
-    st = fn(-1, *args, None)
-    if st.code == _lib.HKB_INVALID_ARGUMENT and st.detail == b"device ordinal out of range":
-        raise _invalid("logits must be on a CUDA device")
-    check(st)
-
-
-def _number(v, name: str) -> float:
-    if isinstance(v, bool) or not isinstance(v, (int, float)):
-        raise _invalid(f"{name} must be a number or a tensor of one number per row")
-    return float(v)
 
 
 def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0,
@@ -156,36 +63,7 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0,
     give token -1, log_prob NaN and kept 0; rows with no logit above -inf give
     -1, -inf and 0.  A NaN logit counts as -inf.
     """
-    rows, lead = _rows(logits)
-    device = logits.device
-    u = _vector(uniforms, lead, device, _UNIFORMS, "uniforms")
-    s = _lib.SampleSettings()
-    s.uniforms = u.data_ptr()
-    s.uniforms_dtype = _lib.F64 if u.dtype == torch.float64 else _lib.F32
-    if isinstance(temperature, torch.Tensor):
-        s.temperatures = _vector(temperature, lead, device, _FLOAT, "temperature").data_ptr()
-    else:
-        s.temperature = _number(temperature, "temperature")
-    if isinstance(top_k, torch.Tensor):
-        s.top_ks = _vector(top_k, lead, device, _INT, "top_k").data_ptr()
-    elif isinstance(top_k, bool) or not isinstance(top_k, int):
-        raise _invalid("top_k must be a whole number or a tensor of one per row")
-    else:
-        s.top_k = max(-1, min(top_k, 2**31 - 1))
-    if isinstance(top_p, torch.Tensor):
-        s.top_ps = _vector(top_p, lead, device, _FLOAT, "top_p").data_ptr()
-    else:
-        s.top_p = _number(top_p, "top_p")
-    if isinstance(min_p, torch.Tensor):
-        s.min_ps = _vector(min_p, lead, device, _FLOAT, "min_p").data_ptr()
-    else:
-        s.min_p = _number(min_p, "min_p")
-    tokens = logits.new_empty(lead, dtype=torch.int32)
-    log_probs = logits.new_empty(lead, dtype=torch.float32)
-    kept = logits.new_empty(lead, dtype=torch.int32)
-    o = _lib.SampleOut(tokens.data_ptr(), log_probs.data_ptr(), kept.data_ptr())
-    _call(_lib.load().hkb_sample_tokens, device, byref(rows), byref(s), byref(o))
-    return SampledTokens(tokens, log_probs, kept)
+    return SampledTokens(*_vocab.sample(logits, uniforms, temperature, top_k, top_p, min_p))
 
 
 def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
@@ -193,97 +71,7 @@ def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
     tokens, in the order (logit down, index up), and log sum exp(x / temperature).
     Places past a row's logits above -inf hold (-inf, -1); a NaN logit counts
     as -inf."""
-    rows, lead = _rows(logits)
-    if isinstance(k, bool) or not isinstance(k, int):
-        raise _invalid("k must be a whole number")
-    k = max(-1, min(k, 2**31 - 1))
-    n = max(0, min(k, _lib.LISTING_MAX))
-    device = logits.device
-    values = logits.new_empty((*lead, n), dtype=logits.dtype)
-    tokens = logits.new_empty((*lead, n), dtype=torch.int32)
-    log_norm = logits.new_empty(lead, dtype=torch.float32)
-    o = _lib.TopOut(values.data_ptr(), tokens.data_ptr(), log_norm.data_ptr())
-    _call(_lib.load().hkb_top_logits, device, byref(rows), k,
-          _number(temperature, "temperature"), byref(o))
-    return TopLogits(values, tokens, log_norm)
-
-
-def _teacher(lead, device, values, tokens, log_norm, temperature) -> _lib.DistillTeacher:
-    _is_tensor(values, "teacher_values")
-    _is_tensor(tokens, "teacher_tokens")
-    code = _DTYPES.get(values.dtype)
-    if code is None:
-        raise _invalid("teacher_values must be float32, float16 or bfloat16")
-    if tokens.dtype is not torch.int32:
-        raise _invalid("teacher_tokens must be int32")
-    shape = values.shape
-    if len(shape) == 0 or shape[:-1] != lead or tokens.shape != shape:
-        raise _invalid("teacher_values and teacher_tokens must be [.., k] with the logits' rows")
-    if values.device != device:
-        raise _invalid("teacher_values must be on the logits' device")
-    if tokens.device != device:
-        raise _invalid("teacher_tokens must be on the logits' device")
-    if not values.is_contiguous() or not tokens.is_contiguous() or values.is_neg():
-        raise _invalid("teacher_values and teacher_tokens must be contiguous")
-    if log_norm is not None:
-        log_norm = _vector(log_norm, lead, device, _FLOAT, "teacher_log_norm").data_ptr()
-    return _lib.DistillTeacher(min(shape[-1], 2**31 - 1), code, values.data_ptr(),
-                               tokens.data_ptr(), log_norm, _number(temperature, "temperature"))
-
-
-def _weights(w, lead, device):
-    """(pointer, stride) of per-row weights: one stride, 0 where broadcast."""
-    if w is None:
-        return None, 0
-    _is_tensor(w, "row_weights")
-    if w.device != device:
-        raise _invalid("row_weights must be on the logits' device")
-    if w.dtype is not torch.float32:
-        raise _invalid("row_weights must be float32")
-    if w.shape != lead:
-        raise _invalid("row_weights must have one number per row")
-    _, step = _flatten(w.shape, w.stride())
-    if step is None or w.is_neg():
-        raise _invalid("row_weights must flatten to one stride")
-    return w.data_ptr(), step
-
-
-def _backward(logits, values, tokens, log_norm, temperature, grad_loss):
-    rows, lead = _rows(logits)
-    device = logits.device
-    t = _teacher(lead, device, values, tokens, log_norm, temperature)
-    grad = logits.new_empty(logits.shape)
-    if rows.rows:
-        _, step = _flatten(grad_loss.shape, grad_loss.stride())
-        if step is None or grad_loss.is_neg():
-            grad_loss = grad_loss.clone(memory_format=torch.contiguous_format).resolve_neg()
-        pointer, step = _weights(grad_loss, lead, device)
-        o = _lib.DistillOut(None, grad.data_ptr(), logits.shape[-1], pointer, step)
-        _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
-    return grad
-
-
-def _forward(logits, values, tokens, log_norm, temperature):
-    rows, lead = _rows(logits)
-    device = logits.device
-    t = _teacher(lead, device, values, tokens, log_norm, temperature)
-    loss = logits.new_empty(lead, dtype=torch.float32)
-    o = _lib.DistillOut(loss.data_ptr(), None, 0, None, 0)
-    _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
-    return loss
-
-
-class _DistillLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, values, tokens, log_norm, temperature):
-        ctx.save_for_backward(logits, values, tokens, log_norm)
-        ctx.temperature = temperature
-        return _forward(logits, values, tokens, log_norm, temperature)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_loss):
-        return _backward(*ctx.saved_tensors, ctx.temperature, grad_loss), None, None, None, None
+    return TopLogits(*_vocab.top(logits, k, temperature))
 
 
 def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=None,
@@ -305,15 +93,7 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     graph (an eager graph of the same leaves would break the capture): there
     it raises HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.
     """
-    if not (isinstance(logits, torch.Tensor) and logits.requires_grad
-            and torch.is_grad_enabled()):
-        return _forward(logits, teacher_values, teacher_tokens, teacher_log_norm, temperature)
-    if logits.is_cuda and torch.cuda.is_current_stream_capturing():
-        raise HkbError(_lib.HKB_FAILED_PRECONDITION,
-                       "autograd through distill_loss cannot be captured; capture "
-                       "distill_loss_and_grad")
-    return _DistillLoss.apply(logits, teacher_values, teacher_tokens, teacher_log_norm,
-                              temperature)
+    return _vocab.loss(logits, teacher_values, teacher_tokens, teacher_log_norm, temperature)
 
 
 def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log_norm=None,
@@ -323,24 +103,8 @@ def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log
     (weights 1 by default), in the logits' type.  A row of weight 0 has gradient
     0.  ``grad_out`` receives the gradient and may be ``logits`` itself, whose
     memory the gradient then takes; autograd does not see this call."""
-    rows, lead = _rows(logits)
-    device = logits.device
-    t = _teacher(lead, device, teacher_values, teacher_tokens, teacher_log_norm, temperature)
-    pointer, step = _weights(row_weights, lead, device)
-    if grad_out is None:
-        grad_out = logits.new_empty(logits.shape)
-        grad_stride = logits.shape[-1]
-    else:
-        _is_tensor(grad_out, "grad_out")
-        if grad_out.device != device:
-            raise _invalid("grad_out must be on the logits' device")
-        if grad_out.dtype is not logits.dtype or grad_out.shape != logits.shape:
-            raise _invalid("grad_out must have the logits' type and shape")
-        grad_stride = _rows(grad_out, "grad_out")[0].row_stride
-    loss = logits.new_empty(lead, dtype=torch.float32)
-    o = _lib.DistillOut(loss.data_ptr(), grad_out.data_ptr(), grad_stride, pointer, step)
-    _call(_lib.load().hkb_distill, device, byref(rows), byref(t), byref(o))
-    return loss, grad_out
+    return _vocab.loss_and_grad(logits, teacher_values, teacher_tokens, teacher_log_norm,
+                                temperature, row_weights, grad_out)
 
 
 __all__ = ["SampledTokens", "TopLogits", "distill_loss", "distill_loss_and_grad",
