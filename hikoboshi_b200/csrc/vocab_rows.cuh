@@ -254,6 +254,24 @@ struct RowSlice {
     for (int v = warp * per_warp + lane; v < end; v += 32)
       f(v * kE - ph + start, reinterpret_cast<Vec<T>*>(s)[v]);
   }
+  // f(x), x an array of kU vectors or of one, over this warp's vectors
+  template <int kU, typename F>
+  __device__ __forceinline__ void for_each_array(F f) const {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int end = min(nvec, (warp + 1) * per_warp);
+    const Vec<T>* vec = reinterpret_cast<const Vec<T>*>(s);
+    int v = warp * per_warp + lane;
+    for (; v + (kU - 1) * 32 < end; v += kU * 32) {
+      Vec<T> x[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) x[u] = vec[v + u * 32];
+      f(x);
+    }
+    for (; v < end; v += 32) {
+      Vec<T> x[1] = {vec[v]};
+      f(x);
+    }
+  }
 };
 
 // Reductions over the CTA and its cluster by a commutative operation; every
@@ -355,7 +373,7 @@ struct Reducer {
 constexpr int kListCap = 2048;
 struct TokenList {
   unsigned count;  // of this CTA's own items
-  unsigned long long item[kListCap];
+  alignas(16) unsigned long long item[kListCap];
 };
 __device__ __forceinline__ unsigned long long list_item(uint32_t key, int index) {
   return ((unsigned long long)key << 32) | (uint32_t)~index;
@@ -395,6 +413,25 @@ __device__ int collect(const RowSlice<T, kClustered>& row, Reducer<kClustered>& 
   }
   cg::this_cluster().sync();
   return total;
+}
+
+// Number of the first n items that are larger than `me`, as counted by every
+// `group`-th thread from `part` on: each takes its share of pairs, four loads at
+// a time.
+__device__ __forceinline__ int count_larger(const unsigned long long* item, int n,
+                                            unsigned long long me, int part, int group) {
+  const ulonglong2* pair = reinterpret_cast<const ulonglong2*>(item);
+  const int pairs = n / 2;
+  int c = 0, j = part;
+  for (; j + 3 * group < pairs; j += 4 * group) {
+    const ulonglong2 a = pair[j], b = pair[j + group], d = pair[j + 2 * group],
+                     e = pair[j + 3 * group];
+    c += (a.x > me) + (a.y > me) + (b.x > me) + (b.y > me) + (d.x > me) + (d.y > me) +
+         (e.x > me) + (e.y > me);
+  }
+  for (; j < pairs; j += group) c += (pair[j].x > me) + (pair[j].y > me);
+  if ((n & 1) && part == 0) c += item[n - 1] > me;
+  return c;
 }
 
 // Sorts n <= kListCap items downwards (bitonic; the CTA's threads).

@@ -671,7 +671,7 @@ __device__ __forceinline__ void finish_list(SampleSmem& sm, int n, const Weights
   unsigned long long me = 0;
   if (mine) {
     me = item[i];
-    for (int j = part; j < n; j += group) place += item[j] > me;
+    place = count_larger(item, n, me, part, group);
   }
   for (int o = group >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
   if (lead) {
@@ -697,8 +697,9 @@ __device__ __forceinline__ void finish_list(SampleSmem& sm, int n, const Weights
     me = sorted[i];
     own = weight[i];
     index = item_index(me);
+#pragma unroll 4
     for (int j = part; j < kept; j += group)
-      if (item_index(sorted[j]) <= index) upto += weight[j];
+      upto += item_index(sorted[j]) <= index ? weight[j] : 0.0;
   }
   for (int o = group >> 1; o > 0; o >>= 1) upto += __shfl_xor_sync(0xffffffffu, upto, o);
   int token = red.min(own > 0.0 && upto > target ? index : 0x7fffffff);
@@ -715,7 +716,6 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ SampleSmem sm;
-  constexpr int kE = Vec<T>::kN;
   const int cluster = kClustered ? (int)cg::this_cluster().num_blocks() : 1;
   const int64_t r = blockIdx.x / cluster;
   RowSlice<T, kClustered> row;
@@ -743,7 +743,11 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
   // Largest logit; a NaN is less than any number in this and every later
   // comparison, so it is never kept.
   float tmax = -CUDART_INF_F;
-  row.for_each([&](int, const Vec<T>& x) { tmax = fmaxf(tmax, x.largest()); });
+  row.template for_each_array<4>([&](auto& x) {
+    constexpr int n = sizeof(x) / sizeof(x[0]);
+#pragma unroll
+    for (int u = 0; u < n; ++u) tmax = fmaxf(tmax, x[u].largest());
+  });
   // of a row with top-k: a key that ceil(k / C) threads of this CTA reach
   if (s.top_k >= vocab) s.top_k = 0;
   const bool list_k = s.top_k > 0 && s.top_k <= kListCap / 2 && s.temperature > 0.0f;

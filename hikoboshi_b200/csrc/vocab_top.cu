@@ -11,6 +11,58 @@ namespace {
 
 constexpr float kLog2ef = 1.44269504f;
 
+// Writes row r's listing: the first k of the n items of the CTA's list in order.
+template <typename T>
+__device__ __forceinline__ void write_listing(TokenList& list, int n, const T* g, int64_t r,
+                                              const TopArgs& a) {
+  const int tid = threadIdx.x, threads = blockDim.x;
+  T* values = static_cast<T*>(a.values) + r * a.k;
+  int32_t* tokens = a.tokens + r * a.k;
+  auto put = [&](int place, int index) {
+    values[place] = g[index];
+    tokens[place] = index;
+  };
+  if (n <= 2 * threads) {
+    // an item's place is the number of larger ones, counted by a group of
+    // threads
+    int group = 32;
+    while (group > 1 && n * group > threads) group >>= 1;
+    for (int i0 = 0; i0 < n; i0 += threads / group) {
+      const int i = i0 + tid / group;
+      const unsigned long long me = i < n ? list.item[i] : 0ull;
+      int place = i < n ? count_larger(list.item, n, me, tid % group, group) : 0;
+      for (int o = group >> 1; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+      if (i < n && tid % group == 0 && place < a.k) put(place, item_index(me));
+    }
+  } else {
+    sort_down(list.item, n);
+    for (int i = tid; i < n && i < a.k; i += threads) put(i, item_index(list.item[i]));
+  }
+  for (int i = n + tid; i < a.k; i += threads) {
+    values[i] = narrow<T>(-CUDART_INF_F);
+    tokens[i] = -1;
+  }
+}
+
+// What the CTAs of a row find together: its largest logit and sum, and the least
+// of the keys that enough of their threads reach.
+struct RowTop {
+  SoftSum soft;
+  uint32_t reached;
+};
+
+}  // namespace
+
+template <>
+__device__ __forceinline__ RowTop shfl_xor(RowTop v, int o) {
+  RowTop r;
+  r.soft = shfl_xor(v.soft, o);
+  r.reached = __shfl_xor_sync(0xffffffffu, v.reached, o);
+  return r;
+}
+
+namespace {
+
 struct TopSmem {
   ReduceScratch red;
   TokenList list;
@@ -22,7 +74,6 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
                                                                int chunk, TopArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ TopSmem sm;
-  constexpr int kE = Vec<T>::kN;
   const int cluster = kClustered ? (int)cg::this_cluster().num_blocks() : 1;
   const int64_t r = blockIdx.x / cluster;
   RowSlice<T, kClustered> row;
@@ -34,84 +85,68 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   else __syncthreads();
   Reducer<kClustered> red(&sm.red);
 
+  const float c = kLog2ef / a.temperature;
+  RowTop mine;
   float tmax = -CUDART_INF_F;
-  row.for_each([&](int, Vec<T>& x) {
+  row.template for_each_array<2>([&](auto& x) {
+    constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
-    for (int e = 0; e < kE; ++e) {
-      const float v = x.at(e);
-      if (v != v) x.clear(e);
-      tmax = fmaxf(tmax, v);
-    }
+    for (int u = 0; u < n; ++u) tmax = fmaxf(tmax, x[u].largest());
+    if (a.log_norm) mine.soft.add(x, c);
   });
-  const float xmax = red.max(tmax);
-  if (a.log_norm) {
-    const float c = kLog2ef / a.temperature;
-    float s = 0.0f;
-    row.for_each([&](int, const Vec<T>& x) {
-#pragma unroll
-      for (int e = 0; e < kE; ++e) {
-        const float v = x.at(e);
-        s += exp2_fast((v == xmax ? 0.0f : v - xmax) * c);
-      }
+  mine.soft.m = tmax;
+  if (a.log_norm && mine.soft.s != mine.soft.s) {
+    // a NaN or +inf among the thread's logits: again, without the NaN (with a
+    // +inf the sum is not used)
+    mine.soft.s = 0.0f;
+    row.for_each_from(-CUDART_MAX_NORMAL_F, [&](int, float y) {
+      if (y > -CUDART_INF_F) mine.soft.s += exp2_fast((y == tmax ? 0.0f : y - tmax) * c);
     });
-    const double total = red.sum((double)s);
-    if (threadIdx.x == 0 && row.rank == 0)
-      a.log_norm[r] = xmax == -CUDART_INF_F
-                          ? xmax
-                          : (float)((double)xmax / (double)a.temperature + log(total));
   }
   // The k-th largest of the row is no less than the k/C-th largest of the
   // threads' own largest logits in the CTA where that is least; few more than
   // k tokens reach it.
-  const uint32_t mine = reached_by(order_key(tmax), (a.k + row.size - 1) / row.size);
-  const uint32_t bound = ~red.max(~mine);
+  mine.reached = reached_by(order_key(tmax), (a.k + row.size - 1) / row.size);
+  mine = red.all(mine, [c](RowTop p, RowTop q) {
+    RowTop t;
+    t.soft = SoftSum::join(p.soft, q.soft, c);
+    t.reached = ::min(p.reached, q.reached);
+    return t;
+  });
+  const float xmax = mine.soft.m;
+  if (a.log_norm && threadIdx.x == 0 && row.rank == 0)
+    a.log_norm[r] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
+                        ? xmax
+                        : (float)((double)xmax / (double)a.temperature + log((double)mine.soft.s));
+  const uint32_t bound = mine.reached;
   const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
   int n = collect(row, red, sm.list, from, [&](int, float x) { return x >= from; });
   if (n > kListCap) {
     // many equal logits, or a row whose large logits lie side by side: the
     // k-th largest key by bisection, and the last index taken of its tokens
-    uint32_t t = kKeyNegInf + 1;
-    int icut = 0x7fffffff;
-    auto count = [&](uint32_t lo, int last) {
+    auto count = [&](float from, int last) {
       int c = 0;
-      row.for_each([&](int i0, const Vec<T>& x) {
-#pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const uint32_t k = order_key(x.at(e));
-          c += k > lo || (k == lo && i0 + e <= last);
-        }
-      });
+      row.for_each_from(from, [&](int i, float x) { c += x > from || (x == from && i <= last); });
       return red.sum(c);
     };
-    uint32_t lo = t, hi = order_key(xmax);
+    uint32_t lo = kKeyNegInf + 1, hi = order_key(xmax);
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      if (count(mid, 0x7fffffff) >= a.k) lo = mid;
+      if (count(key_value(mid), 0x7fffffff) >= a.k) lo = mid;
       else hi = mid - 1;
     }
-    t = lo;
+    const float t = key_value(lo);
     int i_lo = 0, i_hi = vocab - 1;
     while (i_lo < i_hi) {
       const int mid = (i_lo + i_hi) / 2;
       if (count(t, mid) >= a.k) i_hi = mid;
       else i_lo = mid + 1;
     }
-    icut = i_lo;
-    n = collect(row, red, sm.list, key_value(t), [&](int i, float x) {
-      const uint32_t k = order_key(x);
-      return k > t || (k == t && i <= icut);
+    n = collect(row, red, sm.list, t, [&](int i, float x) {
+      return x > t || (x == t && i <= i_lo);
     });
   }
-  if (row.rank != 0) return;
-  sort_down(sm.list.item, n);
-  T* values = static_cast<T*>(a.values) + r * a.k;
-  int32_t* tokens = a.tokens + r * a.k;
-  for (int i = threadIdx.x; i < a.k; i += blockDim.x) {
-    const bool there = i < n;
-    const int index = there ? item_index(sm.list.item[i]) : -1;
-    values[i] = there ? g[index] : narrow<T>(-CUDART_INF_F);
-    tokens[i] = index;
-  }
+  if (row.rank == 0) write_listing(sm.list, n, g, r, a);
 }
 
 // Many rows: a CTA streams a row for its maxima and sum, then again to collect
@@ -242,34 +277,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* 
     __syncthreads();
     n = a.k;
   }
-  T* values = static_cast<T*>(a.values) + r * a.k;
-  int32_t* tokens = a.tokens + r * a.k;
-  if (n <= 2 * threads) {
-    // an item's place is the number of larger ones
-    for (int i = tid; i < n; i += threads) {
-      const unsigned long long me = sm.list.item[i];
-      int place = 0;
-#pragma unroll 8
-      for (int j = 0; j < n; ++j) place += sm.list.item[j] > me;
-      if (place < a.k) {
-        const int index = item_index(me);
-        values[place] = g[index];
-        tokens[place] = index;
-      }
-    }
-    for (int i = n + tid; i < a.k; i += threads) {
-      values[i] = narrow<T>(-CUDART_INF_F);
-      tokens[i] = -1;
-    }
-    return;
-  }
-  sort_down(sm.list.item, n);
-  for (int i = tid; i < a.k; i += threads) {
-    const bool there = i < n;
-    const int index = there ? item_index(sm.list.item[i]) : -1;
-    values[i] = there ? g[index] : narrow<T>(-CUDART_INF_F);
-    tokens[i] = index;
-  }
+  write_listing(sm.list, n, g, r, a);
 }
 
 // Rows of up to kWarpVocab tokens, a warp each.  A short listing takes the
