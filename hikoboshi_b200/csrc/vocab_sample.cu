@@ -782,7 +782,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     // ones far below and, by the factor of the exponents, without weight.
     row.for_each([&](int, Vec<T>& x) {
 #pragma unroll
-      for (int e = 0; e < kE; ++e) {
+      for (int e = 0; e < Vec<T>::kN; ++e) {
         const float v = x.at(e);
         if (v > -CUDART_INF_F)
           reinterpret_cast<T*>(x.w)[e] = narrow<T>(v == CUDART_INF_F ? 0.0f : -60000.0f);
