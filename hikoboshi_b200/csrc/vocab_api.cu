@@ -137,8 +137,8 @@ hkb_status hkb_top_logits(int device, const hkb_vocab_rows* rows, int32_t k, flo
   if (st.code != HKB_OK) return st;
   if (out == nullptr) return invalid("output must be non-null");
   if (k < 1 || k > HKB_LISTING_MAX) return invalid("k must be 1 to HKB_LISTING_MAX");
-  if (!(std::isfinite(temperature) && temperature > 0.0f))
-    return invalid("temperature must be finite and > 0");
+  if (!(temperature >= HKB_TEMPERATURE_MIN && temperature <= HKB_TEMPERATURE_MAX))
+    return invalid("temperature must be 1e-30 to 1e30");
   if (rows->rows == 0) return {HKB_OK, ""};
   if (out->values == nullptr || out->tokens == nullptr)
     return invalid("values and tokens must be non-null");
@@ -161,8 +161,8 @@ hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill
   if (t->k < 1 || t->k > HKB_LISTING_MAX)
     return invalid("a row's listing must have 1 to HKB_LISTING_MAX entries");
   if (!real_dtype(t->dtype)) return invalid("teacher values must be F32, F16 or BF16");
-  if (!(std::isfinite(t->temperature) && t->temperature > 0.0f))
-    return invalid("temperature must be finite and > 0");
+  if (!(t->temperature >= HKB_TEMPERATURE_MIN && t->temperature <= HKB_TEMPERATURE_MAX))
+    return invalid("temperature must be 1e-30 to 1e30");
   if (out->row_weight_stride < 0) return invalid("the row weight stride must not be negative");
   if (out->grad != nullptr) {
     if (out->grad_row_stride < rows->vocab)

@@ -197,6 +197,15 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
       twice = true;
     }
   const bool row_twice = __syncthreads_or(twice);
+  if (row_twice)
+    // the first of a token's entries stands for it, so that sums over the
+    // entries do not change from run to run
+    for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
+      if (ls.own[k] == 0) continue;
+      int first = 0;
+      while (ls.token[first] != ls.token[k]) ++first;
+      ls.own[k] = first == k ? 1 : -1;
+    }
   for (int k = threadIdx.x; k < a.k; k += blockDim.x)
     if (ls.own[k] > 0)
       row.s[row.ph + ls.token[k] - row.start] = narrow<T>(tail ? -CUDART_INF_F : ls.x[k]);
@@ -306,6 +315,16 @@ __device__ __forceinline__ EntrySums shfl_xor(EntrySums v, int o) {
 
 namespace {
 
+// Of the entries of one token the first stands for it.
+__device__ __forceinline__ void own_first(const Listing& ls, int k_all) {
+  for (int k = threadIdx.x; k < k_all; k += blockDim.x) {
+    if (ls.token[k] < 0) continue;
+    int first = 0;
+    while (ls.token[first] != ls.token[k]) ++first;
+    ls.own[k] = first == k;
+  }
+}
+
 struct StreamSmem {
   ReduceScratch red;
   Exp2Table table;
@@ -374,16 +393,21 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
   }
   amax = key_value((uint32_t)(head >> 32));
   EntrySums sums{0.0, 0.0, 0.0, 0};
+  bool twice_here = false;
   if (marked) {
     for (int k = tid; k < a.k; k += threads) {
       const int token = ls.token[k];
       if (token < 0) continue;
       const int bit = token + row.ph;
       const int own = !(atomicOr(&marks[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1u);
-      sums.twice |= !own;
+      twice_here |= !own;
       ls.own[k] = own;
     }
-    if (tail) __syncthreads();  // the marks are read
+    sums.twice = twice_here;
+    // The marks are read in the first pass.  Of a token's entries any may stand
+    // for it where only its gradient is written; in a sum it is the first, so
+    // that the sum does not change from run to run.
+    if (tail && __syncthreads_or(twice_here)) own_first(ls, a.k);
   }
 
   const double inv_tau = 1.0 / (double)a.temperature;

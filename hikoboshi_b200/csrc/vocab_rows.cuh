@@ -382,9 +382,8 @@ __device__ __forceinline__ uint32_t item_key(unsigned long long it) { return (ui
 __device__ __forceinline__ int item_index(unsigned long long it) { return (int)~(uint32_t)it; }
 
 // Collects the row's elements for which pick(index, value) holds, none of them
-// below `skip`.  Returns
-// their number; if it is at most kListCap, rank 0's list holds them all, in no
-// particular order, else the lists are of no use.
+// below `skip`.  Returns their number; if it is at most kListCap, rank 0's list
+// holds them all, in no particular order, else the lists are of no use.
 template <typename T, bool kClustered, typename F>
 __device__ int collect(const RowSlice<T, kClustered>& row, Reducer<kClustered>& red,
                        TokenList& list, float skip, F pick) {

@@ -92,8 +92,22 @@ struct Extent {
   float most, least;
 };
 
+// The same of list items, with their weights' sum in multiples of 2^-52.
+struct ListExtent {
+  unsigned long long sum;
+  float most, least;
+};
+
 }  // namespace
 
+template <>
+__device__ __forceinline__ ListExtent shfl_xor(ListExtent v, int o) {
+  ListExtent r;
+  r.sum = __shfl_xor_sync(0xffffffffu, v.sum, o);
+  r.most = __shfl_xor_sync(0xffffffffu, v.most, o);
+  r.least = __shfl_xor_sync(0xffffffffu, v.least, o);
+  return r;
+}
 template <>
 __device__ __forceinline__ Extent shfl_xor(Extent v, int o) {
   Extent r;
@@ -105,6 +119,12 @@ __device__ __forceinline__ Extent shfl_xor(Extent v, int o) {
 
 namespace {
 
+__device__ __forceinline__ ListExtent join(Reducer<false>& red, ListExtent v) {
+  return red.all(v, [](ListExtent p, ListExtent q) {
+    return ListExtent{p.sum + q.sum, fmaxf(p.most, q.most), fminf(p.least, q.least)};
+  });
+}
+
 struct SampleSmem {
   Bounds bounds[kMaxWarps];
   ReduceScratch red;
@@ -113,7 +133,7 @@ struct SampleSmem {
   int number[kMaxWarps];
   unsigned sub_count;
   unsigned long long sub[kSubList];
-  double sub_weight[kSubList];
+  unsigned long long sub_weight[kSubList];
   double step[32];  // a warp owns at most 17 steps of 32 vectors
   double total;
   Exp2Table table;
@@ -341,6 +361,14 @@ __device__ __forceinline__ Bracket bracket(SampleSmem& sm, float scale, const We
           (int)(uint32_t)both.y};
 }
 
+// Sums over the list are in whole multiples of 2^-52, as the list's own order
+// changes from run to run and must not change the sums: at most 2^11 weights of
+// at most 1 fit 64 bits, and lose 2^-42 in all.
+constexpr double kFixedOne = 4503599627370496.0;
+__device__ __forceinline__ unsigned long long fixed_weight(double w) {
+  return __double2ull_rn(w * kFixedOne);
+}
+
 // Three counts of up to kListCap in one word.
 __device__ __forceinline__ unsigned long long three_counts(bool a, bool b, bool c) {
   return (a ? 1ull : 0ull) | (b ? 1ull << 20 : 0ull) | (c ? 1ull << 40 : 0ull);
@@ -376,52 +404,54 @@ __device__ __forceinline__ int nth_index(SampleSmem& sm, int n, uint32_t key, in
 // mass, `above` before the first, reaches `need`; 0 if none does.  The bins of
 // the row's search again, now of the list's own span, leave a few items; each
 // of these adds up what comes before it.
-__device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int n, const Weights wt,
-                                                          double above, double need) {
+__device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int n,
+                                                             const Weights wt, double above,
+                                                             double need) {
   Reducer<false> red(&sm.block);
   const int tid = threadIdx.x, threads = blockDim.x;
   const unsigned long long* item = sm.list.item;
+  auto weight = [&](float x) { return fixed_weight(wt.weight(x)); };
+  const double goal = (need - above) * kFixedOne;  // for the list's own sums
+  unsigned long long sum = 0;                      // of its items before xhi
   float xhi = CUDART_INF_F, xlo = -CUDART_INF_F;
   int left = n;
   for (int round = 0; left > kSubList; ++round) {
     // span of the items that are left
-    Extent ext{0.0, -CUDART_INF_F, CUDART_INF_F};
+    ListExtent ext{0, -CUDART_INF_F, CUDART_INF_F};
     for (int i = tid; i < n; i += threads) {
       const float x = key_value(item_key(item[i]));
       if (x > xhi || x < xlo) continue;
       ext.most = fmaxf(ext.most, x);
       ext.least = fminf(ext.least, x);
     }
-    ext = red.all(ext, [](Extent p, Extent q) {
-      return Extent{0.0, fmaxf(p.most, q.most), fminf(p.least, q.least)};
-    });
+    ext = join(red, ext);
     xhi = ext.most;
     xlo = ext.least;
     const float scale = (float)kBins / (xhi - xlo);
     if (xlo < xhi && (!(scale > 0.0f && scale < CUDART_INF_F) || round == 16)) {
       // no width of bins tells them apart (spans near the type's smallest
       // numbers): the border's key by bisection
-      auto mass_from = [&](uint32_t key) {
-        double m = 0.0;
+      auto sum_from = [&](uint32_t key) {
+        unsigned long long m = 0;
         for (int i = tid; i < n; i += threads) {
           const uint32_t k = item_key(item[i]);
-          if (k >= key && key_value(k) <= xhi) m += wt.weight(key_value(k));
+          if (k >= key && key_value(k) <= xhi) m += weight(key_value(k));
         }
         return red.sum(m);
       };
       uint32_t lo = order_key(xlo), hi = order_key(xhi);
       while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
-        if (above + mass_from(mid) >= need) lo = mid;
+        if ((double)(sum + sum_from(mid)) >= goal) lo = mid;
         else hi = mid - 1;
       }
-      if (key_value(lo) < xhi) above += mass_from(lo + 1);
+      if (key_value(lo) < xhi) sum += sum_from(lo + 1);
       xhi = xlo = key_value(lo);
     }
     if (xlo == xhi) {
       // equal logits: by their number
-      const double w = wt.weight(xhi);
-      const double ties = w > 0.0 ? fmax(1.0, ceil((need - above) / w)) : 1.0;
+      const double w = (double)weight(xhi);
+      const double ties = w > 0.0 ? fmax(1.0, ceil((goal - (double)sum) / w)) : 1.0;
       if (ties > (double)left) return 0;
       __syncthreads();
       return list_item(order_key(xhi), nth_index(sm, n, order_key(xhi), (int)ties));
@@ -434,29 +464,27 @@ __device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int
       if (x <= xhi && x >= xlo) atomicAdd(&sm.hist[bin_of(x)], 1u);
     }
     __syncthreads();
-    const Bracket br =
-        bracket(sm, scale, wt, xhi, need - above, [&](int b) { return (int)sm.hist[b]; });
-    ext = Extent{0.0, -CUDART_INF_F, CUDART_INF_F};
+    const Bracket br = bracket(sm, scale, wt, xhi, (goal - (double)sum) / kFixedOne,
+                               [&](int b) { return (int)sm.hist[b]; });
+    ext = ListExtent{0, -CUDART_INF_F, CUDART_INF_F};
     for (int i = tid; i < n; i += threads) {
       const float x = key_value(item_key(item[i]));
       if (x > xhi || x < xlo) continue;
       const int b = bin_of(x);
       if (b <= br.certain) {
-        ext.mass += wt.weight(x);
+        ext.sum += weight(x);
       } else if (b <= br.end) {
         ext.most = fmaxf(ext.most, x);
         ext.least = fminf(ext.least, x);
       }
     }
-    ext = red.all(ext, [](Extent p, Extent q) {
-      return Extent{p.mass + q.mass, fmaxf(p.most, q.most), fminf(p.least, q.least)};
-    });
-    above += ext.mass;
+    ext = join(red, ext);
+    sum += ext.sum;
     left = br.upto_end - br.upto_certain;
     xhi = ext.most;
     xlo = ext.least;
   }
-  // the items that are left, and the running mass at each of them
+  // the items that are left, and the running sum at each of them
   if (tid == 0) sm.sub_count = 0;
   __syncthreads();
   for (int i = tid; i < n; i += threads) {
@@ -464,16 +492,16 @@ __device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int
     if (x > xhi || x < xlo) continue;
     const unsigned at = atomicAdd(&sm.sub_count, 1u);
     sm.sub[at] = item[i];
-    sm.sub_weight[at] = wt.weight(x);
+    sm.sub_weight[at] = weight(x);
   }
   __syncthreads();
   unsigned long long border = 0;
   if (tid < left) {
     const unsigned long long me = sm.sub[tid];
-    double run = above;
+    unsigned long long run = sum;
 #pragma unroll 4
-    for (int j = 0; j < left; ++j) run += sm.sub[j] >= me ? sm.sub_weight[j] : 0.0;
-    if (run >= need) border = me;
+    for (int j = 0; j < left; ++j) run += sm.sub[j] >= me ? sm.sub_weight[j] : 0ull;
+    if ((double)run >= goal) border = me;
   }
   return red.max(border);
 }
@@ -482,7 +510,7 @@ __device__ __forceinline__ unsigned long long border_in_list(SampleSmem& sm, int
 constexpr int kOwnItems = 8;  // kListCap items over at least 256 threads
 
 struct Three {
-  double v[3];
+  unsigned long long v[3];
 };
 
 }  // namespace
@@ -500,7 +528,7 @@ namespace {
 struct OwnItems {
   uint32_t key[kOwnItems];
   int index[kOwnItems];
-  double w[kOwnItems];  // 0 where the thread has no item
+  unsigned long long w[kOwnItems];  // 0 where the thread has no item
   bool has[kOwnItems];
 
   __device__ __forceinline__ void read(const SampleSmem& sm, int n, const Weights wt) {
@@ -510,12 +538,12 @@ struct OwnItems {
       has[j] = i < n;
       key[j] = 0;
       index[j] = 0x7fffffff;
-      w[j] = 0.0;
+      w[j] = 0;
       if (has[j]) {
         const unsigned long long it = sm.list.item[i];
         key[j] = item_key(it);
         index[j] = item_index(it);
-        w[j] = wt.weight(key_value(key[j]));
+        w[j] = fixed_weight(wt.weight(key_value(key[j])));
       }
     }
   }
@@ -523,13 +551,13 @@ struct OwnItems {
   // once: the barrier is the same.
   template <typename In, typename F>
   __device__ __forceinline__ Three sums(Reducer<false>& red, In in, F f) const {
-    Three t{{0.0, 0.0, 0.0}};
+    Three t{{0, 0, 0}};
 #pragma unroll
     for (int j = 0; j < kOwnItems; ++j)
       if (has[j]) {
-        const double v = f(j);
+        const unsigned long long v = f(j);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) t.v[i] += in(j, i) ? v : 0.0;
+        for (int i = 0; i < 3; ++i) t.v[i] += in(j, i) ? v : 0ull;
       }
     return red.all(t, [](Three p, Three q) {
       return Three{{p.v[0] + q.v[0], p.v[1] + q.v[1], p.v[2] + q.v[2]}};
@@ -591,10 +619,10 @@ __device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const We
   if (s.top_k > 0 && n > s.top_k) cut(nth_item(sm, n, s.top_k));
   if (s.top_p < 1.0f) {
     if (need < 0.0) {
-      double mass = 0.0;
+      unsigned long long mass = 0;
       for (int i = threadIdx.x; i < n; i += blockDim.x)
-        mass += wt.weight(key_value(item_key(sm.list.item[i])));
-      need = (double)s.top_p * red.sum(mass);
+        mass += fixed_weight(wt.weight(key_value(item_key(sm.list.item[i]))));
+      need = (double)s.top_p * ((double)red.sum(mass) / kFixedOne);
       __syncthreads();
     }
     const unsigned long long border = border_in_list(sm, n, wt, 0.0, fmax(need, 1e-300));
@@ -607,18 +635,18 @@ __device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const We
   int kept = 0;
 #pragma unroll
   for (int j = 0; j < kOwnItems; ++j) {
-    own.has[j] = own.has[j] && own.w[j] >= (double)s.min_p;
+    own.has[j] = own.has[j] && wt.weight(key_value(own.key[j])) >= (double)s.min_p;
     kept += own.has[j];
   }
   kept = red.sum(kept);
-  const double total = own.sums(red, [](int, int) { return true; }, weight).v[0];
+  const double total = (double)own.sums(red, [](int, int) { return true; }, weight).v[0];
   const double target = s.u * total;
   // smallest index up to which the mass exceeds the target (rounding, or u = 1,
   // may leave none: the last with any)
   int from = 0x7fffffff, to = -1;
 #pragma unroll
   for (int j = 0; j < kOwnItems; ++j)
-    if (own.has[j] && own.w[j] > 0.0) {
+    if (own.has[j] && own.w[j] != 0) {
       from = ::min(from, own.index[j]);
       to = ::max(to, own.index[j]);
     }
@@ -631,17 +659,17 @@ __device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const We
     int k = 3;
 #pragma unroll
     for (int i = 2; i >= 0; --i)
-      if (t.v[i] > target) k = i;
+      if ((double)t.v[i] > target) k = i;
     const int end = ::min(to, from + step * (k + 1) - 1);
-    from += step * k;
+    from = ::min(from + step * k, to);
     if (k < 3) to = end;
-    else from = ::min(from, to);
   }
 #pragma unroll
   for (int j = 0; j < kOwnItems; ++j)
     if (own.has[j] && own.index[j] == from) {
       a.tokens[r] = from;
-      a.log_probs[r] = (float)(wt.exponent(key_value(own.key[j])) * kLn2 - log(total));
+      a.log_probs[r] =
+          (float)(wt.exponent(key_value(own.key[j])) * kLn2 - log(total / kFixedOne));
       a.kept[r] = kept;
     }
 }

@@ -70,7 +70,7 @@ def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
     """The ``k`` largest logits of each row of ``logits`` [.., V] with their
     tokens, in the order (logit down, index up), and log sum exp(x / temperature).
     Places past a row's logits above -inf hold (-inf, -1); a NaN logit counts
-    as -inf."""
+    as -inf.  ``temperature`` is 1e-30 to 1e30."""
     return TopLogits(*_vocab.top(logits, k, temperature))
 
 
@@ -86,9 +86,9 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     their true masses and all others form one class with what is left, against
     the student's mass outside the list.  A negative token or a value of -inf is
     no entry; a row without entries has loss and gradient 0 whatever its logits.
-    A token >= V makes its row NaN.
+    A token >= V makes its row NaN.  ``temperature`` is 1e-30 to 1e30.
 
-    The backward pass reads ``logits`` again, so they must not be overwritten
+    The loss is differentiable once.  The backward pass reads ``logits`` again, so they must not be overwritten
     before it.  Autograd through this call cannot be captured into a CUDA
     graph (an eager graph of the same leaves would break the capture): there
     it raises HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.

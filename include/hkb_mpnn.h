@@ -287,6 +287,9 @@ hkb_status hkb_write_logprobs_npz(const char* path, int32_t num_seqs, int32_t re
 #define HKB_VOCAB_MAX 262144
 #define HKB_VOCAB_ROWS_MAX 134217728
 #define HKB_LISTING_MAX 1024
+/* of log-norms and of distillation */
+#define HKB_TEMPERATURE_MIN 1e-30f
+#define HKB_TEMPERATURE_MAX 1e30f
 
 typedef enum { HKB_F32 = 0, HKB_F16 = 1, HKB_BF16 = 2, HKB_F64 = 3 } hkb_dtype;
 
@@ -345,7 +348,7 @@ typedef struct {
 /* The k largest logits of each row with their tokens, in the order (logit
  * down, index up): what a teacher stores of its answer.  k is 1 to
  * HKB_LISTING_MAX; places past the row's logits above -inf hold (-inf, -1).  A
- * NaN logit counts as -inf.  temperature (finite, > 0) only scales log_norm,
+ * NaN logit counts as -inf.  temperature (1e-30 to 1e30) only scales log_norm,
  * which is -inf for a row with no logit above -inf. */
 hkb_status hkb_top_logits(int device, const hkb_vocab_rows* rows, int32_t k, float temperature,
                           const hkb_top_out* out, void* stream);
@@ -357,7 +360,7 @@ typedef struct {
   const int32_t* tokens; /* [N,k]; negative = no entry, as is a value of -inf */
   const float* log_norm; /* [N] teacher's log sum exp(a / temperature) over its
                             whole row, or NULL */
-  float temperature;     /* finite, > 0 */
+  float temperature;     /* 1e-30 to 1e30 */
 } hkb_distill_teacher;
 
 typedef struct {

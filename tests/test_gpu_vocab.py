@@ -694,3 +694,40 @@ def test_extreme_temperatures(vocab):
         for t in (1e-45, 1e-38, 1e-20, 1e20, 1e30, 3e38):
             for f in (dict(), dict(top_p=0.7), dict(top_k=5), dict(min_p=0.5), dict(top_p=0.3, top_k=9)):
                 check_sample(vocab.sample_tokens(x, u, temperature=t, **f), x, u, temperature=t, **f)
+
+
+@pytest.mark.parametrize("size", [2500, 60000])
+def test_sampling_repeats_bit_for_bit_at_exact_borders(vocab, size):
+    # rows that repeat themselves put borders exactly on u and p: whichever side
+    # they fall, they fall the same way every time
+    block = logits(1, size // 50, F32, 5)
+    x = block.repeat(1, 50).expand(8, size).contiguous()
+    x[4:] = (x[4:] * 4).round() / 4
+    u = torch.tensor([0.1, 0.25, 0.5, 0.98] * 2, device="cuda")
+    for f in (dict(), dict(top_p=0.5), dict(top_p=0.25, top_k=1000), dict(top_k=900),
+              dict(top_p=0.75, temperature=2.0)):
+        want = vocab.sample_tokens(x, u, **f)
+        for _ in range(10):
+            got = vocab.sample_tokens(x, u, **f)
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), f
+
+
+def test_loss_is_differentiable_once(vocab):
+    x = logits(4, 50, F32, 1).requires_grad_()
+    v, t, _ = teacher(x.detach(), 3, F32, 1, 1.0, False)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(vocab.distill_loss(x, v, t).sum(), x, create_graph=True)
+
+
+def test_extreme_distill_temperatures(vocab):
+    for size in (21, 500, 30000):
+        for rows in (3, 160):
+            x = logits(rows, size, F32, 1)
+            for tau in (1e-3, 1e4):
+                v, t, norm = teacher(x, 5, F32, 2, tau, True)
+                for n in (None, norm):
+                    loss, grad = vocab.distill_loss_and_grad(x, v, t, teacher_log_norm=n,
+                                                             temperature=tau)
+                    check_distill(loss[:3], grad[:3], x[:3], v[:3], t[:3],
+                                  None if n is None else n[:3], tau)
+                check_top([a[:3] for a in vocab.top_logits(x, 5, temperature=tau)], x[:3], 5, tau)

@@ -57,7 +57,7 @@ def test_top_is_checked():
     for k, text in ((0, "k must be 1"), (-3, "k must be 1"), (1025, "HKB_LISTING_MAX"),
                     (2**40, "HKB_LISTING_MAX"), (2.0, "whole number")):
         refused(lambda: vocab.top_logits(X, k), text)
-    for t in (0.0, -1.0, float("inf"), float("nan")):
+    for t in (0.0, -1.0, 1e-31, 1e31, float("inf"), float("nan")):
         refused(lambda: vocab.top_logits(X, 3, temperature=t), "temperature")
 
 
@@ -68,6 +68,7 @@ def test_top_is_checked():
     (dict(teacher_log_norm=torch.zeros(2)), "one number per row"),
     (dict(teacher_log_norm=U.double()), "float32"),
     (dict(temperature=0.0), "temperature"), (dict(temperature=float("nan")), "temperature"),
+    (dict(temperature=1e-31), "temperature"), (dict(temperature=1e31), "temperature"),
     (dict(values=torch.zeros(3, 0), tokens=TT[:, :0]), "HKB_LISTING_MAX"),
     (dict(values=torch.zeros(3, 1025), tokens=torch.zeros(3, 1025, dtype=torch.int32)),
      "HKB_LISTING_MAX"),
