@@ -34,7 +34,8 @@ cudaError_t launch_sample_tokens(cudaStream_t st, const VocabRows& r, const Samp
 
 struct TopArgs {
   int k;
-  float temperature;
+  double inv_temperature;
+  float c;           // log2(e) / temperature
   void* values;      // [N,k], the logits' type
   int32_t* tokens;   // [N,k]
   float* log_norm;   // [N] or null
@@ -47,7 +48,8 @@ struct DistillArgs {
   const void* values;    // [N,k]
   const int32_t* tokens; // [N,k]
   const float* log_norm; // [N] or null
-  float temperature;
+  double temperature, inv_temperature;
+  float c;               // log2(e) / temperature
   float* loss;           // [N] or null
   void* grad;            // [N, vocab] or null
   int64_t grad_row_stride;

@@ -65,6 +65,8 @@ hkb_status launched(cudaError_t e) {
   return {HKB_INTERNAL_ERROR, cudaGetErrorString(e)};
 }
 
+constexpr double kLog2e = 1.4426950408889634074;
+
 bool real_dtype(int d) { return d == HKB_F32 || d == HKB_F16 || d == HKB_BF16; }
 uintptr_t elem_bytes(int d) { return d == HKB_F32 ? 4 : 2; }
 
@@ -146,7 +148,8 @@ hkb_status hkb_top_logits(int device, const hkb_vocab_rows* rows, int32_t k, flo
   if (guard.status().code != HKB_OK) return guard.status();
   TopArgs a{};
   a.k = k;
-  a.temperature = temperature;
+  a.inv_temperature = 1.0 / (double)temperature;
+  a.c = (float)(kLog2e * a.inv_temperature);
   a.values = out->values;
   a.tokens = out->tokens;
   a.log_norm = out->log_norm;
@@ -193,7 +196,9 @@ hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill
   a.values = t->values;
   a.tokens = t->tokens;
   a.log_norm = t->log_norm;
-  a.temperature = t->temperature;
+  a.temperature = (double)t->temperature;
+  a.inv_temperature = 1.0 / a.temperature;
+  a.c = (float)(kLog2e * a.inv_temperature);
   a.loss = out->loss;
   a.grad = out->grad;
   a.grad_row_stride = out->grad_row_stride;

@@ -53,7 +53,7 @@ struct RowFactors {
 // without the class.
 __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double body, float xmax,
                                                   double listed, double q_sum, double inv_tau,
-                                                  float temperature, float weight) {
+                                                  double temperature, float weight) {
   RowFactors f;
   const double lift = bmax == xmax           ? 1.0
                       : bmax == -CUDART_INF_F ? 0.0
@@ -61,7 +61,7 @@ __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double 
   f.total = body * lift + listed;
   f.rest_q = tail && bmax != -CUDART_INF_F ? fmax(0.0, 1.0 - q_sum) : 0.0;
   f.mass = q_sum + f.rest_q;
-  const double wt = (double)weight * (double)temperature, each = f.mass / f.total;
+  const double wt = (double)weight * temperature, each = f.mass / f.total;
   f.base = bmax == -CUDART_INF_F ? 0.0f : bmax;
   f.G = (float)(wt * (each * lift - (f.rest_q > 0.0 ? f.rest_q / body : 0.0)));
   f.P = wt * each;
@@ -72,11 +72,11 @@ __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double 
 // dot = sum q (log q - (x - xmax) / tau).  Everything is relative to the row's
 // largest logit, so logits of any size leave the loss its digits.
 __device__ __forceinline__ float row_loss(const RowFactors& f, double dot, float bmax, float xmax,
-                                          double body, double inv_tau, float temperature) {
+                                          double body, double inv_tau, double temperature) {
   double l = dot + f.mass * log(f.total);
   if (f.rest_q > 0.0)
     l += f.rest_q * (log(f.rest_q / body) - ((double)bmax - (double)xmax) * inv_tau);
-  return (float)((double)temperature * (double)temperature * l);
+  return (float)(temperature * temperature * l);
 }
 
 struct DistillSmem {
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
 
   // the teacher's masses, while the row is on its way
   const bool tail = a.log_norm != nullptr;
-  const double inv_tau = 1.0 / (double)a.temperature;
+  const double inv_tau = a.inv_temperature;
   Reducer<false> block(&sm.block);
   float amax = -CUDART_INF_F;
   bool any = false, bad = false;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   listed_max = red.max(listed_max);
   const float xmax = fmaxf(bmax, listed_max);
   const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
-  const float c = (float)(kLog2e * inv_tau);
+  const float c = a.c;
   float s = 0.0f;
   row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
@@ -410,8 +410,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     if (tail && __syncthreads_or(twice_here)) own_first(ls, a.k);
   }
 
-  const double inv_tau = 1.0 / (double)a.temperature;
-  const float c = (float)(kLog2e * inv_tau);
+  const double inv_tau = a.inv_temperature;
+  const float c = a.c;
   SoftSum soft;
   row.template walk<kU>([&](auto& x, int v, int step, bool, int) {
     if (tail) {
@@ -549,7 +549,7 @@ __device__ __forceinline__ void for_each_entry(const DistillArgs& a, int64_t r, 
 // stay in registers between the sum and the gradient, which replaces the row's
 // copy and leaves as the row came.
 template <typename T, int kPad>
-__global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logits,
+__global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_kernel(const T* logits,
                                                                    int64_t row_stride,
                                                                    int64_t n_rows, int vocab,
                                                                    DistillArgs a) {
@@ -563,7 +563,7 @@ __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logi
   sr.load(reinterpret_cast<T*>(smem_raw), logits + r0 * row_stride, row_stride, rows, vocab);
   table.fill();
   const bool tail = a.log_norm != nullptr;
-  const double inv_tau = 1.0 / (double)a.temperature;
+  const double inv_tau = a.inv_temperature;
   unsigned listed = 0;
   bool bad = false;
   float amax = -CUDART_INF_F;
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logi
         q_sum *= q_scale;
       }
       const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
-      const float c = (float)(kLog2e * inv_tau);
+      const float c = a.c;
       float e[kPad], sum = 0.0f, rest = 0.0f;  // of the body and, relative to xmax, of the list
 #pragma unroll
       for (int i = 0; i < kPad; ++i) {
@@ -641,10 +641,10 @@ __global__ void __launch_bounds__(kShortRows) distill_short_kernel(const T* logi
       if (a.loss) {
         double l = dot + mass * log(total);
         if (rest_q > 0.0) l += rest_q * (log(share) - ((double)bmax - (double)xmax) * inv_tau);
-        a.loss[r] = (float)((double)a.temperature * (double)a.temperature * l);
+        a.loss[r] = (float)(a.temperature * a.temperature * l);
       }
       if (a.grad) {
-        const double wt = (double)weight * (double)a.temperature;
+        const double wt = (double)weight * a.temperature;
         const double each = mass / total;
         // gradient: e G off the list, e P - q Q on it (the body's e G where
         // listed tokens are part of the body: lift is 1 then)

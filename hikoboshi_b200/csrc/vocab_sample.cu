@@ -1228,32 +1228,45 @@ __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __res
     sort_short(key, vocab, sizeof(T) == 2, value);
     const int nk = cut_k ? s.top_k : __popc(live);
     const float c = (float)c2;
-    auto light = [&](int i) {
-      const float x = value(i);
-      return exp2_fast((x == xmax ? 0.0f : x - xmax) * c);
+    // 32-bit weights, in the places of the 64-bit ones
+    auto light = [&](int i) -> float& {
+      return *reinterpret_cast<float*>(weight + i * kShortRows);
     };
     float sum = 0.0f;
-    keep = 0;
+    if (s.top_p < 1.0f) {
 #pragma unroll
-    for (int j = 0; j < kPad; ++j)
-      if (j < nk) {
+      for (int i = 0; i < kPad; ++i)
+        if (i < vocab) {
+          const float x = value(i);
+          const float w = x > -CUDART_INF_F ? exp2_fast((x == xmax ? 0.0f : x - xmax) * c) : 0.0f;
+          light(i) = w;
+          sum += w;
+        }
+    }
+    if (cut_k) {
+      keep = 0;
+      sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < kPad; ++j) {
+        if (j >= nk) break;
         const int i = 31 - (int)(key[j] & 31);
         keep |= 1u << i;
         if (s.top_p < 1.0f) sum += light(i);
       }
+    }
     if (s.top_p < 1.0f) {
       const float need = s.top_p * sum, slack = 4e-6f * sum;
       unsigned head = 0;
       float run = 0.0f;
       bool close = s.temperature > 1e30f;  // 32-bit differences of logits may overflow
 #pragma unroll
-      for (int j = 0; j < kPad; ++j)
-        if (j < nk && (j == 0 || run < need)) {
-          const int i = 31 - (int)(key[j] & 31);
-          head |= 1u << i;
-          run += light(i);
-          close |= fabsf(run - need) < slack;
-        }
+      for (int j = 0; j < kPad; ++j) {
+        if (j >= nk || (j > 0 && !(run < need))) break;
+        const int i = 31 - (int)(key[j] & 31);
+        head |= 1u << i;
+        run += light(i);
+        close |= fabsf(run - need) < slack;
+      }
       if (close) {
         // in 64 bits, over the order in shared memory
         signed char* order = reinterpret_cast<signed char*>(weight);

@@ -9,8 +9,6 @@ namespace hkb {
 namespace vocab {
 namespace {
 
-constexpr float kLog2ef = 1.44269504f;
-
 // Writes row r's listing: the first k of the n items of the CTA's list in order.
 template <typename T>
 __device__ __forceinline__ void write_listing(TokenList& list, int n, const T* g, int64_t r,
@@ -85,7 +83,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   else __syncthreads();
   Reducer<kClustered> red(&sm.red);
 
-  const float c = kLog2ef / a.temperature;
+  const float c = a.c;
   RowTop mine;
   float tmax = -CUDART_INF_F;
   row.template for_each_array<2>([&](auto& x) {
@@ -117,7 +115,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
   if (a.log_norm && threadIdx.x == 0 && row.rank == 0)
     a.log_norm[r] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
                         ? xmax
-                        : (float)((double)xmax / (double)a.temperature + log((double)mine.soft.s));
+                        : (float)((double)xmax * a.inv_temperature + log((double)mine.soft.s));
   const uint32_t bound = mine.reached;
   const float from = bound <= kKeyNegInf ? -CUDART_MAX_NORMAL_F : key_value(bound);
   int n = collect(row, red, sm.list, from, [&](int, float x) { return x >= from; });
@@ -169,7 +167,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* 
   const int tid = threadIdx.x, threads = blockDim.x;
   if (tid == 0) sm.list.count = 0;
 
-  const float c = kLog2ef / a.temperature;
+  const float c = a.c;
   SoftSum soft;
   float part[kU];  // largest logit of the vectors in each slot
 #pragma unroll
@@ -199,7 +197,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* 
     if (tid == 0) {
       const bool inf = soft.m == -CUDART_INF_F || soft.m == CUDART_INF_F;
       a.log_norm[r] =
-          inf ? soft.m : (float)((double)soft.m / (double)a.temperature + log((double)soft.s));
+          inf ? soft.m : (float)((double)soft.m * a.inv_temperature + log((double)soft.s));
     }
   }
   // a lower bound of the k-th largest logit: one that k of the threads' own
@@ -302,7 +300,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) top_warp_kernel(const T* __res
   row.read();
   const float xmax = row.largest();
   if (a.log_norm) {
-    const float c = kLog2ef / a.temperature;
+    const float c = a.c;
     float s = 0.0f;
 #pragma unroll
     for (int e = 0; e < kPer; ++e)
@@ -311,7 +309,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) top_warp_kernel(const T* __res
     if (lane == 0)
       a.log_norm[r] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
                           ? xmax
-                          : (float)((double)xmax / (double)a.temperature + log(total));
+                          : (float)((double)xmax * a.inv_temperature + log(total));
   }
   T* values = static_cast<T*>(a.values) + r * a.k;
   int32_t* tokens = a.tokens + r * a.k;
@@ -392,7 +390,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) top_warp_kernel(const T* __res
 // Short rows, one thread each: sorts the row in registers.  The listing goes
 // through shared memory, so that it leaves coalesced.
 template <typename T, int kPad>
-__global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restrict__ logits,
+__global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 12 : 6) top_short_kernel(const T* __restrict__ logits,
                                                                int64_t row_stride, int64_t n_rows,
                                                                int vocab, TopArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -412,7 +410,7 @@ __global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restri
     for (int j = 0; j < kPad; ++j)
       if (j < listed) places[j * kShortRows + tid] = key[j] ? (signed char)(31 - (key[j] & 31)) : -1;
     if (a.log_norm) {
-      const float c = kLog2ef / a.temperature;
+      const float c = a.c;
       const float xmax = key[0] ? value(31 - (int)(key[0] & 31)) : -CUDART_INF_F;
       float s = 0.0f;
 #pragma unroll
@@ -423,7 +421,7 @@ __global__ void __launch_bounds__(kShortRows) top_short_kernel(const T* __restri
         }
       a.log_norm[r0 + tid] = xmax == -CUDART_INF_F || xmax == CUDART_INF_F
                                  ? xmax
-                                 : (float)((double)xmax / (double)a.temperature + log((double)s));
+                                 : (float)fma((double)xmax, a.inv_temperature, (double)logf(s));
     }
   }
   __syncthreads();
