@@ -34,6 +34,7 @@ F64 = 3
 VOCAB_MAX = 262144
 VOCAB_ROWS_MAX = 134217728
 LISTING_MAX = 1024
+DISTILL_STATS = 5
 
 # Every symbol include/hkb_mpnn.h declares.
 EXPORTED = ["hkb_mpnn_create", "hkb_mpnn_destroy", "hkb_mpnn_design",
@@ -44,7 +45,7 @@ EXPORTED = ["hkb_mpnn_create", "hkb_mpnn_destroy", "hkb_mpnn_design",
             "hkb_structure_load_file", "hkb_structure_load_text", "hkb_structure_residue_count",
             "hkb_structure_copy", "hkb_structure_destroy", "hkb_backbone_noise",
             "hkb_write_design_fasta", "hkb_write_logprobs_npz",
-            "hkb_sample_tokens", "hkb_top_logits", "hkb_distill"]
+            "hkb_sample_tokens", "hkb_top_logits", "hkb_distill", "hkb_distill_backward"]
 
 
 class StructureOptions(ctypes.Structure):
@@ -107,7 +108,7 @@ class DistillTeacher(ctypes.Structure):
 
 class DistillOut(ctypes.Structure):
     _fields_ = [("loss", c_void_p), ("grad", c_void_p), ("grad_row_stride", c_int64),
-                ("row_weights", c_void_p), ("row_weight_stride", c_int64)]
+                ("row_weights", c_void_p), ("row_weight_stride", c_int64), ("stats", c_void_p)]
 
 
 class HkbError(RuntimeError):
@@ -186,6 +187,8 @@ def load() -> ctypes.CDLL:
     lib.hkb_distill.restype = Status
     lib.hkb_distill.argtypes = [c_int, POINTER(VocabRows), POINTER(DistillTeacher),
                                 POINTER(DistillOut), c_void_p]
+    lib.hkb_distill_backward.restype = Status
+    lib.hkb_distill_backward.argtypes = lib.hkb_distill.argtypes
     _lib = lib
     return lib
 

@@ -152,13 +152,18 @@ void run(const Tensor& x, F call) {
   refuse(s.detail, s.code);
 }
 
+// The loss; `stats`, if given, receives what a backward pass needs.
 Tensor loss_only(const Tensor& x, const Tensor& values, const Tensor& tokens,
-                 const std::optional<Tensor>& log_norm, double temperature) {
+                 const std::optional<Tensor>& log_norm, double temperature, Tensor* stats) {
   const hkb_vocab_rows rows = rows_of(x, "logits");
   const hkb_distill_teacher t = teacher_of(x, values, tokens, log_norm, temperature);
   Tensor loss = at::empty(lead_of(x), x.options().dtype(at::kFloat));
   hkb_distill_out o{};
   o.loss = loss.data_ptr<float>();
+  if (stats) {
+    *stats = at::empty({rows.rows, HKB_DISTILL_STATS}, x.options().dtype(at::kDouble));
+    o.stats = stats->data_ptr<double>();
+  }
   run(x, [&](int d, void* st) { return hkb_distill(d, &rows, &t, &o, st); });
   return loss;
 }
@@ -168,10 +173,14 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& values,
                         const Tensor& tokens, const std::optional<Tensor>& log_norm,
                         double temperature) {
-    ctx->save_for_backward({x, values, tokens, log_norm ? *log_norm : Tensor()});
+    Tensor stats, loss;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      loss = loss_only(x, values, tokens, log_norm, temperature, &stats);
+    }
+    ctx->save_for_backward({x, values, tokens, log_norm ? *log_norm : Tensor(), stats});
     ctx->saved_data["temperature"] = temperature;
-    at::AutoDispatchBelowADInplaceOrView below;
-    return loss_only(x, values, tokens, log_norm, temperature);
+    return loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
@@ -194,7 +203,9 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
       set_weights(&o, w, x);
       o.grad = grad.data_ptr();
       o.grad_row_stride = x.size(-1);
-      run(x, [&](int d, void* st) { return hkb_distill(d, &rows, &t, &o, st); });
+      Tensor stats = saved[4];
+      o.stats = stats.data_ptr<double>();
+      run(x, [&](int d, void* st) { return hkb_distill_backward(d, &rows, &t, &o, st); });
       return {grad, Tensor(), Tensor(), Tensor(), Tensor()};
     } catch (const Refusal& r) {
       TORCH_CHECK(false, "distill_loss backward: ", r.detail);
@@ -339,7 +350,7 @@ PyObject* loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const std::optional<Tensor> norm = optional_arg(args[3], "teacher_log_norm");
     const double temperature = number_arg(args[4], "temperature");
     if (!(x.requires_grad() && at::GradMode::is_enabled()))
-      return THPVariable_Wrap(loss_only(x, values, tokens, norm, temperature));
+      return THPVariable_Wrap(loss_only(x, values, tokens, norm, temperature, nullptr));
     if (x.is_cuda() &&
         c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
       refuse("autograd through distill_loss cannot be captured; capture distill_loss_and_grad",

@@ -55,8 +55,10 @@ struct DistillArgs {
   int64_t grad_row_stride;
   const float* row_weights;
   int64_t row_weight_stride;
+  double* stats;         // [N, HKB_DISTILL_STATS] or null
 };
 cudaError_t launch_distill(cudaStream_t st, const VocabRows& r, const DistillArgs& a);
+cudaError_t launch_distill_backward(cudaStream_t st, const VocabRows& r, const DistillArgs& a);
 
 // Launch shape of the row kernels: CTAs per row, threads and elements per CTA.
 struct RowShape {

@@ -88,6 +88,55 @@ VocabRows internal_rows(const hkb_vocab_rows& v) {
   return {v.rows, v.vocab, v.dtype, v.logits, v.row_stride};
 }
 
+hkb_status check_distill(const hkb_vocab_rows* rows, const hkb_distill_teacher* t,
+                         const hkb_distill_out* out) {
+  const hkb_status st = check_rows(rows);
+  if (st.code != HKB_OK) return st;
+  if (t == nullptr || out == nullptr) return invalid("teacher and output must be non-null");
+  if (t->k < 1 || t->k > HKB_LISTING_MAX)
+    return invalid("a row's listing must have 1 to HKB_LISTING_MAX entries");
+  if (!real_dtype(t->dtype)) return invalid("teacher values must be F32, F16 or BF16");
+  if (!(t->temperature >= HKB_TEMPERATURE_MIN && t->temperature <= HKB_TEMPERATURE_MAX))
+    return invalid("temperature must be 1e-30 to 1e30");
+  if (out->row_weight_stride < 0) return invalid("the row weight stride must not be negative");
+  if (out->grad != nullptr) {
+    if (out->grad_row_stride < rows->vocab)
+      return invalid("the gradient's rows must not overlap");
+    const uintptr_t b = elem_bytes(rows->dtype);
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(rows->logits);
+    const uintptr_t g0 = reinterpret_cast<uintptr_t>(out->grad);
+    if (g0 % b != 0) return invalid("gradient pointer is not aligned to its type");
+    if (rows->rows > 0) {
+      const uintptr_t n = (uintptr_t)rows->rows - 1;
+      const uintptr_t x1 = x0 + (n * (uintptr_t)rows->row_stride + rows->vocab) * b;
+      const uintptr_t g1 = g0 + (n * (uintptr_t)out->grad_row_stride + rows->vocab) * b;
+      const bool same = x0 == g0 && (n == 0 || rows->row_stride == out->grad_row_stride);
+      if (!same && x0 < g1 && g0 < x1)
+        return invalid("grad must be the logits' own buffer or lie apart from it");
+    }
+  }
+  return {HKB_OK, ""};
+}
+
+DistillArgs internal_distill(const hkb_distill_teacher& t, const hkb_distill_out& out) {
+  DistillArgs a{};
+  a.k = t.k;
+  a.teacher_dtype = t.dtype;
+  a.values = t.values;
+  a.tokens = t.tokens;
+  a.log_norm = t.log_norm;
+  a.temperature = (double)t.temperature;
+  a.inv_temperature = 1.0 / a.temperature;
+  a.c = (float)(kLog2e * a.inv_temperature);
+  a.loss = out.loss;
+  a.grad = out.grad;
+  a.grad_row_stride = out.grad_row_stride;
+  a.row_weights = out.row_weights;
+  a.row_weight_stride = out.row_weight_stride;
+  a.stats = out.stats;
+  return a;
+}
+
 }  // namespace
 }  // namespace hkb
 
@@ -158,53 +207,32 @@ hkb_status hkb_top_logits(int device, const hkb_vocab_rows* rows, int32_t k, flo
 
 hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill_teacher* t,
                        const hkb_distill_out* out, void* stream) {
-  const hkb_status st = check_rows(rows);
-  if (st.code != HKB_OK) return st;
-  if (t == nullptr || out == nullptr) return invalid("teacher and output must be non-null");
-  if (t->k < 1 || t->k > HKB_LISTING_MAX)
-    return invalid("a row's listing must have 1 to HKB_LISTING_MAX entries");
-  if (!real_dtype(t->dtype)) return invalid("teacher values must be F32, F16 or BF16");
-  if (!(t->temperature >= HKB_TEMPERATURE_MIN && t->temperature <= HKB_TEMPERATURE_MAX))
-    return invalid("temperature must be 1e-30 to 1e30");
-  if (out->row_weight_stride < 0) return invalid("the row weight stride must not be negative");
-  if (out->grad != nullptr) {
-    if (out->grad_row_stride < rows->vocab)
-      return invalid("the gradient's rows must not overlap");
-    const uintptr_t b = elem_bytes(rows->dtype);
-    const uintptr_t x0 = reinterpret_cast<uintptr_t>(rows->logits);
-    const uintptr_t g0 = reinterpret_cast<uintptr_t>(out->grad);
-    if (g0 % b != 0) return invalid("gradient pointer is not aligned to its type");
-    if (rows->rows > 0) {
-      const uintptr_t n = (uintptr_t)rows->rows - 1;
-      const uintptr_t x1 = x0 + (n * (uintptr_t)rows->row_stride + rows->vocab) * b;
-      const uintptr_t g1 = g0 + (n * (uintptr_t)out->grad_row_stride + rows->vocab) * b;
-      const bool same = x0 == g0 && (n == 0 || rows->row_stride == out->grad_row_stride);
-      if (!same && x0 < g1 && g0 < x1)
-        return invalid("grad must be the logits' own buffer or lie apart from it");
-    }
-  }
-  if (rows->rows == 0) return {HKB_OK, ""};
+  const hkb_status st = check_distill(rows, t, out);
+  if (st.code != HKB_OK || rows->rows == 0) return st;
   if (out->loss == nullptr && out->grad == nullptr)
     return invalid("loss or grad must be non-null");
   if (t->values == nullptr || t->tokens == nullptr)
     return invalid("teacher values and tokens must be non-null");
   DeviceGuard guard(device);
   if (guard.status().code != HKB_OK) return guard.status();
-  DistillArgs a{};
-  a.k = t->k;
-  a.teacher_dtype = t->dtype;
-  a.values = t->values;
-  a.tokens = t->tokens;
-  a.log_norm = t->log_norm;
-  a.temperature = (double)t->temperature;
-  a.inv_temperature = 1.0 / a.temperature;
-  a.c = (float)(kLog2e * a.inv_temperature);
-  a.loss = out->loss;
-  a.grad = out->grad;
-  a.grad_row_stride = out->grad_row_stride;
-  a.row_weights = out->row_weights;
-  a.row_weight_stride = out->row_weight_stride;
-  return launched(launch_distill(static_cast<cudaStream_t>(stream), internal_rows(*rows), a));
+  return launched(launch_distill(static_cast<cudaStream_t>(stream), internal_rows(*rows),
+                                 internal_distill(*t, *out)));
+}
+
+hkb_status hkb_distill_backward(int device, const hkb_vocab_rows* rows,
+                                const hkb_distill_teacher* t, const hkb_distill_out* out,
+                                void* stream) {
+  const hkb_status st = check_distill(rows, t, out);
+  if (st.code != HKB_OK || rows->rows == 0) return st;
+  if (out->loss != nullptr) return invalid("a backward pass has no loss");
+  if (out->grad == nullptr || out->stats == nullptr)
+    return invalid("a backward pass needs grad and stats");
+  if (t->values == nullptr || t->tokens == nullptr)
+    return invalid("teacher values and tokens must be non-null");
+  DeviceGuard guard(device);
+  if (guard.status().code != HKB_OK) return guard.status();
+  return launched(launch_distill_backward(static_cast<cudaStream_t>(stream), internal_rows(*rows),
+                                          internal_distill(*t, *out)));
 }
 
 }  // extern "C"

@@ -40,8 +40,8 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
 // What a row's loss and gradient need beside the row.
 struct RowFactors {
   float base;     // of the body's exponents
-  float G;        // gradient of an unlisted token: exp2((x - base) c) * G
-  double P, Q;    // gradient on the list: P exp((x - xmax) / tau) - Q q
+  double F;       // gradient of an unlisted token: exp2((x - base) c) * F * Q
+  double each, Q; // gradient on the list: Q each exp((x - xmax) / tau) - Q q
   double total;   // of the row's weights, relative to its largest logit
   double mass;    // the teacher's
   double rest_q;  // of it, the unlisted tokens' where they are a class
@@ -61,12 +61,28 @@ __device__ __forceinline__ RowFactors row_factors(bool tail, float bmax, double 
   f.total = body * lift + listed;
   f.rest_q = tail && bmax != -CUDART_INF_F ? fmax(0.0, 1.0 - q_sum) : 0.0;
   f.mass = q_sum + f.rest_q;
-  const double wt = (double)weight * temperature, each = f.mass / f.total;
+  const double each = f.mass / f.total;
   f.base = bmax == -CUDART_INF_F ? 0.0f : bmax;
-  f.G = (float)(wt * (each * lift - (f.rest_q > 0.0 ? f.rest_q / body : 0.0)));
-  f.P = wt * each;
-  f.Q = wt;
+  f.F = each * lift - (f.rest_q > 0.0 ? f.rest_q / body : 0.0);
+  f.each = each;
+  f.Q = (double)weight * temperature;
   return f;
+}
+
+__device__ __forceinline__ double listed_gradient(double Q, double each, double e, double q) {
+  return __dmul_rn(__dmul_rn(Q, each), e) - __dmul_rn(Q, q);
+}
+
+// What a backward pass needs of a row's forward pass.
+enum StatFlags { kStatBad = 1, kStatEmpty = 2, kStatTwice = 4 };
+__device__ __forceinline__ void write_stats(double* stats, int64_t r, const RowFactors& f,
+                                            double q_scale, float xmax, float from, int flags) {
+  double* s = stats + r * HKB_DISTILL_STATS;
+  s[0] = f.F;
+  s[1] = f.each;
+  s[2] = q_scale;
+  s[3] = __hiloint2double(__float_as_int(f.base), __float_as_int(xmax));
+  s[4] = __hiloint2double(__float_as_int(from), flags);
 }
 
 // dot = sum q (log q - (x - xmax) / tau).  Everything is relative to the row's
@@ -82,6 +98,7 @@ __device__ __forceinline__ float row_loss(const RowFactors& f, double dot, float
 struct DistillSmem {
   ReduceScratch cluster;
   ReduceScratch block;
+  Exp2Table table;
 };
 
 // Listing of a row in shared memory, behind the slice's buffer.
@@ -117,6 +134,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   ls.token = reinterpret_cast<int*>(ls.x + a.k);
   ls.own = ls.token + a.k;
 
+  sm.table.fill();
   // the teacher's masses, while the row is on its way
   const bool tail = a.log_norm != nullptr;
   const double inv_tau = a.inv_temperature;
@@ -144,21 +162,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     const bool zero_weight =
         a.row_weights != nullptr && a.row_weights[r * a.row_weight_stride] == 0.0f;
     if (writer && a.loss) a.loss[r] = v;
+    if (writer && a.stats)
+      write_stats(a.stats, r, RowFactors{}, 0.0, 0.0f, 0.0f, row_bad ? kStatBad : kStatEmpty);
     if (grad) fill_slice(row, grad, zero_weight ? 0.0f : v);
     return;
   }
-  // log q_k = (a_k - from) / tau - norm
-  double norm;
-  if (tail) {
-    norm = (double)a.log_norm[r];
-  } else {
-    amax = block.max(amax);
-    double e = 0.0;
-    for (int k = threadIdx.x; k < a.k; k += blockDim.x)
-      if (ls.token[k] >= 0) e += exp(((double)ls.x[k] - (double)amax) * inv_tau);
-    norm = log(block.sum(e));
-  }
-  const double from = tail ? 0.0 : (double)amax;
+  // masses: exp(a / tau - norm), or relative to the largest until their sum is known
+  if (!tail) amax = block.max(amax);
+  const double from = tail ? 0.0 : (double)amax, norm = tail ? (double)a.log_norm[r] : 0.0;
   double q_sum = 0.0, dot = 0.0;  // sum q; over the entries in this slice sum q log q
   float listed_max = -CUDART_INF_F;
   for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
@@ -166,8 +177,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     double q = 0.0;
     int own = 0;
     if (token >= 0) {
-      const double log_q = ((double)ls.x[k] - from) * inv_tau - norm;
-      q = exp(log_q);
+      const double log_q = ((double)ls.x[k] - from) * inv_tau - norm, t = log_q * kLog2e;
+      q = t <= 0.0 ? sm.table(t) : exp2(t);
       q_sum += q;
       const int at = token - row.start;
       if (at >= 0 && at < row.n) {
@@ -181,7 +192,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     ls.q[k] = q;
     ls.own[k] = own;
   }
-  q_sum = block.sum(q_sum);
+  q_sum = block.sum(q_sum);  // of all entries, in every CTA
   // One entry stands for a token that is listed more than once: each writes
   // its number in the token's place, the one that is found there stays.  Then
   // the place gets -inf (unlisted class) or its logit back.
@@ -239,15 +250,24 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   const double2 sums = red.sum(make_double2(listed, dot));
   listed = sums.x;
   dot = sums.y;
+  const double sum_q = q_sum, q_scale = tail ? 1.0 : 1.0 / sum_q;
+  q_sum *= q_scale;
+  if (!tail) dot = dot * q_scale - log(sum_q);
   const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
   const RowFactors f =
       row_factors(tail, bmax, body, xmax, listed, q_sum, inv_tau, a.temperature, weight);
   if (writer && a.loss) a.loss[r] = row_loss(f, dot, bmax, xmax, body, inv_tau, a.temperature);
+  if (a.stats) {
+    const bool twice_at_all = red.max((int)row_twice);  // in any CTA's slice
+    if (writer)
+      write_stats(a.stats, r, f, q_scale, xmax, tail ? 0.0f : amax, twice_at_all ? kStatTwice : 0);
+  }
   if (grad == nullptr) return;
   if (weight == 0.0f) {
     fill_slice(row, grad, 0.0f);
     return;
   }
+  const float G = (float)(f.Q * f.F);
   T* gs = grad + row.start - row.ph;  // element e0 of the slice's vectors goes to gs[e0]
   const bool same_phase = (reinterpret_cast<uintptr_t>(gs) & 15) == 0;
   row.for_each([&](int i0, const Vec<T>& x) {
@@ -255,7 +275,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
 #pragma unroll
     for (int i = 0; i < kE / 2; ++i) {
       const float2 p = x.pair(i);
-      y.set_pair(i, make_float2(exp2_fast((p.x - base) * c) * f.G, exp2_fast((p.y - base) * c) * f.G));
+      y.set_pair(i, make_float2(exp2_fast((p.x - base) * c) * G, exp2_fast((p.y - base) * c) * G));
     }
     const int e0 = i0 - row.start + row.ph;
     if (same_phase && e0 >= row.ph && e0 + kE <= row.ph + row.n) {
@@ -276,7 +296,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
     const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
-    grad[ls.token[k]] = narrow<T>((float)(f.P * e - f.Q * q));
+    grad[ls.token[k]] = narrow<T>((float)listed_gradient(f.Q, f.each, e, q * q_scale));
   }
 }
 
@@ -362,7 +382,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
   const bool tail = a.log_norm != nullptr;
   T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
   const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
-  const bool marked = tail || grad != nullptr;
+  const bool marked = tail || grad != nullptr || a.stats != nullptr;
   if (marked)
     for (int w = tid; w < (row.end + 31) / 32; w += threads) marks[w] = 0;
   unsigned flags = 0;  // 1: an entry, 2: a token outside the vocabulary
@@ -387,6 +407,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
   if (row_bad || !row_any) {
     const float v = row_bad ? CUDART_NAN_F : 0.0f;
     if (tid == 0 && a.loss) a.loss[r] = v;
+    if (tid == 0 && a.stats)
+      write_stats(a.stats, r, RowFactors{}, 0.0, 0.0f, 0.0f, row_bad ? kStatBad : kStatEmpty);
     if (grad)
       for (int i = tid; i < vocab; i += threads) grad[i] = narrow<T>(weight == 0.0f ? 0.0f : v);
     return;
@@ -465,6 +487,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     // what the list and the loss need waits in shared memory
     sm.f = f;
     sm.sums = sums;
+    if (a.stats)
+      write_stats(a.stats, r, f, q_scale, xmax, tail ? 0.0f : amax, sums.twice ? kStatTwice : 0);
   }
   auto write_loss = [&] {
     const double dot = tail ? sums.dot : sums.dot * q_scale - log(sums.q);
@@ -479,7 +503,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
   T* gv = grad - row.ph;  // vector v of the row goes to gv[v * kE ..]
   const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
   const float2 minus = make_float2(-f.base, -f.base), scale = make_float2(c, c),
-               G = make_float2(f.G, f.G);
+               G = make_float2((float)(f.Q * f.F), (float)(f.Q * f.F));
   row.template walk<kU>([&](auto& x, int v, int step, bool whole, int) {
     constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
@@ -512,12 +536,115 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
     const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
-    grad[ls.token[k]] = narrow<T>((float)(sm.f.P * e - sm.f.Q * (q * scale_q)));
+    grad[ls.token[k]] = narrow<T>((float)listed_gradient(sm.f.Q, sm.f.each, e, q * scale_q));
   }
   // the last warp has fewest entries to see to
   if (tid == threads - 1 && a.loss) {
     const double dot = tail ? sm.sums.dot : sm.sums.dot * scale_q - log(sum_q);
     a.loss[r] = row_loss(sm.f, dot, bmax, xmax, body, inv_tau, a.temperature);
+  }
+}
+
+// The gradient from a forward pass's statistics: a row is read once, in parts of
+// a CTA each.  The same formulas as above, to the bit.
+template <typename T>
+__global__ void __launch_bounds__(256, 4) distill_backward_kernel(const T* logits,
+                                                                  int64_t row_stride, int vocab,
+                                                                  int parts, int part_vectors,
+                                                                  DistillArgs a) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  __shared__ Exp2Table table;
+  constexpr int kE = Vec<T>::kN, kU = 4;
+  const int64_t r = blockIdx.x / (unsigned)parts;
+  const int part = (int)(blockIdx.x % (unsigned)parts);
+  const int tid = threadIdx.x, threads = blockDim.x;
+  const T* g = logits + r * row_stride;
+  const RowStream<T> row(g, vocab);
+  T* gv = static_cast<T*>(a.grad) + r * a.grad_row_stride - row.ph;
+  // this CTA's whole vectors, and its elements with the row's ends
+  const int v0 = ::min(row.hi, row.lo + part * part_vectors);
+  const int v1 = part == parts - 1 ? ::max(v0, row.hi) : ::min(row.hi, v0 + part_vectors);
+  const int e_first = part == 0 ? row.ph : v0 * kE;
+  const int e_last = part == parts - 1 ? row.end : v1 * kE;  // one behind
+  Listing ls;
+  ls.q = reinterpret_cast<double*>(smem_raw);
+  ls.x = reinterpret_cast<float*>(ls.q + a.k);
+  ls.token = reinterpret_cast<int*>(ls.x + a.k);
+  table.fill();
+
+  const double* st = a.stats + r * HKB_DISTILL_STATS;
+  const double F = st[0], each = st[1], q_scale = st[2];
+  const float base = __int_as_float(__double2hiint(st[3])), xmax = __int_as_float(__double2loint(st[3]));
+  const float amax = __int_as_float(__double2hiint(st[4]));
+  const int flags = __double2loint(st[4]);
+  const float weight = a.row_weights ? a.row_weights[r * a.row_weight_stride] : 1.0f;
+  if ((flags & (kStatBad | kStatEmpty)) || weight == 0.0f) {
+    const T v = narrow<T>((flags & kStatBad) && weight != 0.0f ? CUDART_NAN_F : 0.0f);
+    for (int e = e_first + tid; e < e_last; e += threads) gv[e] = v;
+    return;
+  }
+  const bool tail = a.log_norm != nullptr;
+  const double inv_tau = a.inv_temperature;
+  const double from = tail ? 0.0 : (double)amax, norm = tail ? (double)a.log_norm[r] : 0.0;
+  __syncthreads();  // the table
+  for (int k = tid; k < a.k; k += threads) {
+    const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
+    int token = a.tokens[r * a.k + k];
+    if (token < 0 || token >= vocab || v == -CUDART_INF_F) token = -1;
+    const int e = token + row.ph;
+    const bool here = token >= 0 && e >= e_first && e < e_last;
+    ls.token[k] = here ? token : -1;
+    if (here) {
+      const double t = (((double)v - from) * inv_tau - norm) * kLog2e;
+      ls.q[k] = t <= 0.0 ? table(t) : exp2(t);
+      ls.x[k] = widen(g[token]);
+    }
+  }
+  __syncthreads();  // read before the gradient may take the logits' place
+  const double Q = (double)weight * a.temperature;
+  const float c = a.c, Gf = (float)(Q * F);
+  const float2 minus = make_float2(-base, -base), scale = make_float2(c, c), G = make_float2(Gf, Gf);
+  const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
+  auto put = [&](const Vec<T>& x, int v, bool whole) {
+    Vec<T> y;
+#pragma unroll
+    for (int i = 0; i < kE / 2; ++i) {
+      const float2 t = __fmul2_rn(__fadd2_rn(x.pair(i), minus), scale);
+      y.set_pair(i, __fmul2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), G));
+    }
+    const int e0 = v * kE;
+    if (same_phase && whole) {
+      __stcs(reinterpret_cast<uint4*>(gv + e0), *reinterpret_cast<const uint4*>(&y));
+    } else {
+#pragma unroll
+      for (int e = 0; e < kE; ++e)
+        if (e0 + e >= row.ph && e0 + e < row.end) gv[e0 + e] = reinterpret_cast<const T*>(y.w)[e];
+    }
+  };
+  const Vec<T>* vec = reinterpret_cast<const Vec<T>*>(row.g);
+  int v = v0 + tid;
+  for (; v + (kU - 1) * threads < v1; v += kU * threads) {
+    Vec<T> x[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) x[u] = vec[v + u * threads];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) put(x[u], v + u * threads, true);
+  }
+  for (; v < v1; v += threads) put(vec[v], v, true);
+  if (tid == 0 && part == 0 && row.lo > 0) put(row.partial(0), 0, false);
+  if (tid == threads - 1 && part == parts - 1 && row.hi >= row.lo && row.hi * kE < row.end)
+    put(row.partial(row.hi), row.hi, false);
+  __syncthreads();
+  for (int k = tid; k < a.k; k += threads) {
+    if (ls.token[k] < 0) continue;
+    double q = ls.q[k];
+    if (flags & kStatTwice) {
+      q = 0.0;
+      for (int j = 0; j < a.k; ++j)
+        if (ls.token[j] == ls.token[k]) q += ls.q[j];
+    }
+    const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
+    gv[row.ph + ls.token[k]] = narrow<T>((float)listed_gradient(Q, each, e, q * q_scale));
   }
 }
 
@@ -702,8 +829,33 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
                             s.chunk, (int)s.smem, a);
 }
 
+template <typename T>
+cudaError_t launch_backward(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  // a short row's thread has the whole row at hand: nothing to save
+  if (v.vocab <= kShortVocab) return launch<T>(st, v, a);
+  // parts of up to 16 vectors a thread; of as few as two while that gives no
+  // four CTAs a SM
+  const int nvec = v.vocab / (16 / (int)sizeof(T)) + 1;
+  int threads = 256, per = 16;
+  while (threads > 32 && threads * 4 > nvec) threads /= 2;
+  while (per > 2 && v.rows * ((nvec + threads * per - 1) / (threads * per)) < 4 * 148) per /= 2;
+  const int part = threads * per, parts = (nvec + part - 1) / part;
+  const int smem = a.k * 16;
+  distill_backward_kernel<T><<<(unsigned)(v.rows * parts), threads, smem, st>>>(
+      static_cast<const T*>(v.logits), v.row_stride, v.vocab, parts, part, a);
+  return cudaGetLastError();
+}
+
 }  // namespace
 }  // namespace vocab
+
+cudaError_t launch_distill_backward(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  switch (v.dtype) {
+    case HKB_F32: return vocab::launch_backward<float>(st, v, a);
+    case HKB_F16: return vocab::launch_backward<__half>(st, v, a);
+    default: return vocab::launch_backward<__nv_bfloat16>(st, v, a);
+  }
+}
 
 cudaError_t launch_distill(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   switch (v.dtype) {

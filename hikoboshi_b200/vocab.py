@@ -88,10 +88,11 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     no entry; a row without entries has loss and gradient 0 whatever its logits.
     A token >= V makes its row NaN.  ``temperature`` is 1e-30 to 1e30.
 
-    The loss is differentiable once.  The backward pass reads ``logits`` again, so they must not be overwritten
-    before it.  Autograd through this call cannot be captured into a CUDA
-    graph (an eager graph of the same leaves would break the capture): there
-    it raises HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.
+    The loss is differentiable once.  The backward pass reads ``logits`` and the
+    teacher's tensors again, so they must not be overwritten before it.
+    Autograd through this call cannot be captured into a CUDA graph (an eager
+    graph of the same leaves would break the capture): there it raises
+    HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.
     """
     return _vocab.loss(logits, teacher_values, teacher_tokens, teacher_log_norm, temperature)
 

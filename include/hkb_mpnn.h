@@ -290,6 +290,8 @@ hkb_status hkb_write_logprobs_npz(const char* path, int32_t num_seqs, int32_t re
 /* of log-norms and of distillation */
 #define HKB_TEMPERATURE_MIN 1e-30f
 #define HKB_TEMPERATURE_MAX 1e30f
+/* numbers a row that a backward pass takes from the forward pass */
+#define HKB_DISTILL_STATS 5
 
 typedef enum { HKB_F32 = 0, HKB_F16 = 1, HKB_BF16 = 2, HKB_F64 = 3 } hkb_dtype;
 
@@ -370,6 +372,8 @@ typedef struct {
   const float* row_weights;  /* d(objective) / d(loss of row r) is
                                 row_weights[r * row_weight_stride]; NULL = 1 */
   int64_t row_weight_stride; /* 0 (one number for all rows) or more */
+  double* stats;             /* [N, HKB_DISTILL_STATS] of each row, for
+                                hkb_distill_backward, or NULL */
 } hkb_distill_out;
 
 /* Divergence of student rows from a teacher's listed logits a_k at tokens t_k,
@@ -395,6 +399,14 @@ typedef struct {
  * any other overlap is not allowed, and rows must not overlap then. */
 hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill_teacher* teacher,
                        const hkb_distill_out* out, void* stream);
+
+/* The gradient alone, after a call of hkb_distill on the same rows and teacher
+ * that wrote out->stats: reads the rows once, where hkb_distill has to read them
+ * twice.  out->grad and out->stats must be non-null (stats is read), out->loss
+ * NULL; the gradient is the one hkb_distill gives. */
+hkb_status hkb_distill_backward(int device, const hkb_vocab_rows* rows,
+                                const hkb_distill_teacher* teacher, const hkb_distill_out* out,
+                                void* stream);
 
 #ifdef __cplusplus
 }

@@ -731,3 +731,28 @@ def test_extreme_distill_temperatures(vocab):
                     check_distill(loss[:3], grad[:3], x[:3], v[:3], t[:3],
                                   None if n is None else n[:3], tau)
                 check_top([a[:3] for a in vocab.top_logits(x, 5, temperature=tau)], x[:3], 5, tau)
+
+
+@pytest.mark.parametrize("rows,size", [(5, 33), (5, 3001), (3, 70001), (160, 40), (160, 5003),
+                                       (150, 40000), (2000, 700)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_is_the_fused_gradient(vocab, rows, size, dtype):
+    # to the bit, with every special row and from any offset
+    base = logits(1, rows * (size + 3) + 16, dtype, 5)[0]
+    for offset in (0, 3):
+        x = base[offset:offset + rows * (size + 3)].view(rows, size + 3)[:, :size].clone() \
+            if offset == 0 else base[offset:offset + rows * (size + 3)].view(rows, size + 3)[:, :size]
+        v, t, norm = teacher(x, 20, dtype, 3, 1.5, True)
+        w = torch.rand(rows, generator=gen(1), device="cuda") + 0.5
+        w[2] = 0.0
+        t[0] = -1
+        t[1, 4] = t[1, 9]
+        t[3 % rows, 2] = size if rows > 4 else t[3 % rows, 2]
+        for n in (None, norm):
+            kw = dict(teacher_log_norm=n, temperature=1.5)
+            loss, grad = vocab.distill_loss_and_grad(x, v, t, row_weights=w, **kw)
+            xr = x.detach().requires_grad_()
+            l2 = vocab.distill_loss(xr, v, t, **kw)
+            (g2,) = torch.autograd.grad(l2, xr, w)
+            assert torch.equal(l2.nan_to_num(-7.0), loss.nan_to_num(-7.0))
+            assert torch.equal(g2.nan_to_num(-7.0), grad.nan_to_num(-7.0))

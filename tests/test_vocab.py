@@ -145,3 +145,20 @@ def test_null_pointers_are_refused():
     bad = _lib.VocabRows(2, 21, _lib.F32, ctypes.addressof(buf) + 2, 21)
     assert b"aligned" in lib.hkb_top_logits(0, ctypes.byref(bad), 1, 1.0,
                                             ctypes.byref(_lib.TopOut()), None).detail
+
+
+def test_backward_entry_is_checked():
+    lib = _lib.load()
+    buf = (ctypes.c_float * 64)()
+    at = ctypes.addressof(buf)
+    rows = _lib.VocabRows(1, 21, _lib.F32, at, 21)
+    t = _lib.DistillTeacher(k=1, temperature=1.0, values=at, tokens=at)
+    for out, text in ((dict(loss=at, grad=at, stats=at), b"no loss"), (dict(grad=at), b"stats"),
+                      (dict(stats=at), b"grad")):
+        o = _lib.DistillOut(grad_row_stride=21, **out)
+        st = lib.hkb_distill_backward(0, ctypes.byref(rows), ctypes.byref(t), ctypes.byref(o), None)
+        assert st.code == _lib.HKB_INVALID_ARGUMENT and text in st.detail, st.detail
+    rows.rows = 0
+    o = _lib.DistillOut(grad_row_stride=21)
+    assert lib.hkb_distill_backward(0, ctypes.byref(rows), ctypes.byref(t), ctypes.byref(o), None
+                                    ).code == _lib.HKB_OK
