@@ -39,10 +39,11 @@ RowShape row_shape(int64_t rows, int vocab, int elem_bytes) {
   // 256 or 512, about two vectors a thread (1024 is no faster for a single row:
   // the barriers take longer)
   s.threads = vecs > 2 * 256 ? 512 : 256;
-  // with more rows than two CTAs a SM, slices below 64 KB do better on four
-  // smaller CTAs: 25,892 rows of 3,227 f32, top-k: 678 us with 512 threads, 340
-  // with 256; but 256 rows of 131,072 bf16 (64 KB), top-p: 348 and 381
-  if (rows * s.cluster > 2 * 148 && vecs <= 4096) s.threads = 256;
+  // with more rows than two CTAs a SM, slices of which four fit a SM (beside the
+  // sampler's 28 KB) do better on 256 threads: 25,892 rows of 3,227 f32, top-k: 678
+  // us with 512 threads, 340 with 256; larger ones do not: 256 rows of 131,072
+  // bf16 (64 KB), top-p: 348 and 381
+  if (rows * s.cluster > 2 * 148 && s.smem <= 28 * 1024) s.threads = 256;
   return s;
 }
 
