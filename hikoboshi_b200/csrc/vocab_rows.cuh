@@ -599,15 +599,25 @@ struct SoftSum {
   }
 };
 
-// Rows from which on streaming is used: one a SM.
-constexpr int kStreamRows = 148;
-
 template <>
 __device__ __forceinline__ SoftSum shfl_xor(SoftSum v, int o) {
   SoftSum r;
   r.m = __shfl_xor_sync(0xffffffffu, v.m, o);
   r.s = __shfl_xor_sync(0xffffffffu, v.s, o);
   return r;
+}
+
+// Streaming is used from more rows than four a SM, where a CTA's set-up and its
+// barriers cost rows in shared memory more, and from more bytes than about two
+// thirds of what the SMs' shared memory holds at once (two slices of 64 KB each).
+// Measured (us), streamed and in shared memory, bf16, loss with its gradient: 150 x
+// 2000: 12 and 10; 300 x 8000: 20 and 12; 600 x 100: 10 and 16; 600 x 8000: 23 and 20;
+// 2000 x 2000: 16 and 29; 2000 x 8000: 29 and 39; 40 x 131072 (10.5 MB): 25 and 20; 74 x
+// 131072 (19 MB): 25 and 33; 150 x 50001 (15 MB): 23 and 31.  Top 64 gains less, and
+// loses where slices are full: 4000 x 8000: 68 and 57; 2000 x 1000: 18 and 25; 74 x
+// 131072: 20 and 27.
+inline bool use_stream(int64_t rows, int vocab, int elem_bytes) {
+  return rows > 4 * 148 || rows * vocab * elem_bytes > 12000000;
 }
 
 // Threads for a CTA that streams rows: a power of two, 20 to 40 vectors a thread.  Fewer threads a row leave room for more CTAs, whose
@@ -629,6 +639,17 @@ inline int stream_threads(int vocab, int elem_bytes) {
 // over the staged row then start in different banks.
 constexpr int kWarpVocab = 31 * 32;
 constexpr int kWarpRows = 4;  // warps of a CTA
+
+// A warp's passes over its tokens take their time, a CTA a row its set-up: with
+// few rows of more than seven tokens a lane the CTA is mostly faster, from four
+// rows a SM the warp.  Measured (us), warp and CTA, f32, top 100 logits / top-p 0.9 /
+// top-k 20: 100 x 224: 14 and 10 / 12 and 12 / 10 and 10; 100 x 500: 18 and 10 / 27
+// and 14 / 16 and 10; 600 x 500: 20 and 16 / 27 and 25 / 16 and 16; 600 x 900: 20 and 14
+// / 27 and 37 / 16 and 16; 2000 x 900: 29 and 29 / 39 and 92 / 25 and 31; 4000 x 100: 18
+// and 39 / 18 and 82 / 16 and 51.
+inline bool use_warp_rows(int64_t rows, int vocab) {
+  return vocab <= 7 * 32 || (vocab <= kWarpVocab && rows >= 4 * 148);
+}
 
 template <typename T, int kPer>
 struct WarpRow {

@@ -740,6 +740,15 @@ __device__ __forceinline__ void finish_list(SampleSmem& sm, int n, const Weights
   }
 }
 
+// Long rows in the shared memory of a CTA or a cluster.  Top-k of up to 1024
+// collects the few tokens above a bound and lets rank 0 finish; without it the
+// mass of the whole row is added up in 64 bits, the top-p border bracketed by
+// bins, and the token found by the running masses of CTAs, warps and steps.
+//
+// Bound by latency with few rows (1 x 32768 f32, top-k: 12 us; cluster barriers
+// of about 1000 cycles each) and by the 64-bit weights with many (192 x 50001
+// f16, unfiltered: 38 us, FP64 pipe 27 %).  Slices of 64 KB at most: two CTAs a
+// SM; of 32 KB 64 rows of 131,072 bf16 took 145 us (top-p) instead of 102.
 template <typename T, bool kClustered>
 __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
@@ -1005,6 +1014,8 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
 // the head is found with 32-bit weights, by bisection of the logits' keys, and
 // again with 64-bit ones where a comparison with the border is too close (or
 // where equal logits share the border: their number needs the exact masses).
+// Bound by instructions: 415,936 x 143 f32, unfiltered, 1.1 ms (9.5 ms with a CTA
+// a row, whose barriers and set-up such rows do not repay).
 template <typename T, int kPer>
 __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
     const T* __restrict__ logits, int64_t row_stride, int64_t n_rows, int vocab, SampleArgs a) {
@@ -1093,34 +1104,58 @@ __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
     over = warp_total(over);
     ties = __reduce_add_sync(0xffffffffu, ties);
     // 32-bit differences of logits may overflow at the largest temperatures
-    const bool close =
-        !(at - need > slack && need - over > slack) || s.temperature > 1e30f;
-    if (close || ties > 1) {
-      auto mass = [&](auto in) {
-        double m = 0.0;
-#pragma unroll 1
-        for (unsigned b = keep; b != 0; b &= b - 1) {
-          const float x = widen(row.s[row.ph + lane * kPer + __ffs(b) - 1]);
-          if (in(x)) m += table(exponent(x));
-        }
-        return warp_total(m);
-      };
-      const double border = (double)s.top_p * mass([](float) { return true; });
-      if (close) {
-        lo = kKeyNegInf + 1;
+    const bool blind = s.temperature > 1e30f;
+    if (blind || ties > 1 || !(at - need > slack && need - over > slack)) {
+      // In 64 bits: from the largest value that 32 bits cannot rule out (or the
+      // row's largest) down, value by value, until the mass is reached or no
+      // smaller value is left.
+      float from = xmax;
+      if (!blind) {
+        lo = order_key(t);
         hi = order_key(xmax);
         while (lo < hi) {
           const uint32_t mid = lo + (hi - lo + 1) / 2;
-          const float from = key_value(mid);
-          if (mass([from](float x) { return x >= from; }) >= border) lo = mid;
+          const float at_least = key_value(mid);
+          float m = 0.0f;
+#pragma unroll
+          for (int e = 0; e < kPer; ++e) m += row.x[e] >= at_least ? w[e] : 0.0f;
+          if (warp_total(m) >= need - slack) lo = mid;
           else hi = mid - 1;
         }
-        t = key_value(lo);
+        from = key_value(lo);
       }
-      const double above = mass([t](float x) { return x > t; });
-      const double each = table(exponent(t));
-      const double n = each > 0.0 ? ceil((border - above) / each) : 1.0;
-      ties = (int)fmin(fmax(n, 1.0), (double)vocab);
+      double mass = 0.0, above = 0.0;
+#pragma unroll 1
+      for (unsigned b = keep; b != 0; b &= b - 1) {
+        const float x = widen(row.s[row.ph + lane * kPer + __ffs(b) - 1]);
+        const double v = table(exponent(x));
+        mass += v;
+        above += x > from ? v : 0.0;
+      }
+      mass = warp_total(mass);
+      above = warp_total(above);
+      const double border = (double)s.top_p * mass;
+      for (t = from;;) {
+        float next = -CUDART_INF_F;
+        ties = 0;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+          const bool in = keep >> e & 1u;
+          ties += in && row.x[e] == t;
+          next = in && row.x[e] < t ? fmaxf(next, row.x[e]) : next;
+        }
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        next = key_value(__reduce_max_sync(0xffffffffu, order_key(next)));
+        const double each = table(exponent(t));
+        const double upto = above + (double)ties * each;
+        if (upto >= border || next == -CUDART_INF_F) {
+          const double n = each > 0.0 ? ceil((border - above) / each) : 1.0;
+          ties = (int)fmin(fmax(n, 1.0), (double)ties);
+          break;
+        }
+        above = upto;
+        t = next;
+      }
     }
     keep = row.head(keep, t, ties);
   }
@@ -1176,6 +1211,9 @@ __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
 // border is closer than twice that repeats it with 64-bit weights.  The kept
 // tokens' mass and the draw are in 64 bits, so their number sets the time on
 // the 64-bit pipe, not V.
+//
+// 524,288 x 21 f32, top-p and min-p: 47 us (8 us of memory traffic), 57 % of the
+// issue rate; taking the largest remaining token until the filters stop took 75.
 template <typename T, int kPad>
 __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __restrict__ logits,
                                                                   int64_t row_stride, int64_t n_rows,
@@ -1325,7 +1363,7 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const SampleArgs& a) {
     });
     return cudaGetLastError();
   }
-  if (v.vocab <= kWarpVocab) {
+  if (use_warp_rows(v.rows, v.vocab)) {
     const int smem = kWarpRows * WarpRow<T, 1>::bytes(v.vocab);
     const unsigned blocks = (unsigned)((v.rows + kWarpRows - 1) / kWarpRows);
     HKB_WARP_WIDTH(v.vocab, (sample_warp_kernel<T, kPer><<<blocks, 32 * kWarpRows, smem, st>>>(

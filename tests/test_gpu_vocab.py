@@ -756,3 +756,48 @@ def test_backward_is_the_fused_gradient(vocab, rows, size, dtype):
             (g2,) = torch.autograd.grad(l2, xr, w)
             assert torch.equal(l2.nan_to_num(-7.0), loss.nan_to_num(-7.0))
             assert torch.equal(g2.nan_to_num(-7.0), grad.nan_to_num(-7.0))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size", [225, 480, 481, 700, 992, 993, 5000])
+def test_thousand_rows(vocab, size, dtype):
+    edges = edge_rows(size, dtype)
+    n = len(edges)
+    x = torch.cat([logits(1100, size, dtype, size), edges])
+    at = torch.cat([torch.arange(4), torch.arange(1100 - 3, 1100 + n)]).cuda()
+    for f in FILTERS:
+        for v in (0.0, 0.3, 1.0):
+            u = torch.full((len(x),), v, device="cuda")
+            got = vocab.sample_tokens(x, u, **f)
+            check_sample([a[at] for a in got], x[at], u[at], **f)
+    for k in (1, 8, 100, min(size, 1024)):
+        got = vocab.top_logits(x, k)
+        check_top([a[at] for a in got], x[at], k)
+    y = x[:1100]
+    for tail in (False, True):
+        v, t, norm = teacher(y, 40, F32, 3, 1.5, tail)
+        loss, grad = vocab.distill_loss_and_grad(y, v, t, temperature=1.5, teacher_log_norm=norm)
+        assert torch.equal(vocab.distill_loss(y, v, t, temperature=1.5, teacher_log_norm=norm), loss)
+        few = at[:7]
+        check_distill(loss[few], grad[few], y[few], v[few], t[few],
+                      norm[few] if tail else None, 1.5)
+
+
+@pytest.mark.parametrize("size", [40, 225, 481, 992])
+def test_thousand_rows_near_borders(vocab, size):
+    # borders that 32 bits cannot place: neighbours in the type, a tail of
+    # weights below the sums' rounding, differences that overflow 32 bits
+    rows = 1100
+    g = gen(size)
+    step = torch.randint(0, 40, (rows, size), generator=g, device="cuda")
+    near = (torch.full((rows, size), 1.0, device="cuda").view(torch.int32) + step.int()).view(F32)
+    tail = -40.0 * torch.rand(rows, size, generator=g, device="cuda")
+    huge = torch.finfo(F32).max * (2 * torch.rand(rows, size, generator=g, device="cuda") - 1)
+    u = torch.rand(rows, generator=g, device="cuda", dtype=torch.float64)
+    at = torch.arange(0, rows, 41, device="cuda")
+    below = float(np.nextafter(np.float32(1), np.float32(0)))
+    for x, temperature in ((near, 1.0), (tail, 1.0), (huge, 2e38)):
+        for f in (dict(top_p=0.5), dict(top_p=0.9), dict(top_p=below),
+                  dict(top_k=size // 2, top_p=0.9)):
+            got = vocab.sample_tokens(x, u, temperature=temperature, **f)
+            check_sample([a[at] for a in got], x[at], u[at], temperature=temperature, **f)
