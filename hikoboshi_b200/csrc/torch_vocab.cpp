@@ -386,6 +386,9 @@ PyObject* loss_and_grad(PyObject*, PyObject* const* args, Py_ssize_t n) {
     o.loss = loss.data_ptr<float>();
     o.grad = grad->data_ptr();
     run(x, [&](int d, void* st) { return hkb_distill(d, &rows, &t, &o, st); });
+    // autograd refuses a backward pass that needs what was here before
+    if (args[6] != Py_None && !grad->is_inference())
+      grad->unsafeGetTensorImpl()->bump_version();
     return tuple_of({loss, *grad});
   });
 }

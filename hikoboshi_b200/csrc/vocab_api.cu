@@ -88,6 +88,15 @@ VocabRows internal_rows(const hkb_vocab_rows& v) {
   return {v.rows, v.vocab, v.dtype, v.logits, v.row_stride};
 }
 
+// Whether `n` rows of `width` elements, `stride` elements apart, share bytes with
+// the memory from `lo` to `hi`.
+bool meets(const void* p, int64_t n, int64_t stride, int64_t width, uintptr_t bytes, uintptr_t lo,
+           uintptr_t hi) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(p);
+  const uintptr_t end = first + (uintptr_t)((n - 1) * stride + width) * bytes;
+  return p != nullptr && first < hi && lo < end;
+}
+
 hkb_status check_distill(const hkb_vocab_rows* rows, const hkb_distill_teacher* t,
                          const hkb_distill_out* out) {
   const hkb_status st = check_rows(rows);
@@ -115,6 +124,23 @@ hkb_status check_distill(const hkb_vocab_rows* rows, const hkb_distill_teacher* 
         return invalid("grad must be the logits' own buffer or lie apart from it");
     }
   }
+  return {HKB_OK, ""};
+}
+
+// The gradient is written while the rest is read, so they must not meet.
+hkb_status check_apart(const hkb_vocab_rows& rows, const hkb_distill_teacher& t,
+                       const hkb_distill_out& out) {
+  if (out.grad == nullptr) return {HKB_OK, ""};
+  const int64_t n = rows.rows;
+  const uintptr_t g0 = reinterpret_cast<uintptr_t>(out.grad);
+  const uintptr_t g1 =
+      g0 + (uintptr_t)((n - 1) * out.grad_row_stride + rows.vocab) * elem_bytes(rows.dtype);
+  if (meets(t.values, n, t.k, t.k, elem_bytes(t.dtype), g0, g1) ||
+      meets(t.tokens, n, t.k, t.k, 4, g0, g1) || meets(t.log_norm, n, 1, 1, 4, g0, g1) ||
+      meets(out.row_weights, n, out.row_weight_stride, 1, 4, g0, g1) ||
+      meets(out.loss, n, 1, 1, 4, g0, g1) ||
+      meets(out.stats, n, HKB_DISTILL_STATS, HKB_DISTILL_STATS, 8, g0, g1))
+    return invalid("grad must lie apart from the teacher, the weights, the loss and the stats");
   return {HKB_OK, ""};
 }
 
@@ -213,6 +239,8 @@ hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill
     return invalid("loss or grad must be non-null");
   if (t->values == nullptr || t->tokens == nullptr)
     return invalid("teacher values and tokens must be non-null");
+  const hkb_status apart = check_apart(*rows, *t, *out);
+  if (apart.code != HKB_OK) return apart;
   DeviceGuard guard(device);
   if (guard.status().code != HKB_OK) return guard.status();
   return launched(launch_distill(static_cast<cudaStream_t>(stream), internal_rows(*rows),
@@ -229,6 +257,8 @@ hkb_status hkb_distill_backward(int device, const hkb_vocab_rows* rows,
     return invalid("a backward pass needs grad and stats");
   if (t->values == nullptr || t->tokens == nullptr)
     return invalid("teacher values and tokens must be non-null");
+  const hkb_status apart = check_apart(*rows, *t, *out);
+  if (apart.code != HKB_OK) return apart;
   DeviceGuard guard(device);
   if (guard.status().code != HKB_OK) return guard.status();
   return launched(launch_distill_backward(static_cast<cudaStream_t>(stream), internal_rows(*rows),

@@ -103,7 +103,9 @@ def distill_loss_and_grad(logits, teacher_values, teacher_tokens, *, teacher_log
     rows: the gradient of ``sum(row_weights * loss)`` with respect to ``logits``
     (weights 1 by default), in the logits' type.  A row of weight 0 has gradient
     0.  ``grad_out`` receives the gradient and may be ``logits`` itself, whose
-    memory the gradient then takes; autograd does not see this call."""
+    memory the gradient then takes; it lies apart from all other arguments.
+    Autograd does not record this call, but counts it as a change of
+    ``grad_out``."""
     return _vocab.loss_and_grad(logits, teacher_values, teacher_tokens, teacher_log_norm,
                                 temperature, row_weights, grad_out)
 

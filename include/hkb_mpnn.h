@@ -396,7 +396,8 @@ typedef struct {
  * A listed token whose student logit is -inf makes the loss +inf.
  *
  * grad may be the logits' own buffer (the same address, row stride and type);
- * any other overlap is not allowed, and rows must not overlap then. */
+ * any other overlap is not allowed, and rows must not overlap then.  It lies
+ * apart from the teacher's arrays, the weights, the loss and the stats. */
 hkb_status hkb_distill(int device, const hkb_vocab_rows* rows, const hkb_distill_teacher* teacher,
                        const hkb_distill_out* out, void* stream);
 

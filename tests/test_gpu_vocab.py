@@ -410,6 +410,19 @@ def test_gradient_in_place_of_the_logits(vocab, size, dtype):
     assert torch.equal(loss, loss2) and torch.equal(grad, y)
 
 
+def test_gradient_in_place_counts_as_a_change(vocab):
+    x = logits(7, 50, F32, 1)
+    v, t, _ = teacher(x, 5, F32, 3, 1.0, False)
+    x.requires_grad_()
+    y = x * 1.0
+    square = (y * y).sum()  # its backward pass needs y
+    before = y._version
+    vocab.distill_loss_and_grad(y.detach(), v, t, grad_out=y.detach())
+    assert y._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        square.backward()
+
+
 @pytest.mark.parametrize("size", [21, 5000])
 def test_broadcast_weights_and_shared_rows(vocab, size):
     x = logits(1, size, F32, 1)

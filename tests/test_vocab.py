@@ -93,6 +93,21 @@ def test_fused_outputs_are_checked(kwargs, text):
     refused(lambda: vocab.distill_loss_and_grad(X, TV, TT, **kwargs), text)
 
 
+def test_gradient_lies_apart_from_what_else_is_read_and_written():
+    x = torch.zeros(3, 21)
+    tokens = torch.zeros(3, 21, dtype=torch.int32)
+    # a student that is its own teacher, listed whole: the teacher's rows are the logits
+    refused(lambda: vocab.distill_loss_and_grad(x, x, tokens, grad_out=x), "apart from the teacher")
+    refused(lambda: vocab.distill_loss_and_grad(x, torch.ones(3, 21), tokens,
+                                                grad_out=tokens.view(torch.float32)),
+            "apart from the teacher")
+    buf = torch.zeros(70)
+    for name in ("row_weights", "teacher_log_norm"):
+        refused(lambda: vocab.distill_loss_and_grad(x, torch.ones(3, 21), tokens,
+                                                    grad_out=buf[:63].view(3, 21),
+                                                    **{name: buf[62:65]}), "apart from the teacher")
+
+
 def test_gradient_may_be_the_logits_but_not_overlap_them():
     buf = torch.zeros(4 * 21)
     x = buf[:63].view(3, 21)
