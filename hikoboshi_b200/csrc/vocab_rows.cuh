@@ -433,14 +433,29 @@ __device__ __forceinline__ int count_larger(const unsigned long long* item, int 
   return c;
 }
 
-// Sorts n <= kListCap items downwards (bitonic; the CTA's threads).
+// Sorts n <= kListCap items downwards: bitonic, the strides below 32 in registers
+// of a warp each.  All the CTA's threads call it, whole warps.
 __device__ __forceinline__ void sort_down(unsigned long long* item, int n) {
-  int size = 1;
+  const int warps = (int)blockDim.x >> 5, warp = (int)threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int size = 32;
   while (size < n) size <<= 1;
   for (int i = n + (int)threadIdx.x; i < size; i += blockDim.x) item[i] = 0;
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
+  auto exchange = [lane](unsigned long long v, int i, int k, int j) {
+    const unsigned long long o = __shfl_xor_sync(0xffffffffu, v, j);
+    return (((lane & j) == 0) == ((i & k) == 0)) == (v < o) ? o : v;
+  };
+  for (int i = warp * 32 + lane; i < size; i += warps * 32) {
+    unsigned long long v = item[i];
+#pragma unroll
+    for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) v = exchange(v, i, k, j);
+    item[i] = v;
+  }
+  __syncthreads();
+  for (int k = 64; k <= size; k <<= 1) {
+    for (int j = k >> 1; j >= 32; j >>= 1) {
       for (int p = threadIdx.x; p < size / 2; p += blockDim.x) {
         const int i = ((p & ~(j - 1)) << 1) | (p & (j - 1)), l = i | j;
         const unsigned long long a = item[i], b = item[l];
@@ -451,6 +466,13 @@ __device__ __forceinline__ void sort_down(unsigned long long* item, int n) {
       }
       __syncthreads();
     }
+    for (int i = warp * 32 + lane; i < size; i += warps * 32) {
+      unsigned long long v = item[i];
+#pragma unroll
+      for (int j = 16; j > 0; j >>= 1) v = exchange(v, i, k, j);
+      item[i] = v;
+    }
+    __syncthreads();
   }
 }
 

@@ -12,7 +12,7 @@ namespace {
 // Writes row r's listing: the first k of the n items of the CTA's list in order.
 template <typename T>
 __device__ __forceinline__ void write_listing(TokenList& list, int n, const T* g, int64_t r,
-                                              const TopArgs& a) {
+                                              const TopArgs& a, int by_count) {
   const int tid = threadIdx.x, threads = blockDim.x;
   T* values = static_cast<T*>(a.values) + r * a.k;
   int32_t* tokens = a.tokens + r * a.k;
@@ -20,7 +20,7 @@ __device__ __forceinline__ void write_listing(TokenList& list, int n, const T* g
     values[place] = g[index];
     tokens[place] = index;
   };
-  if (n <= 2 * threads) {
+  if (n <= by_count) {
     // an item's place is the number of larger ones, counted by a group of
     // threads
     int group = 32;
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
       return x > t || (x == t && i <= i_lo);
     });
   }
-  if (row.rank == 0) write_listing(sm.list, n, g, r, a);
+  if (row.rank == 0) write_listing(sm.list, n, g, r, a, 2 * (int)blockDim.x);
 }
 
 // Many rows: a CTA streams a row for its maxima and sum, then again, from L2, to
@@ -158,7 +158,49 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
 struct TopStreamSmem {
   ReduceScratch red;
   TokenList list;
+  int scan[kMaxWarps];
+  uint32_t bound;
 };
+
+// A lower bound of the k-th largest logit from the counts of the keys' upper 12
+// bits, in the list's memory; 0 if the row has fewer than k.
+constexpr int kTopBins = 4096;
+// Longest list that is ordered by counting larger items instead of sorting (5000 x
+// 8000 bf16 with 32 threads a row, top 40: 133 us, 143 with 48; top 128: 176, 182 with
+// 192).
+constexpr int kByCount = 96;
+static_assert(kTopBins * sizeof(int) <= kListCap * sizeof(unsigned long long), "");
+
+template <typename T>
+__device__ __forceinline__ uint32_t bound_by_counts(const RowStream<T>& row, TopStreamSmem& sm,
+                                                    int k) {
+  constexpr int kE = Vec<T>::kN;
+  int* bins = reinterpret_cast<int*>(sm.list.item);
+  const int tid = threadIdx.x, threads = blockDim.x, per = kTopBins / threads;
+  for (int i = tid; i < kTopBins; i += threads) bins[i] = 0;
+  if (tid == 0) sm.bound = 0;
+  __syncthreads();
+  row.template walk<1>([&](auto& x, int, int, bool, int) {
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const float y = x[0].at(e);
+      if (y > -CUDART_INF_F) atomicAdd(&bins[order_key(y) >> 20], 1);
+    }
+  });
+  __syncthreads();
+  // thread t sums the t-th share of the bins from the top
+  const int top = kTopBins - 1 - tid * per;
+  int mine = 0, all;
+  for (int i = 0; i < per; ++i) mine += bins[top - ((i + tid) & (per - 1))];  // in turn: banks
+  int above = block_scan(mine, sm.scan, &all) - mine;
+  if (above < k && above + mine >= k) {
+    int bin = top;
+    while (above + bins[bin] < k) above += bins[bin--];
+    sm.bound = (uint32_t)bin << 20;
+  }
+  __syncthreads();
+  return sm.bound;
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* __restrict__ logits,
@@ -211,6 +253,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* 
   uint32_t bound = 0;
   if (a.k <= threads / 2) {
     bound = reached_by(order_key(tmax), a.k);
+  } else if (threads < kStreamThreads) {
+    bound = bound_by_counts(row, sm, a.k);
   } else {
     for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
       int n = 0;
@@ -281,7 +325,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) top_stream_kernel(const T* 
     __syncthreads();
     n = a.k;
   }
-  write_listing(sm.list, n, g, r, a);
+  write_listing(sm.list, n, g, r, a, kByCount);
 }
 
 // Rows of up to kWarpVocab tokens, a warp each.  A short listing takes the
@@ -466,11 +510,18 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const TopArgs& a) {
     return cudaGetLastError();
   }
   if (use_stream(v.rows, v.vocab, (int)sizeof(T))) {
-    // twice as many threads as tokens wanted, where the row has work for them:
-    // the bound then comes from the threads' own maxima and is a close one
     int threads = stream_threads(v.vocab, (int)sizeof(T));
     const int vectors = v.vocab / (16 / (int)sizeof(T)) + 1;
-    while (threads < kStreamThreads && threads < 2 * a.k && threads < vectors) threads *= 2;
+    // Twice as many threads as tokens wanted, where the row has work for them: the
+    // bound then comes from the threads' own maxima.  Else it comes from counts.
+    // Measured (us), maxima and counts, bf16: 12,899 x 3,101, top 64: 160 and 229;
+    // top 128: 238 and 217; top 298: 991 and 342; 5000 x 8000, top 64: 82 and 154;
+    // top 128: 133 and 129; 2000 x 20000, top 128: 74 and 121; top 298: 139 and 111;
+    // 571 x 70000, top 298: 66 and 84; top 700: 139 and 92.  Counting with 128 and 256
+    // threads: 36,363 x 1100, top 298: 662 and 801; top 700: 1026 and 1169.
+    const bool by_maxima = a.k <= 64 ? 2 * a.k <= vectors : 16 * a.k <= vectors;
+    const int most = by_maxima ? kStreamThreads : 128;
+    while (threads < most && threads < (by_maxima ? 2 * a.k : a.k / 2)) threads *= 2;
     top_stream_kernel<T><<<(unsigned)v.rows, threads, 0, st>>>(
         static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
     return cudaGetLastError();
