@@ -338,8 +338,9 @@ __device__ __forceinline__ EntrySums shfl_xor(EntrySums v, int o) {
 namespace {
 
 // Of the entries of one token the first stands for it.
-__device__ __forceinline__ void own_first(const Listing& ls, int k_all) {
-  for (int k = threadIdx.x; k < k_all; k += blockDim.x) {
+__device__ __forceinline__ void own_first(const Listing& ls, int k_all, int tid,
+                                          int threads) {
+  for (int k = tid; k < k_all; k += threads) {
     if (ls.token[k] < 0) continue;
     int first = 0;
     while (ls.token[first] != ls.token[k]) ++first;
@@ -347,14 +348,20 @@ __device__ __forceinline__ void own_first(const Listing& ls, int k_all) {
   }
 }
 
+constexpr int kTeamThreads = 128;  // of a CTA whose rows are its teams'
+
+template <int kTeam>
 struct StreamSmem {
   ReduceScratch red;
   Exp2Table table;
-  RowFactors f;
-  EntrySums sums;
+  struct {
+    RowFactors f;
+    EntrySums sums;
+  } row[kTeam ? kTeamThreads / (kTeam ? kTeam : 1) : 1];
 };
 
-// Many rows: a CTA streams a row for its sum, then again for the gradient.  The
+// Many rows: a CTA, or a team of lanes, streams a row for its sum, then again for
+// the gradient.  The
 // listed tokens are marked in a bit map in the phase of the row's vectors, a
 // vector's marks in one byte or half a byte, so that the first pass leaves them
 // out where the unlisted ones form a class; the entry that sets a mark stands
@@ -363,26 +370,32 @@ struct StreamSmem {
 // 4096 x 131072 bf16, loss and gradient: 503 us, 4.3 TB/s, DRAM 73 % and XU 54 %
 // busy (1072 with the row in a cluster's shared memory); 1024 x 32768 f32, loss: 33
 // us, 4.1 TB/s.
-template <typename T>
-__global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const T* logits,
-                                                                           int64_t row_stride,
-                                                                           int vocab,
-                                                                           DistillArgs a) {
+template <typename T, int kTeam>
+__global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ? 8 : 2)
+    distill_stream_kernel(const T* logits, int64_t row_stride, int64_t n_rows, int vocab,
+                          int row_bytes, DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ StreamSmem sm;
+  __shared__ StreamSmem<kTeam> sm;
   constexpr int kE = Vec<T>::kN, kU = 4;
-  const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x, threads = blockDim.x;
+  Team<kTeam> team(&sm.red);
+  const int tid = team.rank(), threads = team.size();
+  const int own_row = kTeam ? (int)threadIdx.x / (kTeam ? kTeam : 1) : 0;
+  auto& mine = sm.row[own_row];
+  const int64_t r = kTeam ? (int64_t)blockIdx.x * (kTeamThreads / (kTeam ? kTeam : 1)) + own_row
+                          : (int64_t)blockIdx.x;
+  sm.table.fill();
+  if (kTeam) {
+    __syncthreads();
+    if (r >= n_rows) return;
+  }
   const T* g = logits + r * row_stride;
   const RowStream<T> row(g, vocab);
   Listing ls;  // q holds masses up to the factor q_scale
-  ls.q = reinterpret_cast<double*>(smem_raw);
+  ls.q = reinterpret_cast<double*>(smem_raw + own_row * row_bytes);
   ls.x = reinterpret_cast<float*>(ls.q + a.k);
   ls.token = reinterpret_cast<int*>(ls.x + a.k);
   ls.own = ls.token + a.k;
   uint32_t* marks = reinterpret_cast<uint32_t*>(ls.own + a.k);
-  Reducer<false> red(&sm.red);
-  sm.table.fill();
 
   const bool tail = a.log_norm != nullptr;
   T* grad = a.grad ? static_cast<T*>(a.grad) + r * a.grad_row_stride : nullptr;
@@ -404,7 +417,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     ls.x[k] = v;
   }
   const unsigned long long head =
-      red.all(((unsigned long long)order_key(amax) << 32) | flags,
+      team.all(((unsigned long long)order_key(amax) << 32) | flags,
               [](unsigned long long p, unsigned long long q) {
                 return (p > q ? p : q) | (p & 3) | (q & 3);
               });
@@ -434,13 +447,13 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     // The marks are read in the first pass.  Of a token's entries any may stand
     // for it where only its gradient is written; in a sum it is the first, so
     // that the sum does not change from run to run.
-    if (tail && __syncthreads_or(twice_here)) own_first(ls, a.k);
+    if (tail && team.any(twice_here)) own_first(ls, a.k, tid, threads);
   }
 
   const double inv_tau = a.inv_temperature;
   const float c = a.c;
   SoftSum soft;
-  row.template walk<kU>([&](auto& x, int v, int step, bool, int) {
+  row.template walk<kU, kTeam>([&](auto& x, int v, int step, bool, int) {
     if (tail) {
       constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
@@ -463,7 +476,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     ls.q[k] = (double)x;
     sum.lmax = fmaxf(sum.lmax, x);
   }
-  sum = red.all(sum, [c](RowSum p, RowSum q) {
+  sum = team.all(sum, [c](RowSum p, RowSum q) {
     return RowSum{SoftSum::join(p.soft, q.soft, c), fmaxf(p.lmax, q.lmax)};
   });
   const float bmax = sum.soft.m, xmax = fmaxf(bmax, sum.lmax);
@@ -482,7 +495,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
     ls.x[k] = (float)ls.q[k];
     ls.q[k] = q;
   }
-  sums = red.all(sums, [](EntrySums p, EntrySums q) {
+  sums = team.all(sums, [](EntrySums p, EntrySums q) {
     return EntrySums{p.q + q.q, p.dot + q.dot, p.listed + q.listed, p.twice | q.twice};
   });
   const double q_scale = tail ? 1.0 : 1.0 / sums.q;
@@ -490,8 +503,8 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
                                    a.temperature, weight);
   if (tid == 0) {
     // what the list and the loss need waits in shared memory
-    sm.f = f;
-    sm.sums = sums;
+    mine.f = f;
+    mine.sums = sums;
     if (a.stats)
       write_stats(a.stats, r, f, q_scale, xmax, tail ? 0.0f : amax, sums.twice ? kStatTwice : 0);
   }
@@ -509,7 +522,7 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
   const bool same_phase = (reinterpret_cast<uintptr_t>(gv) & 15) == 0;
   const float2 minus = make_float2(-f.base, -f.base), scale = make_float2(c, c),
                G = make_float2((float)(f.Q * f.F), (float)(f.Q * f.F));
-  row.template walk<kU>([&](auto& x, int v, int step, bool whole, int) {
+  row.template walk<kU, kTeam>([&](auto& x, int v, int step, bool whole, int) {
     constexpr int n = sizeof(x) / sizeof(x[0]);
 #pragma unroll
     for (int u = 0; u < n; ++u) {
@@ -529,9 +542,9 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
       }
     }
   });
-  __syncthreads();
-  const bool twice = sm.sums.twice;
-  const double sum_q = sm.sums.q, scale_q = tail ? 1.0 : 1.0 / sum_q;
+  team.sync();
+  const bool twice = mine.sums.twice;
+  const double sum_q = mine.sums.q, scale_q = tail ? 1.0 : 1.0 / sum_q;
   for (int k = tid; k < a.k; k += threads) {
     if (ls.token[k] < 0 || !ls.own[k]) continue;
     double q = ls.q[k];
@@ -541,12 +554,12 @@ __global__ void __launch_bounds__(kStreamThreads, 2) distill_stream_kernel(const
         if (ls.token[j] == ls.token[k]) q += ls.q[j];
     }
     const double e = exp(((double)ls.x[k] - (double)xmax) * inv_tau);
-    grad[ls.token[k]] = narrow<T>((float)listed_gradient(sm.f.Q, sm.f.each, e, q * scale_q));
+    grad[ls.token[k]] = narrow<T>((float)listed_gradient(mine.f.Q, mine.f.each, e, q * scale_q));
   }
   // the last warp has fewest entries to see to
   if (tid == threads - 1 && a.loss) {
-    const double dot = tail ? sm.sums.dot : sm.sums.dot * scale_q - log(sum_q);
-    a.loss[r] = row_loss(sm.f, dot, bmax, xmax, body, inv_tau, a.temperature);
+    const double dot = tail ? mine.sums.dot : mine.sums.dot * scale_q - log(sum_q);
+    a.loss[r] = row_loss(mine.f, dot, bmax, xmax, body, inv_tau, a.temperature);
   }
 }
 
@@ -799,6 +812,28 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
   sr.store(static_cast<T*>(a.grad) + r0 * a.grad_row_stride, a.grad_row_stride);
 }
 
+// A row of a few hundred tokens costs a warp some 1400 instructions, most of them
+// the same for any V: the reductions, the masses' sums and logarithms.  Teams of 4
+// or 8 lanes share them, when there are rows for two CTAs a SM.  More entries
+// than four (sixteen) a lane take it back; a lane adds at most 128 weights.  Measured
+// (us), loss and gradient, bf16, a CTA, 4 and 8 lanes a row: 100,000 x 40, 10
+// entries: 184, 41 and 63; 40 entries: 213, 84 and 86; 100,000 x 400, 10: 209, 78 and
+// 98; 40: 246, 139 and 127; 120: 369 and 305 with 8; 10,000 x 400, 10: 29, 20 and 18;
+// 2400 x 400, 10: 12, 16 and 14.
+template <int kTeam>
+bool use_team(const VocabRows& v, int k) {
+  return v.vocab <= (kTeam == 4 ? 512 : 31 * 32) && k <= (kTeam == 4 ? 16 : 128) &&
+         v.rows >= 2 * 148 * (kTeamThreads / kTeam);
+}
+template <typename T, int kTeam>
+cudaError_t launch_teams(cudaStream_t st, const VocabRows& v, const DistillArgs& a, int row_bytes) {
+  constexpr int kTeams = kTeamThreads / kTeam;
+  distill_stream_kernel<T, kTeam>
+      <<<(unsigned)((v.rows + kTeams - 1) / kTeams), kTeamThreads, row_bytes * kTeams, st>>>(
+          static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, row_bytes, a);
+  return cudaGetLastError();
+}
+
 template <typename T>
 cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   if (v.vocab <= kShortVocab) {
@@ -811,12 +846,14 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   if (use_stream(v.rows, v.vocab, (int)sizeof(T))) {
     // bits of a row in its vectors' phase, in whole words
     const int words = (v.vocab + 16 / (int)sizeof(T) - 1 + 31) / 32;
-    const int smem = a.k * 20 + words * 4;
-    ensure_dynamic_smem((const void*)distill_stream_kernel<T>,
+    const int bytes = (a.k * 20 + words * 4 + 7) / 8 * 8;
+    if (use_team<4>(v, a.k)) return launch_teams<T, 4>(st, v, a, bytes);
+    if (use_team<8>(v, a.k)) return launch_teams<T, 8>(st, v, a, bytes);
+    ensure_dynamic_smem((const void*)distill_stream_kernel<T, 0>,
                         HKB_LISTING_MAX * 20 + HKB_VOCAB_MAX / 8 + 8);
-    distill_stream_kernel<T>
-        <<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), smem, st>>>(
-            static_cast<const T*>(v.logits), v.row_stride, v.vocab, a);
+    distill_stream_kernel<T, 0>
+        <<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), bytes, st>>>(
+            static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, 0, a);
     return cudaGetLastError();
   }
   const RowShape s = row_shape(v.rows, v.vocab, (int)sizeof(T));

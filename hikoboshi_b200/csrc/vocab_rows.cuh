@@ -545,12 +545,14 @@ struct RowStream {
   // f(x, v, step, whole, slot) over the CTA's threads: x an array of vectors v,
   // v + step, ..., in the slots slot, slot + 1, ... of kU that a thread's vectors
   // take in turn.  The next kU loads are in flight while f works on kU vectors; the
-  // ends of the row that fill no vector come last, one vector each.
-  template <int kU, typename F>
+  // ends of the row that fill no vector come last, one vector each.  With kTeam
+  // the row is a team's of that many lanes, not the CTA's.
+  template <int kU, int kTeam = 0, typename F>
   __device__ __forceinline__ void walk(F f) const {
-    const int threads = blockDim.x;
+    const int threads = kTeam ? kTeam : (int)blockDim.x;
+    const int tid = kTeam ? (int)threadIdx.x % (kTeam ? kTeam : 1) : (int)threadIdx.x;
     const Vec<T>* vec = reinterpret_cast<const Vec<T>*>(g);
-    int v = lo + (int)threadIdx.x;
+    int v = lo + tid;
     if (v + (kU - 1) * threads < hi) {
       Vec<T> y[kU];
 #pragma unroll
@@ -572,12 +574,57 @@ struct RowStream {
         Vec<T> x[1] = {vec[v + u * threads]};
         f(x, v + u * threads, threads, true, u);
       }
-    if ((threadIdx.x == 0 && lo > 0) ||
-        ((int)threadIdx.x == threads - 1 && hi >= lo && hi * kE < end)) {
-      const int at = threadIdx.x == 0 && lo > 0 ? 0 : hi;
+    if ((tid == 0 && lo > 0) || (tid == threads - 1 && hi >= lo && hi * kE < end)) {
+      const int at = tid == 0 && lo > 0 ? 0 : hi;
       Vec<T> x[1] = {partial(at)};
       f(x, at, threads, false, kU - 1);
     }
+  }
+};
+
+// The threads that share a row: the CTA, or kTeam neighbouring lanes, of which a
+// warp then has several, each at its own place in the code.
+template <int kTeam>
+struct Team {
+  unsigned mask;
+  __device__ __forceinline__ explicit Team(ReduceScratch*)
+      : mask((kTeam == 32 ? 0xffffffffu : (1u << (kTeam & 31)) - 1u)
+             << (threadIdx.x & 31 & ~(unsigned)(kTeam - 1))) {}
+  __device__ __forceinline__ int rank() const { return threadIdx.x & (kTeam - 1); }
+  __device__ __forceinline__ int size() const { return kTeam; }
+  __device__ __forceinline__ void sync() const { __syncwarp(mask); }
+  __device__ __forceinline__ bool any(bool p) const {
+    __syncwarp(mask);
+    return __any_sync(mask, p);
+  }
+  template <typename V, typename Op>
+  __device__ __forceinline__ V all(V v, Op op) const {
+    static_assert(sizeof(V) % 4 == 0, "moved as words");
+#pragma unroll
+    for (int o = kTeam / 2; o > 0; o >>= 1) {
+      unsigned w[sizeof(V) / 4];
+      memcpy(w, &v, sizeof(V));
+#pragma unroll
+      for (unsigned& x : w) x = __shfl_xor_sync(mask, x, o);
+      V y;
+      memcpy(&y, w, sizeof(V));
+      v = op(v, y);
+    }
+    __syncwarp(mask);
+    return v;
+  }
+};
+template <>
+struct Team<0> {
+  Reducer<false> red;
+  __device__ __forceinline__ explicit Team(ReduceScratch* s) : red(s) {}
+  __device__ __forceinline__ int rank() const { return threadIdx.x; }
+  __device__ __forceinline__ int size() const { return blockDim.x; }
+  __device__ __forceinline__ void sync() const { __syncthreads(); }
+  __device__ __forceinline__ bool any(bool p) const { return __syncthreads_or(p); }
+  template <typename V, typename Op>
+  __device__ __forceinline__ V all(V v, Op op) {
+    return red.all(v, op);
   }
 };
 

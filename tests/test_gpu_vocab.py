@@ -814,3 +814,60 @@ def test_thousand_rows_near_borders(vocab, size):
                   dict(top_k=size // 2, top_p=0.9)):
             got = vocab.sample_tokens(x, u, temperature=temperature, **f)
             check_sample([a[at] for a in got], x[at], u[at], temperature=temperature, **f)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("size,offset", [(33, 0), (33, 1), (40, 3), (96, 0), (241, 5), (300, 0), (512, 1), (600, 1),
+                                         (992, 0)])
+def test_distill_thousands_of_short_rows(vocab, size, offset, dtype):
+    # several rows to a warp; the last CTA is not full
+    rows, k = 9503, 12
+    pitch = size + 2 * offset
+    base = logits(1, rows * pitch + offset, dtype, 2)[0]
+    x = base[offset:].view(rows, pitch)[:, :size]
+    v, t, norm = teacher(x, k, F32, 3, 1.5, True)
+    t[0] = -1
+    t[1, 3:] = -1
+    t[2, 4] = t[2, 9]
+    t[3, :] = t[3, 0]
+    v[4, 5:] = -INF
+    v[5] = -INF
+    t[6, 2] = size
+    x[0] = float("nan")
+    x[7, t[7, 1].long()] = -INF
+    x[8] = -INF
+    x[9, 5] = float("nan")
+    x[10, 7] = INF
+    x[11] = torch.finfo(dtype).min
+    v[12, 3] = float("nan")
+    w = torch.rand(rows, generator=gen(1), device="cuda") + 0.5
+    w[14] = 0.0
+    at = torch.tensor([1, 2, 3, 4, 11, 13, 14, 15, 77, rows - 2, rows - 1], device="cuda")
+    for n in (None, norm):
+        kw = dict(teacher_log_norm=n, temperature=1.5)
+        loss, grad = vocab.distill_loss_and_grad(x, v, t, row_weights=w, **kw)
+        assert loss[0] == 0 and (grad[0] == 0).all() and loss[5] == 0 and (grad[5] == 0).all()
+        assert loss[7] == INF and (grad[14] == 0).all()
+        for r in (6, 8, 9, 10, 12):
+            assert loss[r].isnan() and grad[r].isnan().all(), r
+        check_distill(loss[at], grad[at], x[at], v[at], t[at], None if n is None else n[at], 1.5,
+                      w[at])
+        again = vocab.distill_loss(x, v, t, **kw)
+        assert torch.equal(again.nan_to_num(-7.0), loss.nan_to_num(-7.0))
+        # in place, and through autograd
+        other = base.clone()
+        y = other[offset:].view(rows, pitch)[:, :size]
+        vocab.distill_loss_and_grad(y, v, t, row_weights=w, grad_out=y, **kw)
+        assert torch.equal(y.nan_to_num(-7.0), grad.nan_to_num(-7.0))
+        if offset:  # what lies between the rows stays
+            assert torch.equal(other[offset:].view(rows, pitch)[:, size:],
+                               base[offset:].view(rows, pitch)[:, size:])
+        z = x.detach().requires_grad_()
+        (g2,) = torch.autograd.grad(vocab.distill_loss(z, v, t, **kw), z, w)
+        assert torch.equal(g2.nan_to_num(-7.0), grad.nan_to_num(-7.0))
+    # from the shortest listing to the longest
+    for n in sorted({1, 17, 33, min(size, 128), size}):
+        v, t, norm = teacher(x[16:], n, F32, 5, 1.0, True)
+        loss, grad = vocab.distill_loss_and_grad(x[16:], v, t, teacher_log_norm=norm)
+        few = torch.tensor([0, 1, 2, rows - 18, rows - 17], device="cuda")
+        check_distill(loss[few], grad[few], x[16:][few], v[few], t[few], norm[few], 1.0)
