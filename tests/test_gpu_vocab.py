@@ -871,3 +871,25 @@ def test_distill_thousands_of_short_rows(vocab, size, offset, dtype):
         loss, grad = vocab.distill_loss_and_grad(x[16:], v, t, teacher_log_norm=norm)
         few = torch.tensor([0, 1, 2, rows - 18, rows - 17], device="cuda")
         check_distill(loss[few], grad[few], x[16:][few], v[few], t[few], norm[few], 1.0)
+
+
+@pytest.mark.parametrize("size", [1500, 4000, 131072])
+def test_sample_from_long_lists_of_neighbours(vocab, size):
+    # heads of 193 to 2048 tokens whose indices lie close together, next to one far off
+    g = gen(size)
+    rows = 6
+    x = torch.full((rows, size), -60.0, device="cuda")
+    for r, (lo, n) in enumerate(((0, 300), (700, 500), (size - 260, 260), (5, 200), (100, 1200),
+                                 (250, 400))):
+        n = min(n, size - lo)
+        x[r, lo:lo + n] = torch.rand(n, generator=g, device="cuda")
+    x[3, size - 1] = 0.5
+    x[5, 250:650] = 0.25  # equal logits
+    for u in (0.0, 0.1, 0.5, 0.93, 1.0):
+        us = torch.full((rows,), u, device="cuda", dtype=torch.float64)
+        for f in (dict(top_p=0.9), dict(top_p=0.999), dict(top_k=250), dict(top_k=1000, top_p=0.95),
+                  dict(top_p=0.97, min_p=0.5)):
+            got = vocab.sample_tokens(x, us, **f)
+            check_sample(got, x, us, **f)
+            again = vocab.sample_tokens(x, us, **f)
+            assert all(torch.equal(p, q) for p, q in zip(got, again))
