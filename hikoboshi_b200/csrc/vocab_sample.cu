@@ -1046,8 +1046,9 @@ __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
     at = warp_total(at);
     over = warp_total(over);
     ties = __reduce_add_sync(0xffffffffu, ties);
-    // 32-bit differences of logits may overflow at the largest temperatures
-    const bool blind = s.temperature > 1e30f;
+    // 32 bits see nothing where differences of logits overflow them (the largest
+    // temperatures) or their scale does (below 4.24e-39: 0 * inf is NaN)
+    const bool blind = s.temperature > 1e30f || c == CUDART_INF_F;
     if (blind || ties > 1 || !(at - need > slack && need - over > slack)) {
       // In 64 bits: from the largest value that 32 bits cannot rule out (or the
       // row's largest) down, value by value, until the mass is reached or no
@@ -1240,7 +1241,8 @@ __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __res
       const float need = s.top_p * sum, slack = 4e-6f * sum;
       unsigned head = 0;
       float run = 0.0f;
-      bool close = s.temperature > 1e30f;  // 32-bit differences of logits may overflow
+      // 32-bit differences of logits may overflow, or their scale
+      bool close = s.temperature > 1e30f || c == CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < kPad; ++j) {
         if (j >= nk || (j > 0 && !(run < need))) break;
