@@ -36,6 +36,17 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, int64_t i)
   return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
+// Whether an entry makes its row NaN: a token outside the vocabulary, or a value
+// that is NaN or +inf (one of -inf is no entry).  Tested before the masses are
+// taken: with an infinite log-norm or value they would be 0 or inf, and the row's
+// loss a number that stands for nothing.
+__device__ __forceinline__ bool bad_entry(int token, float v, int vocab) {
+  return token >= vocab || !(v < CUDART_INF_F);
+}
+// Likewise the log-norm of a row with entries.
+__device__ __forceinline__ bool bad_norm(const float* log_norm, int64_t r) {
+  return log_norm != nullptr && !(fabsf(log_norm[r]) < CUDART_INF_F);
+}
 
 // What a row's loss and gradient need beside the row.
 struct RowFactors {
@@ -147,13 +158,14 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
     int token = a.tokens[r * a.k + k];
     if (token < 0 || v == -CUDART_INF_F) token = -1;
-    bad |= token >= vocab;
+    bad |= token >= 0 && bad_entry(token, v, vocab);
     any |= token >= 0;
     if (token >= 0) amax = fmaxf(amax, v);
     ls.token[k] = token;
     ls.x[k] = v;
   }
-  const bool row_bad = __syncthreads_or(bad), row_any = __syncthreads_or(any);
+  const bool row_any = __syncthreads_or(any);
+  const bool row_bad = __syncthreads_or(bad) || (row_any && bad_norm(a.log_norm, r));
   cp_async_wait_all();
   if (kClustered) cg::this_cluster().sync();
   else __syncthreads();
@@ -403,14 +415,14 @@ __global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ?
   const bool marked = tail || grad != nullptr || a.stats != nullptr;
   if (marked)
     for (int w = tid; w < (row.end + 31) / 32; w += threads) marks[w] = 0;
-  unsigned flags = 0;  // 1: an entry, 2: a token outside the vocabulary
+  unsigned flags = 0;  // 1: an entry, 2: a bad one
   float amax = -CUDART_INF_F;
   for (int k = tid; k < a.k; k += threads) {
     const float v = load_value(a.values, a.teacher_dtype, r * a.k + k);
     int token = a.tokens[r * a.k + k];
     if (token < 0 || v == -CUDART_INF_F) token = -1;
     if (token >= 0) {
-      flags |= token < vocab ? 1u : 2u;
+      flags |= bad_entry(token, v, vocab) ? 2u : 1u;
       amax = fmaxf(amax, v);
     }
     ls.token[k] = token;
@@ -421,7 +433,7 @@ __global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ?
               [](unsigned long long p, unsigned long long q) {
                 return (p > q ? p : q) | (p & 3) | (q & 3);
               });
-  const bool row_bad = head & 2, row_any = head & 1;
+  const bool row_any = head & 1, row_bad = head & 2 || (row_any && bad_norm(a.log_norm, r));
   if (row_bad || !row_any) {
     const float v = row_bad ? CUDART_NAN_F : 0.0f;
     if (tid == 0 && a.loss) a.loss[r] = v;
@@ -718,10 +730,11 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
   if (tid < rows)
     for_each_entry(a, r, [&](float v, int token) {
       if (token < 0 || v == -CUDART_INF_F) return;
-      bad |= token >= vocab;
+      bad |= bad_entry(token, v, vocab);
       listed |= token < vocab ? 1u << token : 0u;
       amax = fmaxf(amax, v);
     });
+  if (tid < rows && listed != 0) bad |= bad_norm(a.log_norm, r);
   cp_async_wait_all();
   __syncthreads();
   if (tid < rows) {

@@ -86,7 +86,9 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     their true masses and all others form one class with what is left, against
     the student's mass outside the list.  A negative token or a value of -inf is
     no entry; a row without entries has loss and gradient 0 whatever its logits.
-    A token >= V makes its row NaN.  ``temperature`` is 1e-30 to 1e30.
+    A token >= V makes its row NaN, and so do an entry's value that is NaN or +inf,
+    a log-norm that is not finite, a NaN or +inf logit, and a row of logits without
+    one above -inf.  ``temperature`` is 1e-30 to 1e30.
 
     The loss is differentiable once.  The backward pass reads ``logits`` and the
     teacher's tensors again, so they must not be overwritten before it.

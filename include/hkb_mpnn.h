@@ -391,8 +391,8 @@ typedef struct {
  *
  * A row without entries has loss 0 and gradient 0 whatever its logits are, and
  * a row of weight 0 has gradient 0.  A token >= vocab makes its row's loss and
- * gradient NaN; so do a NaN or +inf logit, teacher value or log_norm, and a
- * row with no logit above -inf.
+ * gradient NaN; so do an entry's value that is NaN or +inf, a log_norm that is not
+ * finite, a NaN or +inf logit, and a row with no logit above -inf.
  * A listed token whose student logit is -inf makes the loss +inf.
  *
  * grad may be the logits' own buffer (the same address, row stride and type);
