@@ -105,8 +105,9 @@ hkb_status check_distill(const hkb_vocab_rows* rows, const hkb_distill_teacher* 
   if (t->k < 1 || t->k > HKB_LISTING_MAX)
     return invalid("a row's listing must have 1 to HKB_LISTING_MAX entries");
   if (!real_dtype(t->dtype)) return invalid("teacher values must be F32, F16 or BF16");
-  if (!(t->temperature >= HKB_TEMPERATURE_MIN && t->temperature <= HKB_TEMPERATURE_MAX))
-    return invalid("temperature must be 1e-30 to 1e30");
+  if (!(t->temperature >= HKB_TEMPERATURE_MIN &&
+        t->temperature <= HKB_DISTILL_TEMPERATURE_MAX))
+    return invalid("temperature must be 1e-30 to 1e4");
   if (out->row_weight_stride < 0) return invalid("the row weight stride must not be negative");
   if (out->grad != nullptr) {
     if (out->grad_row_stride < rows->vocab)

@@ -8,6 +8,8 @@
 // lose it to cancellation.  The gradient is e_i G for every unlisted token,
 // with e_i recomputed from the row in shared memory and one factor G per row,
 // and is set entry by entry on the list.
+#include <type_traits>
+
 #include "hkb_mpnn.h"
 #include "kernels.hpp"
 #include "vocab.hpp"
@@ -18,6 +20,17 @@ namespace vocab {
 namespace {
 
 constexpr double kLog2e = 1.4426950408889634074;
+
+// The loss carries temperature^2 and the listed gradient temperature, while the
+// divergence itself falls with them: an error of the row's sum of weights, up to
+// 2e-7 with 32-bit exponentials, comes out as temperature^2 times that.  At 16
+// that is 5e-5 of a loss of about one, at 100 a thousandth, at 1e4 nothing is
+// left.  Above kWideTemperature the weights and their sums are therefore 64-bit
+// (kWide): off by temperature^2 * 1e-14 at most, 1e-6 at the largest temperature
+// that is accepted.  What that costs (us, loss and gradient, 32 and 64 bits):
+// 524,288 x 21 f32 53 and 87; 100,000 x 100 bf16 49 and 78; 48 x 1009 f16 11 and 12;
+// 2000 x 50001 bf16 103 and 287; 4096 x 131072 bf16 488 and 1139.
+constexpr double kWideTemperature = 16.0;
 
 template <int kBytes>
 struct BitsOf;
@@ -106,6 +119,46 @@ __device__ __forceinline__ float row_loss(const RowFactors& f, double dot, float
   return (float)(temperature * temperature * l);
 }
 
+// exp((x - ref) / tau) in 64 bits for x <= ref, c2 = log2(e) / tau; NaN for a NaN
+// and for x = ref = +-inf.
+__device__ __forceinline__ double wide_weight(float x, float ref, double c2,
+                                              const Exp2Table& table) {
+  const double t = ((double)x - (double)ref) * c2;
+  return t <= 0.0 ? table(t) : t;
+}
+
+// SoftSum in 64 bits.
+struct WideSum {
+  float m;
+  double s;
+
+  __device__ __forceinline__ WideSum() : m(-INFINITY), s(0.0) {}
+
+  template <typename T, int kU>
+  __device__ __forceinline__ void add(Vec<T> (&x)[kU], double c2, const Exp2Table& table) {
+    float vm = x[0].largest();
+#pragma unroll
+    for (int u = 1; u < kU; ++u) vm = fmaxf(vm, x[u].largest());
+    if (vm > m) {
+      s *= table(((double)m - (double)vm) * c2);
+      m = vm;
+    }
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < kU; ++u)
+#pragma unroll
+      for (int e = 0; e < Vec<T>::kN; ++e) s += wide_weight(x[u].at(e), ref, c2, table);
+  }
+  __device__ __forceinline__ static WideSum join(WideSum a, WideSum b, double c2) {
+    WideSum r;
+    r.m = fmaxf(a.m, b.m);
+    const double fa = a.m == r.m ? 1.0 : exp2(((double)a.m - (double)r.m) * c2);
+    const double fb = b.m == r.m ? 1.0 : exp2(((double)b.m - (double)r.m) * c2);
+    r.s = __dadd_rn(__dmul_rn(a.s, fa), __dmul_rn(b.s, fb));
+    return r;
+  }
+};
+
 struct DistillSmem {
   ReduceScratch cluster;
   ReduceScratch block;
@@ -128,7 +181,7 @@ __device__ void fill_slice(const RowSlice<T, kClustered>& row, T* grad, float va
 
 // Few rows, in the shared memory of a CTA or a cluster: bound by latency (48 x
 // 1009 f16: 10 us).
-template <typename T, bool kClustered>
+template <typename T, bool kClustered, bool kWide>
 __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
     const T* logits, int64_t row_stride, int vocab, int chunk, int slice_bytes, DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -247,10 +300,13 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
   const float xmax = fmaxf(bmax, listed_max);
   const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
   const float c = a.c;
-  float s = 0.0f;
+  std::conditional_t<kWide, double, float> s = 0;
   row.for_each([&](int, const Vec<T>& x) {
 #pragma unroll
-    for (int e = 0; e < kE; ++e) s += exp2_fast((x.at(e) - base) * c);
+    for (int e = 0; e < kE; ++e) {
+      if constexpr (kWide) s += wide_weight(x.at(e), base, kLog2e * inv_tau, sm.table);
+      else s += exp2_fast((x.at(e) - base) * c);
+    }
   });
   double listed = 0.0;  // sum over listed tokens exp((x - xmax) / tau)
   for (int k = threadIdx.x; k < a.k; k += blockDim.x) {
@@ -316,8 +372,9 @@ __global__ void __launch_bounds__(kMaxThreads, 2) distill_rows_kernel(
 
 
 // A row's sum and its largest listed logit.
+template <typename Sum>
 struct RowSum {
-  SoftSum soft;
+  Sum soft;
   float lmax;
 };
 
@@ -332,7 +389,20 @@ struct EntrySums {
 }  // namespace
 
 template <>
-__device__ __forceinline__ RowSum shfl_xor(RowSum v, int o) {
+__device__ __forceinline__ WideSum shfl_xor(WideSum v, int o) {
+  WideSum r;
+  r.m = __shfl_xor_sync(0xffffffffu, v.m, o);
+  r.s = __shfl_xor_sync(0xffffffffu, v.s, o);
+  return r;
+}
+template <>
+__device__ __forceinline__ RowSum<SoftSum> shfl_xor(RowSum<SoftSum> v, int o) {
+  v.soft = shfl_xor(v.soft, o);
+  v.lmax = __shfl_xor_sync(0xffffffffu, v.lmax, o);
+  return v;
+}
+template <>
+__device__ __forceinline__ RowSum<WideSum> shfl_xor(RowSum<WideSum> v, int o) {
   v.soft = shfl_xor(v.soft, o);
   v.lmax = __shfl_xor_sync(0xffffffffu, v.lmax, o);
   return v;
@@ -382,7 +452,7 @@ struct StreamSmem {
 // 4096 x 131072 bf16, loss and gradient: 503 us, 4.3 TB/s, DRAM 73 % and XU 54 %
 // busy (1072 with the row in a cluster's shared memory); 1024 x 32768 f32, loss: 33
 // us, 4.1 TB/s.
-template <typename T, int kTeam>
+template <typename T, int kTeam, bool kWide>
 __global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ? 8 : 2)
     distill_stream_kernel(const T* logits, int64_t row_stride, int64_t n_rows, int vocab,
                           int row_bytes, DistillArgs a) {
@@ -464,7 +534,8 @@ __global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ?
 
   const double inv_tau = a.inv_temperature;
   const float c = a.c;
-  SoftSum soft;
+  using Sum = std::conditional_t<kWide, WideSum, SoftSum>;
+  Sum soft;
   row.template walk<kU, kTeam>([&](auto& x, int v, int step, bool, int) {
     if (tail) {
       constexpr int n = sizeof(x) / sizeof(x[0]);
@@ -478,18 +549,23 @@ __global__ void __launch_bounds__(kTeam ? kTeamThreads : kStreamThreads, kTeam ?
             if (m >> e & 1u) x[u].clear(e);
       }
     }
-    soft.add(x, c);
+    if constexpr (kWide) soft.add(x, kLog2e * inv_tau, sm.table);
+    else soft.add(x, c);
   });
 
-  RowSum sum{soft, -CUDART_INF_F};
+  RowSum<Sum> sum{soft, -CUDART_INF_F};
   for (int k = tid; k < a.k; k += threads) {
     if (ls.token[k] < 0) continue;
     const float x = widen(g[ls.token[k]]);
     ls.q[k] = (double)x;
     sum.lmax = fmaxf(sum.lmax, x);
   }
-  sum = team.all(sum, [c](RowSum p, RowSum q) {
-    return RowSum{SoftSum::join(p.soft, q.soft, c), fmaxf(p.lmax, q.lmax)};
+  sum = team.all(sum, [c, inv_tau](RowSum<Sum> p, RowSum<Sum> q) {
+    RowSum<Sum> t;
+    if constexpr (kWide) t.soft = Sum::join(p.soft, q.soft, kLog2e * inv_tau);
+    else t.soft = Sum::join(p.soft, q.soft, c);
+    t.lmax = fmaxf(p.lmax, q.lmax);
+    return t;
   });
   const float bmax = sum.soft.m, xmax = fmaxf(bmax, sum.lmax);
   const double body = (double)sum.soft.s;
@@ -708,15 +784,16 @@ __device__ __forceinline__ void for_each_entry(const DistillArgs& a, int64_t r, 
 // copy and leaves as the row came.  Bound by instructions (66 % of issue, FP64 16
 // %): 524,288 x 21 f32, 8 entries: 49 us (20 us of memory traffic); with 64-bit
 // exponentials for the student too it was 120.
-template <typename T, int kPad>
-__global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_kernel(const T* logits,
+template <typename T, int kPad, bool kWide>
+__global__ void __launch_bounds__(kShortRows, kWide ? 3 : kPad <= 24 ? 8 : 5) distill_short_kernel(const T* logits,
                                                                    int64_t row_stride,
                                                                    int64_t n_rows, int vocab,
                                                                    DistillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
   __shared__ Exp2Table table;
   const int tid = threadIdx.x;
-  float* qs = reinterpret_cast<float*>(smem_raw + ShortRows<T>::bytes(vocab)) + tid;
+  using S = std::conditional_t<kWide, double, float>;
+  S* qs = reinterpret_cast<S*>(smem_raw + ShortRows<T>::bytes(vocab)) + tid;
   const int64_t r0 = (int64_t)blockIdx.x * kShortRows, r = r0 + tid;
   const int rows = (int)::min((int64_t)kShortRows, n_rows - r0);
   ShortRows<T> sr;
@@ -755,7 +832,7 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
           const float v = value(i);
           if (body >> i & 1u) bmax = fmaxf(bmax, v);
           else lmax = fmaxf(lmax, v);
-          qs[i * kShortPitch] = 0.0f;
+          qs[i * kShortPitch] = 0;
         }
       const float xmax = fmaxf(bmax, lmax);
       // masses exp(a / tau - norm), or relative to the largest until their sum
@@ -770,7 +847,7 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
         q_sum += q;
         // a mass that underflows counts nothing, also on a masked token
         if (q != 0.0) dot += q * (log_q - ((double)value(token) - (double)xmax) * inv_tau);
-        qs[token * kShortPitch] += (float)q;
+        qs[token * kShortPitch] += (S)q;
       });
       double q_scale = 1.0;
       if (!tail) {
@@ -780,20 +857,24 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
       }
       const float base = bmax == -CUDART_INF_F ? 0.0f : bmax;
       const float c = a.c;
-      float e[kPad], sum = 0.0f, rest = 0.0f;  // of the body and, relative to xmax, of the list
+      auto weight_of = [&](float x, float ref) -> S {
+        if constexpr (kWide) return wide_weight(x, ref, kLog2e * inv_tau, table);
+        else return exp2_fast((x - ref) * c);
+      };
+      S e[kPad], sum = 0, rest = 0;  // of the body and, relative to xmax, of the list
 #pragma unroll
       for (int i = 0; i < kPad; ++i) {
-        e[i] = 0.0f;
+        e[i] = 0;
         if (i < vocab) {
           const bool in_body = body >> i & 1u;
-          e[i] = exp2_fast((value(i) - (in_body ? base : xmax)) * c);
+          e[i] = weight_of(value(i), in_body ? base : xmax);
           if (in_body) sum += e[i];
           else rest += e[i];
         }
       }
-      const float lift = bmax == -CUDART_INF_F ? 0.0f
-                         : bmax == xmax        ? 1.0f
-                                               : exp2_fast((bmax - xmax) * c);
+      const S lift = bmax == -CUDART_INF_F ? (S)0
+                     : bmax == xmax        ? (S)1
+                                           : weight_of(bmax, xmax);
       const double total = fma((double)sum, (double)lift, (double)rest);
       double rest_q = 0.0;
       if (tail && bmax != -CUDART_INF_F) rest_q = fmax(0.0, 1.0 - q_sum);
@@ -809,13 +890,13 @@ __global__ void __launch_bounds__(kShortRows, kPad <= 24 ? 8 : 5) distill_short_
         const double each = mass / total;
         // gradient: e G off the list, e P - q Q on it (the body's e G where
         // listed tokens are part of the body: lift is 1 then)
-        const float G = (float)(wt * (each * (double)lift - share));
-        const float P = (float)(wt * each), Q = (float)(wt * q_scale);
+        const S G = (S)(wt * (each * (double)lift - share));
+        const S P = (S)(wt * each), Q = (S)(wt * q_scale);
 #pragma unroll
         for (int i = 0; i < kPad; ++i)
           if (i < vocab) {
-            const float y = listed >> i & 1u ? e[i] * P - qs[i * kShortPitch] * Q : e[i] * G;
-            sr.at(tid, i) = narrow<T>(weight == 0.0f ? 0.0f : y);
+            const S y = listed >> i & 1u ? e[i] * P - qs[i * kShortPitch] * Q : e[i] * G;
+            sr.at(tid, i) = narrow<T>(weight == 0.0f ? 0.0f : (float)y);
           }
       }
     }
@@ -838,33 +919,39 @@ bool use_team(const VocabRows& v, int k) {
   return v.vocab <= (kTeam == 4 ? 512 : 31 * 32) && k <= (kTeam == 4 ? 16 : 128) &&
          v.rows >= 2 * 148 * (kTeamThreads / kTeam);
 }
-template <typename T, int kTeam>
+template <typename T, int kTeam, bool kWide>
 cudaError_t launch_teams(cudaStream_t st, const VocabRows& v, const DistillArgs& a, int row_bytes) {
   constexpr int kTeams = kTeamThreads / kTeam;
-  distill_stream_kernel<T, kTeam>
+  distill_stream_kernel<T, kTeam, kWide>
       <<<(unsigned)((v.rows + kTeams - 1) / kTeams), kTeamThreads, row_bytes * kTeams, st>>>(
           static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, row_bytes, a);
   return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+template <typename T, bool kWide>
+cudaError_t launch_as(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   if (v.vocab <= kShortVocab) {
-    const int smem = ShortRows<T>::bytes(v.vocab) + (int)sizeof(float) * kShortPitch * v.vocab;
+    constexpr int kMass = kWide ? sizeof(double) : sizeof(float);
+    const int smem = ShortRows<T>::bytes(v.vocab) + kMass * kShortPitch * v.vocab;
     const unsigned blocks = (unsigned)((v.rows + kShortRows - 1) / kShortRows);
-    HKB_SHORT_WIDTH(v.vocab, (distill_short_kernel<T, kPad><<<blocks, kShortRows, smem, st>>>(
-                                 static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a)));
+    HKB_SHORT_WIDTH(v.vocab, {
+      if (kWide)  // 49 KB at 32 tokens of 32 bits
+        ensure_dynamic_smem((const void*)distill_short_kernel<T, kPad, kWide>,
+                            ShortRows<T>::bytes(kPad) + kMass * kShortPitch * kPad);
+      distill_short_kernel<T, kPad, kWide><<<blocks, kShortRows, smem, st>>>(
+          static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, a);
+    });
     return cudaGetLastError();
   }
   if (use_stream(v.rows, v.vocab, (int)sizeof(T))) {
     // bits of a row in its vectors' phase, in whole words
     const int words = (v.vocab + 16 / (int)sizeof(T) - 1 + 31) / 32;
     const int bytes = (a.k * 20 + words * 4 + 7) / 8 * 8;
-    if (use_team<4>(v, a.k)) return launch_teams<T, 4>(st, v, a, bytes);
-    if (use_team<8>(v, a.k)) return launch_teams<T, 8>(st, v, a, bytes);
-    ensure_dynamic_smem((const void*)distill_stream_kernel<T, 0>,
+    if (use_team<4>(v, a.k)) return launch_teams<T, 4, kWide>(st, v, a, bytes);
+    if (use_team<8>(v, a.k)) return launch_teams<T, 8, kWide>(st, v, a, bytes);
+    ensure_dynamic_smem((const void*)distill_stream_kernel<T, 0, kWide>,
                         HKB_LISTING_MAX * 20 + HKB_VOCAB_MAX / 8 + 8);
-    distill_stream_kernel<T, 0>
+    distill_stream_kernel<T, 0, kWide>
         <<<(unsigned)v.rows, stream_threads(v.vocab, (int)sizeof(T)), bytes, st>>>(
             static_cast<const T*>(v.logits), v.row_stride, v.rows, v.vocab, 0, a);
     return cudaGetLastError();
@@ -881,10 +968,17 @@ cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  auto kernel = s.cluster > 1 ? distill_rows_kernel<T, true> : distill_rows_kernel<T, false>;
+  auto kernel =
+      s.cluster > 1 ? distill_rows_kernel<T, true, kWide> : distill_rows_kernel<T, false, kWide>;
   ensure_dynamic_smem((const void*)kernel, 131072 + 16 + HKB_LISTING_MAX * 20);
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<const T*>(v.logits), v.row_stride, v.vocab,
                             s.chunk, (int)s.smem, a);
+}
+
+template <typename T>
+cudaError_t launch(cudaStream_t st, const VocabRows& v, const DistillArgs& a) {
+  return a.temperature > kWideTemperature ? launch_as<T, true>(st, v, a)
+                                          : launch_as<T, false>(st, v, a);
 }
 
 template <typename T>

@@ -289,7 +289,10 @@ hkb_status hkb_write_logprobs_npz(const char* path, int32_t num_seqs, int32_t re
 #define HKB_LISTING_MAX 1024
 /* of log-norms and of distillation */
 #define HKB_TEMPERATURE_MIN 1e-30f
+/* of log-norms */
 #define HKB_TEMPERATURE_MAX 1e30f
+/* of distillation, whose loss grows out of what 64 bits hold of the divergence */
+#define HKB_DISTILL_TEMPERATURE_MAX 1e4f
 /* numbers a row that a backward pass takes from the forward pass */
 #define HKB_DISTILL_STATS 5
 
@@ -362,7 +365,7 @@ typedef struct {
   const int32_t* tokens; /* [N,k]; negative = no entry, as is a value of -inf */
   const float* log_norm; /* [N] teacher's log sum exp(a / temperature) over its
                             whole row, or NULL */
-  float temperature;     /* 1e-30 to 1e30 */
+  float temperature;     /* 1e-30 to 1e4 */
 } hkb_distill_teacher;
 
 typedef struct {
@@ -394,6 +397,11 @@ typedef struct {
  * gradient NaN; so do an entry's value that is NaN or +inf, a log_norm that is not
  * finite, a NaN or +inf logit, and a row with no logit above -inf.
  * A listed token whose student logit is -inf makes the loss +inf.
+ *
+ * The student's weights and their sum are 32-bit up to temperature 16 (the loss
+ * is off by up to 2e-7 temperature^2), 64-bit above it (1e-14 temperature^2).  log_norm
+ * is a 32-bit number: 2^-24 |log_norm| is the relative error of every listed mass
+ * that it brings along, and the gradient's the temperature times that.
  *
  * grad may be the logits' own buffer (the same address, row stride and type);
  * any other overlap is not allowed, and rows must not overlap then.  It lies
