@@ -369,6 +369,12 @@ constexpr double kFixedOne = 4503599627370496.0;
 __device__ __forceinline__ unsigned long long fixed_weight(double w) {
   return __double2ull_rn(w * kFixedOne);
 }
+// For the draw: a weight above zero counts at least 2^-52, so that u = 0 finds the
+// first kept token of any weight; 2^-41 of the mass in all.
+__device__ __forceinline__ unsigned long long drawn_weight(double w) {
+  const unsigned long long f = fixed_weight(w);
+  return f == 0 && w > 0.0 ? 1ull : f;
+}
 
 // Three counts of up to kListCap in one word.
 __device__ __forceinline__ unsigned long long three_counts(bool a, bool b, bool c) {
@@ -563,7 +569,7 @@ __device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const We
   while (most >> shift >= kBuckets) ++shift;
 #pragma unroll
   for (int j = 0; j < kOwnItems; ++j)
-    if (own[j] != 0) atomicAdd(&bucket[item_index(own[j]) >> shift], fixed_weight(w[j]));
+    if (own[j] != 0) atomicAdd(&bucket[item_index(own[j]) >> shift], drawn_weight(w[j]));
   if (tid == 0) sm.sub_count = 0;
   __syncthreads();
   // a thread has one bucket, or two
@@ -592,7 +598,7 @@ __device__ __forceinline__ void finish_long_list(SampleSmem& sm, int n, const We
     if (own[j] != 0 && item_index(own[j]) >> shift == at) {
       const unsigned i = atomicAdd(&sm.sub_count, 1u);
       item[2 * i] = (unsigned)item_index(own[j]);
-      item[2 * i + 1] = fixed_weight(w[j]);
+      item[2 * i + 1] = drawn_weight(w[j]);
     }
   __syncthreads();
   const int m = (int)sm.sub_count;  // at most 2^shift <= 512

@@ -39,3 +39,38 @@ def test_temperatures_below_the_smallest_normal_number(vocab, size, rows, dtype)
                 u = torch.full((rows,), v, device="cuda")
                 got = vocab.sample_tokens(x, u, temperature=t, **f)
                 check_sample([a[at] for a in got], x[at], u[at], temperature=t, **f)
+
+
+# a thread, a warp, a CTA and a cluster a row; lists of up to 192 tokens and longer ones
+@pytest.mark.parametrize("size", [21, 200, 900, 5000, 60000])
+@pytest.mark.parametrize("rows", [6, 700])
+def test_the_smallest_uniform_draws_the_first_kept_token(vocab, size, rows):
+    # light tokens lie before the heavy ones, by up to 2^-100 of the largest weight
+    z = torch.arange(size, device="cuda", dtype=F32) * (69.0 / size) - 69.0
+    x = z.expand(rows, size).clone()
+    x[1] = x[1].flip(0)
+    x[2] = x[2].roll(size // 2)
+    x[3, 0] = -float("inf")
+    x[4] = (x[4] / 8).round() * 8
+    u = torch.zeros(rows, device="cuda")
+    for f in (dict(), dict(top_k=size // 2), dict(top_k=150), dict(top_k=250), dict(top_k=800),
+              dict(top_k=1000, top_p=0.999999), dict(top_k=2000), dict(min_p=1e-25),
+              dict(top_k=900, min_p=1e-20)):
+        got = vocab.sample_tokens(x, u, **f)
+        for r in (0, 1, 2, 3, 4, rows - 1):
+            y = x[r].double()
+            order = y.argsort(descending=True, stable=True)
+            n = int((y > -float("inf")).sum())
+            if f.get("top_k"):
+                n = min(n, f["top_k"])
+            w = (y - y.max()).exp()
+            run = w[order[:n]].cumsum(0)
+            if "top_p" in f:
+                p = float(torch.tensor(f["top_p"], dtype=F32))
+                n = min(n, 1 + int((run < p * run[-1]).sum()))
+            if "min_p" in f:
+                m = float(torch.tensor(f["min_p"], dtype=F32))
+                n = min(n, int((w >= m).sum()))
+            # the definition: the first token whose running mass exceeds 0
+            assert int(got.tokens[r]) == int(order[:n].min()), (r, f)
+            assert int(got.kept[r]) == n, (r, f)
