@@ -349,6 +349,8 @@ PyObject* loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor& tokens = tensor_arg(args[2], "teacher_tokens");
     const std::optional<Tensor> norm = optional_arg(args[3], "teacher_log_norm");
     const double temperature = number_arg(args[4], "temperature");
+    // without this a tangent would be dropped
+    if (x._fw_grad(0).defined()) refuse("distill_loss has no forward-mode derivative");
     if (!(x.requires_grad() && at::GradMode::is_enabled()))
       return THPVariable_Wrap(loss_only(x, values, tokens, norm, temperature, nullptr));
     if (x.is_cuda() &&

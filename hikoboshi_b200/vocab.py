@@ -92,7 +92,8 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     sums are 32-bit and the loss is off by up to 2e-7 temperature^2, above that
     they are 64-bit.
 
-    The loss is differentiable once.  The backward pass reads ``logits`` and the
+    The loss is differentiable once, backwards; logits with a forward-mode tangent
+    are refused.  The backward pass reads ``logits`` and the
     teacher's tensors again, so they must not be overwritten before it.
     Autograd through this call cannot be captured into a CUDA graph (an eager
     graph of the same leaves would break the capture): there it raises
