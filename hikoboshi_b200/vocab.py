@@ -17,6 +17,14 @@ dimension of stride 1 and leading dimensions that flatten to rows of one
 stride; nothing is copied or converted on the way.  The work goes to torch's
 current stream of that device, without synchronisation, workspaces or state.
 Unfit arguments raise :class:`HkbError` with ``HKB_INVALID_ARGUMENT``.
+
+Of all results only :func:`distill_loss` is differentiable, and with respect to
+``logits`` alone: a teacher's tensors are constants, and what the other functions
+return is detached, also from logits that require grad.  The functions are not
+registered torch operators: ``torch.func`` transforms and
+``torch.compile(fullgraph=True)`` raise, ``torch.compile`` without it calls them
+between its graphs, and tracers of dispatched operators (``torch.export``,
+``make_fx``) must not be used on them.
 """
 from __future__ import annotations
 
@@ -61,7 +69,7 @@ def sample_tokens(logits, uniforms, *, temperature=1.0, top_k=0, top_p=1.0,
     Each setting is a number, or a tensor [..] with a setting per row (f32,
     ``top_k`` i32).  Rows whose tensor settings or uniforms are out of range
     give token -1, log_prob NaN and kept 0; rows with no logit above -inf give
-    -1, -inf and 0.  A NaN logit counts as -inf.
+    -1, -inf and 0.  A NaN logit counts as -inf.  Not differentiable.
     """
     return SampledTokens(*_vocab.sample(logits, uniforms, temperature, top_k, top_p, min_p))
 
@@ -70,7 +78,7 @@ def top_logits(logits, k: int, *, temperature: float = 1.0) -> TopLogits:
     """The ``k`` largest logits of each row of ``logits`` [.., V] with their
     tokens, in the order (logit down, index up), and log sum exp(x / temperature).
     Places past a row's logits above -inf hold (-inf, -1); a NaN logit counts
-    as -inf.  ``temperature`` is 1e-30 to 1e30."""
+    as -inf.  ``temperature`` is 1e-30 to 1e30.  Not differentiable."""
     return TopLogits(*_vocab.top(logits, k, temperature))
 
 

@@ -19,3 +19,30 @@ def test_forward_mode_is_refused_instead_of_dropping_the_tangent():
             assert e.value.code == 1 and "forward-mode" in e.value.detail
         # without a tangent the call is what it was
         assert vocab.distill_loss(X, V, T).shape == (0,)
+
+
+def test_results_other_than_the_loss_are_detached():
+    x, u = X.clone().requires_grad_(), torch.zeros(0)
+    top = vocab.top_logits(x, 4)
+    drawn = vocab.sample_tokens(x, u)
+    both = vocab.distill_loss_and_grad(x, V, T)
+    assert not any(a.requires_grad for a in (*top, *drawn, *both))
+    # a teacher's tensors are constants
+    v = V.clone().requires_grad_()
+    norm = torch.zeros(0, requires_grad=True)
+    assert not vocab.distill_loss(X, v, T, teacher_log_norm=norm).requires_grad
+    loss = vocab.distill_loss(x, v, T, teacher_log_norm=norm)
+    gx, gv, gn = torch.autograd.grad(loss.sum(), (x, v, norm), allow_unused=True)
+    assert gx is not None and gv is None and gn is None
+
+
+@pytest.mark.parametrize("transform", [
+    lambda f: torch.func.vmap(f)(torch.zeros(2, 3, 21), torch.zeros(2, 3, 4),
+                                 torch.zeros(2, 3, 4, dtype=torch.int32)),
+    lambda f: torch.func.grad(lambda x: f(x, V, T).sum())(X),
+    lambda f: torch.func.jvp(lambda x: f(x, V, T), (X,), (X,)),
+    lambda f: torch.compile(lambda x: f(x, V, T), fullgraph=True, backend="eager")(X),
+], ids=["vmap", "grad", "jvp", "compile"])
+def test_transforms_raise(transform):
+    with pytest.raises(RuntimeError):
+        transform(vocab.distill_loss)
