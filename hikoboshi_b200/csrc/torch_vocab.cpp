@@ -152,6 +152,11 @@ void run(const Tensor& x, F call) {
   refuse(s.detail, s.code);
 }
 
+bool capturing(const Tensor& x) {
+  return x.is_cuda() &&
+         c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None;
+}
+
 // The loss; `stats`, if given, receives what a backward pass needs.
 Tensor loss_only(const Tensor& x, const Tensor& values, const Tensor& tokens,
                  const std::optional<Tensor>& log_norm, double temperature, Tensor* stats) {
@@ -191,6 +196,10 @@ struct DistillLoss : torch::autograd::Function<DistillLoss> {
     if (!w.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     TORCH_CHECK(!(at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad())),
                 "distill_loss is differentiable once: its gradient has none");
+    // the forward pass was not captured, so an eager graph of the same leaves
+    // lives: to accumulate their gradients would break the capture
+    TORCH_CHECK(!capturing(x), "distill_loss backward: autograd through distill_loss cannot be "
+                               "captured; capture distill_loss_and_grad");
     int64_t n, step;
     if (w.is_neg() || !flatten(w.sizes(), w.strides(), &n, &step))
       w = w.resolve_neg().contiguous();
@@ -353,8 +362,7 @@ PyObject* loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (x._fw_grad(0).defined()) refuse("distill_loss has no forward-mode derivative");
     if (!(x.requires_grad() && at::GradMode::is_enabled()))
       return THPVariable_Wrap(loss_only(x, values, tokens, norm, temperature, nullptr));
-    if (x.is_cuda() &&
-        c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    if (capturing(x))
       refuse("autograd through distill_loss cannot be captured; capture distill_loss_and_grad",
              HKB_FAILED_PRECONDITION);
     return THPVariable_Wrap(DistillLoss::apply(x, values, tokens, norm, temperature));

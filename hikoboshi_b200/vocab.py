@@ -105,7 +105,8 @@ def distill_loss(logits, teacher_values, teacher_tokens, *, teacher_log_norm=Non
     teacher's tensors again, so they must not be overwritten before it.
     Autograd through this call cannot be captured into a CUDA graph (an eager
     graph of the same leaves would break the capture): there it raises
-    HKB_FAILED_PRECONDITION; capture :func:`distill_loss_and_grad`.
+    HKB_FAILED_PRECONDITION, a backward pass alone RuntimeError; capture
+    :func:`distill_loss_and_grad`.
     """
     return _vocab.loss(logits, teacher_values, teacher_tokens, teacher_log_norm, temperature)
 

@@ -46,3 +46,27 @@ def test_results_other_than_the_loss_are_detached():
 def test_transforms_raise(transform):
     with pytest.raises(RuntimeError):
         transform(vocab.distill_loss)
+
+
+@pytest.mark.gpu
+def test_a_backward_pass_alone_is_refused_in_a_capture():
+    x = torch.randn(4, 50, device="cuda")
+    v, t = x.topk(3)
+    t, w = t.int(), torch.ones(4, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        z = x.clone().requires_grad_()
+        loss = vocab.distill_loss(z, v, t)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            torch.autograd.grad(loss, z, w, retain_graph=True)
+        _, inside = vocab.distill_loss_and_grad(x, v, t, row_weights=w)
+    graph.replay()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):  # the eager graph is as it was
+        (after,) = torch.autograd.grad(loss, z, w)
+    torch.cuda.synchronize()
+    assert torch.equal(inside, after)
