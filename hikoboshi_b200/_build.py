@@ -74,12 +74,19 @@ def build_library(verbose: bool = False) -> Path:
 VOCAB_MODULE = PKG / "_vocab.so"
 
 
-def build_vocab_module(verbose: bool = False) -> Path:
+def build_vocab_module(verbose: bool = False) -> Path | None:
     """``hikoboshi_b200._vocab`` (csrc/torch_vocab.cpp): the torch binding of the
-    operators on vocabulary rows, linked to the in-tree library and to torch."""
+    operators on vocabulary rows, linked to the in-tree library and to torch.
+    Without torch there is none: the library and its numpy front-end need no
+    torch."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        print("build: torch cannot be imported; hikoboshi_b200.vocab is left out")
+        return None
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     src = CSRC / "torch_vocab.cpp"
     deps = [src, ROOT / "include" / "hkb_mpnn.h"]
     # the library is linked by name: a rebuilt one needs no new module
@@ -88,7 +95,7 @@ def build_vocab_module(verbose: bool = False) -> Path:
         return VOCAB_MODULE
     t = Path(torch.__file__).resolve().parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            f"-I{ROOT / 'include'}", f"-isystem{t / 'include'}",
            f"-isystem{t / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
            f"-isystem{sysconfig.get_paths()['include']}", f"-isystem{CUDA_HOME / 'include'}",
