@@ -72,13 +72,15 @@ def build_library(verbose: bool = False) -> Path:
 
 
 VOCAB_MODULE = PKG / "_vocab.so"
+VOCAB_STAMP = OBJ / "_vocab.stamp"
 
 
 def build_vocab_module(verbose: bool = False) -> Path | None:
     """``hikoboshi_b200._vocab`` (csrc/torch_vocab.cpp): the torch binding of the
     operators on vocabulary rows, linked to the in-tree library and to torch.
-    Without torch there is none: the library and its numpy front-end need no
-    torch."""
+    It fits the torch and the Python that it was compiled for, which the stamp
+    beside the objects names; for others it is compiled anew.  Without torch
+    there is none: the library and its numpy front-end need no torch."""
     import sysconfig
 
     try:
@@ -87,11 +89,12 @@ def build_vocab_module(verbose: bool = False) -> Path | None:
         print("build: torch cannot be imported; hikoboshi_b200.vocab is left out")
         return None
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    built_for = f"torch {torch.__version__} abi {abi} python {sysconfig.get_config_var('SOABI')}"
     src = CSRC / "torch_vocab.cpp"
     deps = [src, ROOT / "include" / "hkb_mpnn.h"]
     # the library is linked by name: a rebuilt one needs no new module
-    if VOCAB_MODULE.exists() and VOCAB_MODULE.stat().st_mtime >= max(d.stat().st_mtime
-                                                                     for d in deps):
+    if (VOCAB_MODULE.exists() and VOCAB_STAMP.exists() and VOCAB_STAMP.read_text() == built_for
+            and VOCAB_MODULE.stat().st_mtime >= max(d.stat().st_mtime for d in deps)):
         return VOCAB_MODULE
     t = Path(torch.__file__).resolve().parent
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
@@ -105,6 +108,8 @@ def build_vocab_module(verbose: bool = False) -> Path | None:
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
+    VOCAB_STAMP.parent.mkdir(exist_ok=True)
+    VOCAB_STAMP.write_text(built_for)
     return VOCAB_MODULE
 
 

@@ -1,4 +1,4 @@
-"""The build on a machine without torch."""
+"""The build on a machine without torch, and after torch was replaced."""
 import subprocess
 import sys
 from pathlib import Path
@@ -15,3 +15,23 @@ def test_the_library_builds_without_torch():
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True)
     assert done.returncode == 0, done.stderr
     assert "torch cannot be imported" in done.stdout
+
+
+def test_the_binding_is_compiled_anew_for_another_torch(tmp_path, monkeypatch):
+    import torch
+    module, stamp, runs = tmp_path / "_vocab.so", tmp_path / "_vocab.stamp", []
+
+    def compiler(cmd, check):
+        runs.append(cmd)
+        module.write_bytes(b"")
+
+    monkeypatch.setattr(_build, "VOCAB_MODULE", module)
+    monkeypatch.setattr(_build, "VOCAB_STAMP", stamp, raising=False)
+    monkeypatch.setattr(_build.subprocess, "run", compiler)
+    assert _build.build_vocab_module() == module and len(runs) == 1
+    assert _build.build_vocab_module() == module and len(runs) == 1  # nothing has changed
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    assert _build.build_vocab_module() == module and len(runs) == 2
+    assert _build.build_vocab_module() == module and len(runs) == 2
+    stamp.unlink()  # of unknown origin
+    assert _build.build_vocab_module() == module and len(runs) == 3
