@@ -164,5 +164,8 @@ def stage_weights(ref_root: str | os.PathLike | None = None) -> Path:
 
 
 if __name__ == "__main__":
-    stage_weights()
+    try:
+        stage_weights()
+    except FileNotFoundError as e:
+        print(f"build: {e}; an engine needs it, the library does not")
     print(build_library(verbose=True))

@@ -35,3 +35,11 @@ def test_the_binding_is_compiled_anew_for_another_torch(tmp_path, monkeypatch):
     assert _build.build_vocab_module() == module and len(runs) == 2
     stamp.unlink()  # of unknown origin
     assert _build.build_vocab_module() == module and len(runs) == 3
+
+
+def test_the_build_script_runs_without_a_weight_image(tmp_path):
+    import os
+    env = dict(os.environ, HKB_REFERENCE_ROOT=str(tmp_path))
+    done = subprocess.run([sys.executable, str(ROOT / "hikoboshi_b200" / "_build.py")], env=env,
+                          capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr
