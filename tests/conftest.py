@@ -18,6 +18,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: long-running CPU oracle comparison")
 
 
+def pytest_collection_modifyitems(items):
+    # without the weight image the tests that need it fail; the others go first, so
+    # that a run that stops at the first failure has them behind it
+    if not WEIGHTS.exists():
+        items.sort(key=lambda item: "weights_path" in getattr(item, "fixturenames", ()))
+
+
 @pytest.fixture(scope="session")
 def weights_path():
     if not WEIGHTS.exists():
