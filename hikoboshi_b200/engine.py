@@ -211,9 +211,13 @@ class DesignEngine:
         from . import vocab
         rows, shapes = self._scored_rows(coords, sources, tokens, orders, seeds)
         us = [np.asarray(u, np.float64) for u in uniforms]
-        if len(us) != len(shapes) or any(u.size != s * n for u, (s, n) in zip(us, shapes)):
+        # a flat array is taken as [S, L], as the tokens are; a transposed one is not
+        if len(us) != len(shapes) or any(u.size != s * n or (u.ndim > 1 and u.shape != (s, n))
+                                         for u, (s, n) in zip(us, shapes)):
             raise _lib.HkbError(_lib.HKB_INVALID_ARGUMENT,
                                 "uniforms must have one number per position")
+        if not all(((u >= 0) & (u <= 1)).all() for u in us):
+            raise _lib.HkbError(_lib.HKB_INVALID_ARGUMENT, "uniforms must be 0 to 1")
         u = torch.from_numpy(np.concatenate([u.reshape(-1) for u in us])).to(rows.device)
         with torch.cuda.device(rows.device):
             got = vocab.sample_tokens(rows, u, temperature=temperature, top_k=top_k, top_p=top_p,
