@@ -779,13 +779,13 @@ __device__ __forceinline__ void for_each_entry(const DistillArgs& a, int64_t r, 
 }
 
 // Short rows, one thread each.  The masses of a row's tokens are added up in
-// shared memory, so a token listed twice needs no special case; the weights
-// stay in registers between the sum and the gradient, which replaces the row's
-// copy and leaves as the row came.  Up to kWideTemperature a token's mass and the
-// listed gradient are 32-bit (a few roundings of 2^-24 of temperature * mass; the
-// loss has the masses in 64 bits): half the shared memory and registers.  Bound by instructions (66 % of issue, FP64 16
-// %): 524,288 x 21 f32, 8 entries: 49 us (20 us of memory traffic); with 64-bit
-// exponentials for the student too it was 120.
+// shared memory, so a token listed twice needs no special case; the weights stay
+// in registers between the sum and the gradient, which replaces the row's copy and
+// leaves as the row came.  Up to kWideTemperature a token's mass and the listed
+// gradient are 32-bit (a few roundings of 2^-24 of temperature * mass; the loss
+// has the masses in 64 bits): half the shared memory and registers.  Bound by
+// instructions (73 % of issue, FP64 16 %): 524,288 x 21 f32, 8 entries: 49 us (20
+// us of memory traffic); with 64-bit exponentials for the student too it was 120.
 template <typename T, int kPad, bool kWide>
 __global__ void __launch_bounds__(kShortRows, kWide ? 3 : kPad <= 24 ? 8 : 5) distill_short_kernel(const T* logits,
                                                                    int64_t row_stride,

@@ -22,8 +22,9 @@ namespace hkb {
 RowShape row_shape(int64_t rows, int vocab, int elem_bytes) {
   const int per16 = 16 / elem_bytes;
   RowShape s{};
-  // slices of at most 64 KB, and more CTAs a row while there are few rows and
-  // a slice keeps 4 KB
+  // slices of at most 64 KB (128 KB where 8 CTAs share a row of more than 131,072
+  // 32-bit logits), and more CTAs a row while there are few rows and a slice keeps
+  // 4 KB
   s.cluster = 1;
   while (s.cluster < vocab::kMaxCluster) {
     const int64_t slice = (int64_t)vocab * elem_bytes / s.cluster;
@@ -695,9 +696,12 @@ __device__ __forceinline__ void finish_list(SampleSmem& sm, int n, const Weights
 // bins, and the token found by the running masses of CTAs, warps and steps.
 //
 // Bound by latency with few rows (1 x 32768 f32, top-k: 12 us; cluster barriers
-// of about 1000 cycles each) and by the 64-bit weights with many (192 x 50001
-// f16, unfiltered: 38 us, FP64 pipe 27 %).  Slices of 64 KB at most: two CTAs a
-// SM; of 32 KB 64 rows of 131,072 bf16 took 145 us (top-p) instead of 102.
+// of about 1000 cycles each; 1 x 131072 bf16, top-p: 82) and by instructions and
+// latency together with more (192 x 50001 f16, unfiltered: 38 us, 61 % of issue,
+// FP64 pipe 30 %, 40 % of the warps active; 1024 x 32768 f32, top-p: 393).  Top-k
+// above 1024 bisects keys instead: 1024 x 32768 f32, top-k 2000: 591.  Slices of
+// 64 KB let two CTAs share a SM, those of 128 KB do not; of 32 KB 64 rows of
+// 131,072 bf16 took 145 us (top-p) instead of 102.
 template <typename T, bool kClustered>
 __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
     const T* __restrict__ logits, int64_t row_stride, int vocab, int chunk, SampleArgs a) {
@@ -963,8 +967,9 @@ __global__ void __launch_bounds__(kMaxThreads, 2) sample_rows_kernel(
 // the head is found with 32-bit weights, by bisection of the logits' keys, and
 // again with 64-bit ones where a comparison with the border is too close (or
 // where equal logits share the border: their number needs the exact masses).
-// Bound by instructions: 415,936 x 143 f32, unfiltered, 1.1 ms (9.5 ms with a CTA
-// a row, whose barriers and set-up such rows do not repay).
+// Bound by instructions: 415,936 x 143 f32, settings per row (nine in ten with a
+// top-p below 1), 1.16 ms (9.5 ms with a CTA a row, whose barriers and set-up such
+// rows do not repay); top-p 0.9 1.09, unfiltered 0.40.
 template <typename T, int kPer>
 __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
     const T* __restrict__ logits, int64_t row_stride, int64_t n_rows, int vocab, SampleArgs a) {
@@ -1162,7 +1167,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) sample_warp_kernel(
 // tokens' mass and the draw are in 64 bits, so their number sets the time on
 // the 64-bit pipe, not V.
 //
-// 524,288 x 21 f32, top-p and min-p: 47 us (8 us of memory traffic), 57 % of the
+// 524,288 x 21 f32, top-p and min-p: 47 us (8 us of memory traffic), 65 % of the
 // issue rate; taking the largest remaining token until the filters stop took 75.
 template <typename T, int kPad>
 __global__ void __launch_bounds__(kShortRows) sample_short_kernel(const T* __restrict__ logits,

@@ -68,7 +68,7 @@ struct TopSmem {
 
 // Few rows: a cluster holds a row, each CTA finds its largest logits and sum in
 // one pass, one joint reduction gives the bound, rank 0 orders what reaches it.
-// Bound by latency: 5 x 100003 f32, top 256: 16 us, 5 % of the issue rate.
+// Bound by latency: 5 x 100003 f32, top 256: 15 us, 40 CTAs of 148 SMs.
 template <typename T, bool kClustered>
 __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __restrict__ logits,
                                                                int64_t row_stride, int vocab,
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(kMaxThreads, 2) top_rows_kernel(const T* __res
 }
 
 // Many rows: a CTA streams a row for its maxima and sum, then again, from L2, to
-// collect what reaches the bound.  Bound by instructions and exponentials (65 %
+// collect what reaches the bound.  Bound by instructions and exponentials (69 %
 // of issue, XU 50 %): 2048 x 131072 bf16, top 64: 153 us, 3.5 TB/s; with the row in
 // a cluster's shared memory it was 652.  256 threads instead of 512: 186 against
 // 166; the next loads in flight during the work: 161 against 166.
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(32 * kWarpRows) top_warp_kernel(const T* __res
 }
 
 // Short rows, one thread each: sorts the row in registers.  The listing goes
-// through shared memory, so that it leaves coalesced.  Bound by instructions (70 %
+// through shared memory, so that it leaves coalesced.  Bound by instructions (78 %
 // of issue): 786,432 x 21 f32, top 8: 47 us (18.5 us of memory traffic); taking the
 // largest remaining token 8 times took 76, and 40 registers a thread for twelve
 // CTAs a SM 51 instead of 57.

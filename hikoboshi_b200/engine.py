@@ -205,7 +205,12 @@ class DesignEngine:
         distribution, cut by ``top_k``, ``top_p`` and ``min_p``
         (:func:`hikoboshi_b200.vocab.sample_tokens`).  ``tokens[b]`` and
         ``uniforms[b]`` (in [0, 1]) are [S_b, L_b].  Returns per protein
-        (tokens [S, L] int32, log_probs [S, L], kept [S, L] int32)."""
+        (tokens [S, L] int32, log_probs [S, L], kept [S, L] int32).
+
+        A position's distribution is given the *old* sequence, so this is no
+        design drawn with filters; and residues without a full backbone, which
+        :meth:`design` leaves as X, are drawn from their scored row like all
+        others."""
         import torch
 
         from . import vocab
