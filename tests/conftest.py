@@ -21,8 +21,10 @@ def pytest_configure(config):
 def pytest_collection_modifyitems(items):
     # without the weight image the tests that need it fail; the others go first, so
     # that a run that stops at the first failure has them behind it
+    # (the command line reads the default image by itself)
     if not WEIGHTS.exists():
-        items.sort(key=lambda item: "weights_path" in getattr(item, "fixturenames", ()))
+        items.sort(key=lambda item: "weights_path" in getattr(item, "fixturenames", ())
+                   or item.name.startswith("test_cli_design"))
 
 
 @pytest.fixture(scope="session")
