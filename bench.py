@@ -24,6 +24,9 @@ decode of all 2,048 sequences (524,288 designed residues per GPU).
   reference sources compiled here) on the host cores, bounded sample.
 
 ``--impl reference`` times that reference CPU path alone on the same metric.
+Where the reference's sources or the published weight image are not at hand, that
+arm prints why, the sample is left out, and the engine runs on weights of random
+values, as ``data`` then says.
 Multi-GPU: one process per GPU (torchrun), proteins sharded by rank, no
 collective on the data path (weak scaling); barrier + max-over-ranks timing.
 """
@@ -53,6 +56,32 @@ FLOP_DECODE_PER_RES = 29_103_360
 FLOP_ENCODE_PER_RES = 54_657_024
 WEIGHTS = ROOT / "hikoboshi_b200" / "weights" / "Hikoboshi-ProteinMPNN-v48-020.safetensors"
 METRIC = "ProteinMPNN v48 designed residues/sec at L=256 x32 seqs; us per decode step"
+
+
+def published_weights() -> bool:
+    return WEIGHTS.exists()
+
+
+def engine_weights():
+    """The published weight image, or one of random values where it is not at hand:
+    the work does not depend on the values."""
+    if published_weights():
+        return WEIGHTS
+    sys.path.insert(0, str(ROOT / "tests"))
+    from random_weights import random_weights
+    return random_weights(0)
+
+
+def data_note(text: str) -> str:
+    return text if published_weights() else text + "; random weights of that architecture"
+
+
+def reference_missing() -> str | None:
+    """Why the reference's own CPU path cannot run here, or None."""
+    from oracle.oracle import REF_SO
+    if not REF_SO.exists():
+        return "the reference's sources are not at hand, so its CPU path is not compiled"
+    return None if published_weights() else "the reference's weight image is not at hand"
 
 
 def dist_env():
@@ -270,7 +299,7 @@ def run_ours(args):
     from hikoboshi_b200 import DesignEngine
     from hikoboshi_b200 import _lib as hl
 
-    eng = DesignEngine(WEIGHTS, device=local, precision=args.precision)
+    eng = DesignEngine(engine_weights(), device=local, precision=args.precision)
     coords_h, src_h = make_inputs(rank)
     R = coords_h.shape[0]
     Q = N_PROT * N_SEQ * L_RES
@@ -381,7 +410,7 @@ def run_ours(args):
             "steps": args.steps, "warmup": max(3, args.warmup), "ms_per_step": step_s * 1000,
             "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
             "dtype": {"f16": "f16", "bf16": "bf16", "fp32": "f32"}[args.precision],
-            "data": "synthetic (seeded ideal-geometry backbones, BASELINE generator)",
+            "data": data_note("synthetic (seeded ideal-geometry backbones, BASELINE generator)"),
             "config": {"workload": "config2: 64 backbones x L=256 x 32 seqs per GPU, T=0.1, "
                                    "random decoding order per sequence",
                        "proteins_per_gpu": N_PROT, "residue_count": L_RES,
@@ -489,7 +518,7 @@ def run_config4(args):
         import torch.distributed as dist
         dist.init_process_group("nccl", timeout=datetime.timedelta(seconds=120), device_id=dev)
     from hikoboshi_b200 import DesignEngine, synthetic_backbone
-    eng = DesignEngine(WEIGHTS, device=local, precision=args.precision)
+    eng = DesignEngine(engine_weights(), device=local, precision=args.precision)
     cs, ss, toks = config4_inputs(rank, synthetic_backbone)
     Q = C4_PROT * C4_SEQ * C4_L
     flush = torch.empty(128 * 1024 * 1024, dtype=torch.float32, device=dev)
@@ -570,7 +599,8 @@ def run_config4(args):
             "n_gpus": world, "steps": args.steps, "warmup": max(3, args.warmup),
             "ms_per_step": d_ms, "higher_is_better": True, "scaling": "weak",
             "vs_baseline": None, "dtype": {"f16": "f16", "bf16": "bf16", "fp32": "f32"}[args.precision],
-            "data": "synthetic (seeded ideal-geometry backbones, uniform random tokens)",
+            "data": data_note("synthetic (seeded ideal-geometry backbones, uniform random "
+                              "tokens)"),
             "config": {"workload": "config4: teacher-forced scoring of 128 backbones x L=384 x 16 "
                                    "sequences per GPU, random decoding order",
                        "precision": args.precision,
@@ -682,7 +712,7 @@ def run_config5(args):
     from hikoboshi_b200 import DesignEngine, synthetic_backbone
     from hikoboshi_b200 import _lib as hl
     from hikoboshi_b200.shard import design_sharded, partition_proteins
-    eng = DesignEngine(WEIGHTS, device=local, precision=args.precision)
+    eng = DesignEngine(engine_weights(), device=local, precision=args.precision)
     Ls = config5_lengths()
     mine = partition_proteins(Ls, C5_SEQ, world)[rank]
     total_res = sum(Ls) * C5_SEQ
@@ -786,7 +816,8 @@ def run_config5(args):
             "n_gpus": world, "steps": steps, "warmup": max(3, args.warmup),
             "ms_per_step": step_s * 1000, "higher_is_better": True, "scaling": "strong",
             "vs_baseline": None, "dtype": {"f16": "f16", "bf16": "bf16", "fp32": "f32"}[args.precision],
-            "data": "synthetic (seeded ideal-geometry backbones, lengths from default_rng(42))",
+            "data": data_note("synthetic (seeded ideal-geometry backbones, lengths from "
+                              "default_rng(42))"),
             "config": {"workload": "config5: 4096 backbones, L uniform in [64, 512], 16 seqs each, "
                                    "T=0.1, length-bucketed LPT partition by protein over the ranks",
                        "designed_residues": total_res, "precision": args.precision,
@@ -872,7 +903,7 @@ def run_small(args):
         return 0
     torch.cuda.set_device(local)
     from hikoboshi_b200 import DesignEngine, synthetic_backbone
-    eng = DesignEngine(WEIGHTS, device=local, precision=args.precision)
+    eng = DesignEngine(engine_weights(), device=local, precision=args.precision)
     c, s_ = synthetic_backbone(cfg["seed"], cfg["L"])
     res_step = cfg["S"] * cfg["L"]
     for _ in range(max(3, args.warmup)):
@@ -889,7 +920,8 @@ def run_small(args):
         "steps": args.steps, "warmup": max(3, args.warmup), "ms_per_step": float(np.mean(dev)) * 1000,
         "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
         "dtype": {"f16": "f16", "bf16": "bf16", "fp32": "f32"}[args.precision],
-        "data": "synthetic", "config": {"workload": args.workload, "precision": args.precision},
+        "data": data_note("synthetic"),
+        "config": {"workload": args.workload, "precision": args.precision},
         "e2e": {"value": res_step / float(np.mean(wall)), "unit": "residues/s",
                 "h2d_bytes_per_step": cfg["L"] * 80,
                 "d2h_bytes_per_step": res_step * (4 + 21 * 4 + 4) + cfg["S"] * 4}}), flush=True)
@@ -906,7 +938,7 @@ def run_profile_case(args):
     16)."""
     from hikoboshi_b200 import DesignEngine, synthetic_backbone
     n = args.profile_proteins
-    eng = DesignEngine(WEIGHTS, device=0, precision=args.precision)
+    eng = DesignEngine(engine_weights(), device=0, precision=args.precision)
     if args.profile_workload == "score":
         cs, ss, toks = config4_inputs(0, synthetic_backbone)
         eng.score(cs[:n], ss[:n], toks[:n], seeds=3)
@@ -939,6 +971,13 @@ def main():
     ap.add_argument("--profile-proteins", type=int, default=16)
     ap.add_argument("--profile-seqs", type=int, default=32)
     args = ap.parse_args()
+    missing = reference_missing()
+    if missing and args.impl == "reference":
+        if dist_env()[0] == 0:
+            print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
+        return 0
+    if missing:
+        args.no_cpu_baseline = True
     if args.profile_case:
         return run_profile_case(args)
     if args.workload in SMALL:
